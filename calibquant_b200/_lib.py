@@ -63,6 +63,25 @@ class U8DecodeArgs(_c.Structure):
     ]
 
 
+class ChunkArgs(_c.Structure):
+    """Mirror of ``struct cq_chunk_args``."""
+
+    _fields_ = [
+        ("batch", _i32), ("n_q_heads", _i32), ("n_kv_heads", _i32), ("head_dim", _i32),
+        ("q_len", _i32), ("t_vis", _i32), ("t_fp", _i32), ("t_sys", _i32),
+        ("bits", _i32), ("group_size", _i32), ("dtype", _i32), ("reserved", _i32),
+        ("q", _vp), ("q_strides", _i64 * 3),
+        ("k_code", _vp), ("k_scale", _vp), ("k_mn", _vp),
+        ("v_code", _vp), ("v_scale", _vp), ("v_mn", _vp),
+        ("k_fp", _vp), ("v_fp", _vp),
+        ("fp_stride_b", _i64), ("fp_stride_h", _i64),
+        ("mask", _vp), ("mask_stride_b", _i64),
+        ("out", _vp), ("out_strides", _i64 * 3),
+        ("lse", _vp),
+        ("t_fp_dev", _vp),
+    ]
+
+
 # name -> (restype, argtypes); every symbol include/calibquant_b200.h declares.
 SIGNATURES = {
     "cq_version": (_c.c_int, []),
@@ -130,6 +149,14 @@ SIGNATURES = {
     "cq_decode_attn": (_c.c_int, [_c.POINTER(DecodeArgs), _vp, _sz, _vp]),
     "cq_decode_attn_profile": (_c.c_int, [_c.POINTER(DecodeArgs), _vp, _sz, _vp, _c.POINTER(_c.c_float)]),
     "cq_workspace_status": (_c.c_int, [_vp, _vp]),
+    "cq_chunk_attn_workspace_bytes": (_sz, [_c.POINTER(ChunkArgs)]),
+    "cq_chunk_attn": (_c.c_int, [_c.POINTER(ChunkArgs), _vp, _sz, _vp]),
+    "cq_key_weights_workspace_bytes": (_sz, [_c.POINTER(ChunkArgs)]),
+    "cq_key_weights": (_c.c_int, [_c.POINTER(ChunkArgs), _vp, _vp, _vp, _vp, _i64, _vp, _sz, _vp]),
+    "cq_evict_groups": (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int,
+                                   _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),
+    "cq_evict_tokens": (_c.c_int, [_vp, _vp, _i64, _i64, _vp, _i64, _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int,
+                                   _c.c_int, _vp, _vp, _vp, _vp, _vp]),
     "cq_host_status_word": (_c.POINTER(_c.c_int), []),
     "cq_qbmm_static_status": (_c.c_int, [_vp]),
     "cq_decode_attn_host_workspace_bytes": (_sz, [_c.POINTER(DecodeArgs)]),

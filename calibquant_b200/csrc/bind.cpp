@@ -771,12 +771,280 @@ PyObject* py_qjl_gqa_score(PyObject*, PyObject* const* a, Py_ssize_t n) {
   CQ_END
 }
 
+// ---- several new tokens on a cache; eviction ------------------------------------------------------------------------------
+void want_same(const Tensor& t, const Tensor& like, const char* what) {
+  if (t.scalar_type() == like.scalar_type() && t.device() == like.device()) return;
+  PyErr_Format(PyExc_ValueError, "%s must have the data type and the device of the queries", what);
+  throw PyRaised();
+}
+void want_size(const Tensor& t, at::IntArrayRef size, at::ScalarType dt, const Tensor& like, const char* what) {
+  if (t.sizes() == size && t.scalar_type() == dt && t.device() == like.device()) return;
+  PyErr_Format(PyExc_ValueError, "%s has another shape, data type or device than the cache it belongs to", what);
+  throw PyRaised();
+}
+bool aligned(const Tensor& t) { return reinterpret_cast<uintptr_t>(t.data_ptr()) % 16 == 0; }
+// contiguous and 16-byte aligned
+Tensor packed_rows(const Tensor& t) { return t.is_contiguous() && aligned(t) ? t : t.clone(at::MemoryFormat::Contiguous); }
+// A packed operand of T tokens: rows x [T of one channel] (keys) or rows x [the channels of a token] (values)
+void want_pack(Tensor (&p)[3], int64_t B, int64_t H, int64_t T, int64_t bits, bool keys, const Tensor& like, const char* what) {
+  const int64_t rows = keys ? 128 : T, len = keys ? T : 128;
+  want_size(p[0], {B, H, rows, len * bits / 32}, at::kInt, like, what);
+  for (int i : {1, 2}) want_size(p[i], {B, H, rows, len / 32}, like.scalar_type(), like, what);
+  for (auto& t : p) t = packed_rows(t);
+}
+
+struct Chunk {      // the arguments that both calls share, and what keeps their memory alive
+  cq_chunk_args d = {};
+  Tensor q, kp[3], vp[3], mask, k_fp, v_fp, live;
+};
+// a[] = q, k_pack, k_fp, t_sys, bits, group_size, mask, t_fp, t_fp_dev
+void chunk_common(Chunk& c, PyObject* q, PyObject* k_pack, PyObject* k_fp, PyObject* t_sys, PyObject* bits, PyObject* group_size,
+                  PyObject* mask, PyObject* t_fp, PyObject* live) {
+  need_cuda(tensor(q)); need_cuda(tensor(k_fp));
+  want_dims(tensor(q), 4, "q");
+  want_dims(tensor(k_fp), 4, "k_fp");
+  c.q = with_rows(tensor(q));
+  c.k_fp = tensor(k_fp);
+  const int64_t B = c.q.size(0), L = c.q.size(1), Hq = c.q.size(2), D = c.q.size(3), Hkv = c.k_fp.size(1);
+  if (Hq % divisor(Hkv, "the number of KV heads")) raise(PyExc_ValueError, "query heads must be a multiple of KV heads");
+  want_same(c.k_fp, c.q, "k_fp");
+  if (c.k_fp.size(0) != B || c.k_fp.size(3) != D) raise(PyExc_ValueError, "k_fp must be [B,Hkv,T,D] with q's batch and head dimension");
+  const int64_t cap = c.k_fp.size(2), n_fp = t_fp == Py_None ? cap : integer(t_fp);
+  if (n_fp < 0 || n_fp > cap) raise(PyExc_ValueError, "t_fp exceeds the cache");
+  if (L > n_fp) raise(PyExc_ValueError, "the new tokens' keys and values must be in the cache: q has more tokens than t_fp");
+  cq_chunk_args& d = c.d;
+  d.batch = (int32_t)B; d.n_q_heads = (int32_t)Hq; d.n_kv_heads = (int32_t)Hkv; d.head_dim = (int32_t)D;
+  d.q_len = (int32_t)L; d.t_fp = (int32_t)n_fp;
+  d.bits = (int32_t)integer(bits); d.group_size = (int32_t)integer(group_size); d.dtype = dtype_enum(c.q);
+  if (integer(t_sys) < 0) raise(PyExc_ValueError, "t_sys is negative");
+  d.t_sys = (int32_t)std::min<int64_t>(integer(t_sys), n_fp);
+  d.q = c.q.data_ptr();
+  for (int i = 0; i < 3; ++i) d.q_strides[i] = c.q.stride(i);
+  if (unpack3(k_pack, c.kp) && c.kp[0].numel() > 0) {
+    if (d.bits != 4 || d.group_size != 32 || D != 128) raise(PyExc_ValueError, "4-bit groups of 32 and a head dimension of 128 only");
+    want_dims(c.kp[0], 4, "a packed operand");
+    const int64_t T = c.kp[0].size(3) * 8;
+    if (T % 32) raise(PyExc_ValueError, "the visual span must be a multiple of 32 tokens");
+    want_pack(c.kp, B, Hkv, T, 4, true, c.q, "k_pack");
+    d.t_vis = (int32_t)T;
+    d.k_code = (const int32_t*)c.kp[0].data_ptr(); d.k_scale = c.kp[1].data_ptr(); d.k_mn = c.kp[2].data_ptr();
+  }
+  c.mask = opt_tensor(mask);
+  if (c.mask.defined()) {
+    need_cuda(c.mask);
+    if (c.mask.device() != c.q.device()) raise(PyExc_ValueError, "mask is on another device than q");
+    if (c.mask.numel() != B * (d.t_vis + n_fp)) {
+      PyErr_Format(PyExc_ValueError, "Attention mask should cover %lld keys of %lld rows", (long long)(d.t_vis + n_fp), (long long)B);
+      throw PyRaised();
+    }
+    c.mask = c.mask.reshape({B, d.t_vis + n_fp});
+    if (c.mask.scalar_type() != c.q.scalar_type() || c.mask.stride(1) != 1) c.mask = c.mask.to(c.q.scalar_type()).contiguous();
+    d.mask = c.mask.data_ptr(); d.mask_stride_b = c.mask.stride(0);
+  }
+  c.live = opt_tensor(live);
+  if (c.live.defined()) {
+    check_counter(c.live);
+    if (c.live.device() != c.q.device() || c.live.numel() < 1) raise(PyExc_ValueError, "t_fp_dev must be one number on q's device");
+    d.t_fp_dev = (const int32_t*)c.live.data_ptr();
+  }
+}
+// Rows of a full-precision cache as the kernels address them; other layouts are copied.
+void chunk_cache(Chunk& c, bool values) {
+  const auto ok = [](const Tensor& t) { return t.stride(3) == 1 && t.stride(2) == t.size(3) && t.stride(0) % 8 == 0 && t.stride(1) % 8 == 0 && aligned(t); };
+  if (!ok(c.k_fp) || (values && (!ok(c.v_fp) || c.k_fp.strides() != c.v_fp.strides()))) {
+    c.k_fp = c.k_fp.clone(at::MemoryFormat::Contiguous);
+    if (values) c.v_fp = c.v_fp.clone(at::MemoryFormat::Contiguous);
+  }
+  c.d.k_fp = c.k_fp.data_ptr();
+  if (values) c.d.v_fp = c.v_fp.data_ptr();
+  c.d.fp_stride_b = c.k_fp.stride(0); c.d.fp_stride_h = c.k_fp.stride(1);
+}
+
+// q, k_pack, v_pack, k_fp, v_fp, t_sys, bits, group_size, mask, out, t_fp, t_fp_dev, return_lse
+PyObject* py_chunk_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  CQ_BEGIN
+  want_args(n, 13, "chunk_attention");
+  Chunk c;
+  chunk_common(c, a[0], a[1], a[3], a[5], a[6], a[7], a[8], a[10], a[11]);
+  cq_chunk_args& d = c.d;
+  c.v_fp = tensor(a[4]);
+  need_cuda(c.v_fp);
+  want_size(c.v_fp, c.k_fp.sizes(), c.k_fp.scalar_type(), c.k_fp, "v_fp");
+  Call call(c.q);
+  chunk_cache(c, true);
+  if (d.t_vis) {
+    if (!unpack3(a[2], c.vp)) raise(PyExc_TypeError, "v_pack is missing");
+    want_pack(c.vp, d.batch, d.n_kv_heads, d.t_vis, 4, false, c.q, "v_pack");
+    d.v_code = (const int32_t*)c.vp[0].data_ptr(); d.v_scale = c.vp[1].data_ptr(); d.v_mn = c.vp[2].data_ptr();
+  }
+  Tensor out = opt_tensor(a[9]);
+  if (out.defined()) {
+    want_size(out, c.q.sizes(), c.q.scalar_type(), c.q, "out");
+    if (!rows_ok(out)) raise(PyExc_ValueError, "out must have contiguous channels, strides that are multiples of 8 and a 16-byte aligned start");
+  } else {
+    out = empty(c.q.sizes(), c.q);
+  }
+  d.out = out.data_ptr();
+  for (int i = 0; i < 3; ++i) d.out_strides[i] = out.stride(i);
+  const bool want_lse = truth(a[12]);
+  Tensor lse;
+  if (want_lse) {
+    lse = empty({d.batch, d.n_q_heads, d.q_len}, c.q, at::kFloat);
+    d.lse = lse.data_ptr<float>();
+  }
+  if (out.numel()) {
+    const size_t nbytes = cq_chunk_attn_workspace_bytes(&d);
+    if (nbytes == 0) {      // refused: the call itself says why
+      const int rc = cq_chunk_attn(&d, nullptr, 0, call.stream);
+      check(rc ? rc : CQ_ERR_WORKSPACE, "cq_chunk_attn");
+    }
+    const Tensor ws = workspace((int64_t)nbytes, c.q.get_device(), call.stream);
+    launch([&] { return cq_chunk_attn(&d, ws.data_ptr(), (size_t)ws.numel(), call.stream); }, "cq_chunk_attn");
+  }
+  return want_lse ? wrap2(out, lse) : wrap(out);
+  CQ_END
+}
+
+// a (visual, full-precision) pair of weights for these keys; false for None
+bool weight_pair(PyObject* o, Tensor (&w)[2], const Chunk& c, const char* what) {
+  if (o == Py_None) return false;
+  PyObject* seq = PySequence_Fast(o, "weights are a (visual, full-precision) pair");
+  if (!seq) throw PyRaised();
+  const bool ok = PySequence_Fast_GET_SIZE(seq) == 2 && THPVariable_Check(PySequence_Fast_GET_ITEM(seq, 0)) && THPVariable_Check(PySequence_Fast_GET_ITEM(seq, 1));
+  if (ok)
+    for (int i : {0, 1}) w[i] = THPVariable_Unpack(PySequence_Fast_GET_ITEM(seq, i));
+  Py_DECREF(seq);
+  if (!ok) raise(PyExc_ValueError, "weights are a (visual, full-precision) pair of tensors");
+  want_dims(w[1], 3, what);
+  want_size(w[0], {c.d.batch, c.d.n_kv_heads, c.d.t_vis}, at::kFloat, c.q, what);
+  want_size(w[1], {c.d.batch, c.d.n_kv_heads, w[1].size(2)}, at::kFloat, c.q, what);
+  if (w[1].size(2) < c.d.t_fp) raise(PyExc_ValueError, "the full-precision weights must cover t_fp keys");
+  return true;
+}
+
+// q, lse, k_pack, k_fp, t_sys, bits, group_size, mask, weights, out, t_fp, t_fp_dev
+PyObject* py_key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  CQ_BEGIN
+  want_args(n, 12, "key_weights");
+  Chunk c;
+  chunk_common(c, a[0], a[2], a[3], a[4], a[5], a[6], a[7], a[10], a[11]);
+  cq_chunk_args& d = c.d;
+  Call call(c.q);
+  chunk_cache(c, false);
+  need_cuda(tensor(a[1]));
+  want_size(tensor(a[1]), {d.batch, d.n_q_heads, d.q_len}, at::kFloat, c.q, "lse");
+  const Tensor lse = contiguous(tensor(a[1]));
+  d.lse = lse.data_ptr<float>();
+  Tensor in[2], out[2];
+  const bool given = weight_pair(a[8], in, c, "weights");
+  if (given)
+    for (auto& t : in) t = contiguous(t);
+  if (weight_pair(a[9], out, c, "out")) {
+    for (auto& t : out)
+      if (!t.is_contiguous()) raise(PyExc_ValueError, "out must be contiguous");
+    if (given && out[1].size(2) != in[1].size(2)) raise(PyExc_ValueError, "weights and out must have the same shapes");
+  } else {
+    out[0] = empty({d.batch, d.n_kv_heads, d.t_vis}, c.q, at::kFloat);
+    out[1] = empty({d.batch, d.n_kv_heads, given ? in[1].size(2) : d.t_fp}, c.q, at::kFloat);
+  }
+  if (d.batch > 0) {
+    const size_t nbytes = cq_key_weights_workspace_bytes(&d);
+    if (nbytes == 0) {
+      const int rc = cq_key_weights(&d, nullptr, nullptr, out[0].data_ptr<float>(), out[1].data_ptr<float>(), out[1].size(2), nullptr, 0, call.stream);
+      check(rc ? rc : CQ_ERR_WORKSPACE, "cq_key_weights");
+    }
+    const Tensor ws = workspace((int64_t)nbytes, c.q.get_device(), call.stream);
+    launch([&] { return cq_key_weights(&d, given ? in[0].data_ptr<float>() : nullptr, given ? in[1].data_ptr<float>() : nullptr, out[0].data_ptr<float>(),
+                          out[1].data_ptr<float>(), out[1].size(2), ws.data_ptr(), (size_t)ws.numel(), call.stream); }, "cq_key_weights");
+  }
+  return wrap2(out[0], out[1]);
+  CQ_END
+}
+
+PyObject* tuple_of(std::initializer_list<PyObject*> items) {
+  PyObject* tup = PyTuple_New((Py_ssize_t)items.size());
+  if (!tup) throw PyRaised();
+  Py_ssize_t i = 0;
+  for (PyObject* o : items) PyTuple_SET_ITEM(tup, i++, o);
+  return tup;
+}
+
+// k_pack, v_pack, weights, keep, bits, group_size
+PyObject* py_evict_groups(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  CQ_BEGIN
+  want_args(n, 6, "evict_groups");
+  Tensor kp[3], vp[3], ko[3], vo[3];
+  if (!unpack3(a[0], kp) || !unpack3(a[1], vp)) raise(PyExc_TypeError, "k_pack and v_pack are (code, scale, mn)");
+  need_cuda(tensor(a[2]));
+  const int64_t keep = integer(a[3]), bits = integer(a[4]), group = integer(a[5]);
+  if ((bits != 1 && bits != 2 && bits != 4) || group != 32) raise(PyExc_ValueError, "1, 2 or 4 bits in groups of 32 only");
+  want_dims(kp[1], 4, "a packed operand");
+  const int64_t B = kp[1].size(0), H = kp[1].size(1), D = kp[1].size(2), G = kp[1].size(3);
+  if (D != 128) raise(PyExc_ValueError, "a head dimension of 128 only");
+  if (keep <= 0 || keep > G) raise(PyExc_ValueError, "keep must be a number of groups between 1 and those there are");
+  (void)dtype_enum(kp[1]);
+  const Tensor like = kp[1];
+  Call call(like);
+  want_pack(kp, B, H, 32 * G, bits, true, like, "k_pack");
+  want_pack(vp, B, H, 32 * G, bits, false, like, "v_pack");
+  want_size(tensor(a[2]), {B, H, 32 * G}, at::kFloat, like, "weights");
+  const Tensor w = packed_rows(tensor(a[2]));
+  ko[0] = empty({B, H, D, keep * bits}, like, at::kInt);
+  vo[0] = empty({B, H, 32 * keep, 4 * bits}, like, at::kInt);
+  for (int i : {1, 2}) {
+    ko[i] = empty({B, H, D, keep}, like);
+    vo[i] = empty({B, H, 32 * keep, 4}, like);
+  }
+  const Tensor wo = empty({B, H, 32 * keep}, like, at::kFloat), kept = empty({B, H, keep}, like, at::kLong);
+  if (B * H)
+    launch([&] { return cq_evict_groups((const int32_t*)kp[0].data_ptr(), kp[1].data_ptr(), kp[2].data_ptr(), (const int32_t*)vp[0].data_ptr(), vp[1].data_ptr(),
+                           vp[2].data_ptr(), w.data_ptr<float>(), (int)B, (int)H, (int)D, (int)(32 * G), (int)keep, (int)bits, (int)group,
+                           (int32_t*)ko[0].data_ptr(), ko[1].data_ptr(), ko[2].data_ptr(), (int32_t*)vo[0].data_ptr(), vo[1].data_ptr(),
+                           vo[2].data_ptr(), wo.data_ptr<float>(), kept.data_ptr<int64_t>(), call.stream); }, "cq_evict_groups");
+  return tuple_of({wrap3(ko[0], ko[1], ko[2]), wrap3(vo[0], vo[1], vo[2]), wrap(wo), wrap(kept)});
+  CQ_END
+}
+
+// k_fp, v_fp, weights, keep, t_sys, recent, t_fp
+PyObject* py_evict_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
+  CQ_BEGIN
+  want_args(n, 7, "evict_tokens");
+  for (int i = 0; i < 3; ++i) need_cuda(tensor(a[i]));
+  Chunk c;
+  c.k_fp = tensor(a[0]); c.v_fp = tensor(a[1]);
+  want_dims(c.k_fp, 4, "k_fp");
+  (void)dtype_enum(c.k_fp);
+  want_size(c.v_fp, c.k_fp.sizes(), c.k_fp.scalar_type(), c.k_fp, "v_fp");
+  const int64_t B = c.k_fp.size(0), H = c.k_fp.size(1), cap = c.k_fp.size(2), D = c.k_fp.size(3), keep = integer(a[3]), sys = integer(a[4]),
+                recent = integer(a[5]), t_fp = a[6] == Py_None ? cap : integer(a[6]);
+  if (D != 128) raise(PyExc_ValueError, "a head dimension of 128 only");
+  if (t_fp < 0 || t_fp > cap) raise(PyExc_ValueError, "t_fp exceeds the cache");
+  if (keep <= 0 || keep > t_fp) raise(PyExc_ValueError, "keep must be a number of tokens between 1 and those there are");
+  if (sys < 0 || recent < 0 || sys > keep || recent > keep - sys) raise(PyExc_ValueError, "the system and recent tokens must fit into keep");
+  Call call(c.k_fp);
+  chunk_cache(c, true);
+  Tensor w = tensor(a[2]);
+  want_dims(w, 3, "weights");
+  want_size(w, {B, H, w.size(2)}, at::kFloat, c.k_fp, "weights");
+  if (w.size(2) < t_fp) raise(PyExc_ValueError, "the weights must cover t_fp tokens");
+  w = contiguous(w);
+  const Tensor ko = empty({B, H, keep, D}, c.k_fp), vo = empty({B, H, keep, D}, c.k_fp);
+  const Tensor wo = empty({B, H, keep}, c.k_fp, at::kFloat), kept = empty({B, H, keep}, c.k_fp, at::kLong);
+  if (B * H)
+    launch([&] { return cq_evict_tokens(c.k_fp.data_ptr(), c.v_fp.data_ptr(), c.k_fp.stride(0), c.k_fp.stride(1), w.data_ptr<float>(), w.size(2), (int)B, (int)H,
+                           (int)D, (int)t_fp, (int)keep, (int)sys, (int)recent, ko.data_ptr(), vo.data_ptr(), wo.data_ptr<float>(),
+                           kept.data_ptr<int64_t>(), call.stream); }, "cq_evict_tokens");
+  return tuple_of({wrap(ko), wrap(vo), wrap(wo), wrap(kept)});
+  CQ_END
+}
+
 #define CQ_FN(name) {#name, (PyCFunction)(void (*)(void))py_##name, METH_FASTCALL, nullptr}
 PyMethodDef methods[] = {
     CQ_FN(workspace), CQ_FN(workspaces_of), CQ_FN(refused), CQ_FN(pack_last_dim), CQ_FN(pack_k_per_channel), CQ_FN(pack_v_per_token),
     CQ_FN(quant_encode), CQ_FN(qbmm), CQ_FN(decode_attention), CQ_FN(u8_decode_attention), CQ_FN(rope_split_append), CQ_FN(linear_small), CQ_FN(small_ok), CQ_FN(heads_of),
     CQ_FN(prefill_rope_split), CQ_FN(prefill_attention),
-    CQ_FN(qjl_quant), CQ_FN(qjl_build), CQ_FN(qjl_gqa_score), {nullptr, nullptr, 0, nullptr}};
+    CQ_FN(qjl_quant), CQ_FN(qjl_build), CQ_FN(qjl_gqa_score), CQ_FN(chunk_attention), CQ_FN(key_weights),
+    CQ_FN(evict_groups), CQ_FN(evict_tokens), {nullptr, nullptr, 0, nullptr}};
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_native", "Tensor-level entry points over libcalibquant_b200.so.", -1, methods};
 
 }  // namespace

@@ -273,6 +273,46 @@ def prefill_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, out=Non
     return native().prefill_attention(q, k, v, out)
 
 
+def chunk_attention(q, k_pack, v_pack, k_fp, v_fp, t_sys, bits=4, group_size=32, mask=None, out=None, t_fp=None,
+                    t_fp_dev=None, return_lse=False):
+    """Attention of several new tokens over [sys | visual (4 bits) | text].
+
+    q [B,L,Hq,D] as :func:`prefill_rope_split` gives it; k_pack/v_pack = (code, scale, mn) as for
+    :func:`decode_attention`, or None; k_fp/v_fp [B,Hkv,T,D] hold the system tokens, the text tokens and, as the last
+    ``L`` of the first ``t_fp`` (default: all), the new tokens themselves.  A new token sees every visual token, and the
+    full-precision tokens up to itself.  ``mask``: optional additive [B, t_fp+T_vis] in key order [sys | visual | text]; a key at
+    -infinity takes no part whatever it holds, a row without keys gives zeros (and a log-sum-exp of -infinity).  Keys and values
+    in the cache that nobody may see need not be numbers, those of the new tokens have to be finite.  ``t_fp_dev``: int32
+    device scalar with the live token count; ``t_fp`` is then the capacity.  No logit calibration.
+    Returns o [B,L,Hq,D], with ``return_lse`` also the scores' log-sum-exp fp32 [B,Hq,L], which :func:`key_weights` takes.
+    """
+    return native().chunk_attention(q, k_pack, v_pack, k_fp, v_fp, t_sys, bits, group_size, mask, out, t_fp, t_fp_dev, return_lse)
+
+
+def key_weights(q, lse, k_pack, k_fp, t_sys, bits=4, group_size=32, mask=None, weights=None, out=None, t_fp=None, t_fp_dev=None):
+    """How much attention the queries of a :func:`chunk_attention` call paid to each key, summed over the queries and the query
+    heads of a KV head: fp32 (w_vis [B,Hkv,T_vis], w_fp [B,Hkv,T_fp]).  Arguments as there, ``lse`` as it was returned.
+
+    ``weights``: a pair that the sums are added to (its full-precision half may hold room for more than ``t_fp`` keys);
+    ``out``: the pair that receives the result, ``out=weights`` adds in place."""
+    return native().key_weights(q, lse, k_pack, k_fp, t_sys, bits, group_size, mask, weights, out, t_fp, t_fp_dev)
+
+
+def evict_groups(k_pack, v_pack, weights, keep, bits=4, group_size=32):
+    """Keep, per batch row and KV head, the ``keep`` groups of 32 visual tokens with the largest sum of ``weights`` [B,Hkv,T_vis]
+    (ties to the lowest index), packed as they are and in their order.
+    Returns (k_pack, v_pack, weights [B,Hkv,32*keep], kept int64 [B,Hkv,keep]).  Heads keep different tokens: a mask over the
+    visual tokens that tells them apart has no place any more."""
+    return native().evict_groups(k_pack, v_pack, weights, keep, bits, group_size)
+
+
+def evict_tokens(k_fp, v_fp, weights, keep, t_sys=0, recent=0, t_fp=None):
+    """Keep, per batch row and KV head, ``keep`` of the first ``t_fp`` (default: all) full-precision tokens [B,Hkv,T,D]: the first
+    ``t_sys``, the last ``recent`` and those with the largest ``weights`` [B,Hkv,>=t_fp] (ties to the lowest index).
+    Returns (k_fp [B,Hkv,keep,D], v_fp, weights [B,Hkv,keep], kept int64 [B,Hkv,keep])."""
+    return native().evict_tokens(k_fp, v_fp, weights, keep, t_sys, recent, t_fp)
+
+
 def prefill_rope_split(qkv, cos, sin, position_ids, n_kv_heads, n_rep, k_cache=None, v_cache=None,
                        vis_start=0, vis_len=0):
     """A whole prompt: split the ``wqkv`` output ``qkv`` [B,T,Hkv*(n_rep+2)*D], rotate queries and keys

@@ -496,6 +496,85 @@ int cq_qjl_gqa_score(const uint8_t* key_quant, const uint8_t* key_outlier_quant,
                      int outlier_sketch_dim, int outlier_count, int dtype, float* scores, void* stream);
 
 /*
+ * ---- several new tokens on a cache, and a cache that gives up keys --------------------------------------------
+ *
+ * No counterpart in the reference, whose forward takes one prompt and then one token at a time (patch_internvl.py:459-476, 556-592).
+ *
+ * cq_chunk_attn: attention of q_len new tokens over [system | visual (4-bit group format) | text].  The keys and values of the new
+ * tokens are the last q_len of the t_fp full-precision tokens.  Query i sees every visual token and the full-precision tokens
+ * t <= t_fp - q_len + i, the values of a packed operand being scale * code + mn:
+ *   s[i,k] = q_i . K_k / sqrt(128) + mask[k],   lse_i = log sum_k exp(s[i,k]),   out_i = sum_k exp(s[i,k] - lse_i) V_k
+ * A key whose mask is -infinity takes no part, whatever its key and value hold; a row without keys gives out 0, lse -infinity.
+ * The scores are exact but for their fp32 sums (packed keys are multiplied as two terms), values and probabilities are rounded to
+ * `dtype` for the second product.  No calibration of logits (calibrate = 0 of cq_decode_attn).
+ *   q, out  element (b,i,h,d) at base + b*strides[0] + i*strides[1] + h*strides[2] + d (strides in elements, multiples of 8)
+ *   lse     fp32 [B,Hq,q_len], or NULL
+ * bits == 4, group_size == 32, head_dim == 128, t_vis a multiple of 32 (0: no packed operands), 0 < q_len <= t_fp, every
+ * pointer 16-byte aligned (mask 2-byte), any number of query heads per KV head.
+ * The first word of the workspace is a sticky status word as in cq_decode_attn; two calls that overlap on the GPU need two workspaces.
+ */
+typedef struct cq_chunk_args {
+  int32_t batch, n_q_heads, n_kv_heads, head_dim;
+  int32_t q_len, t_vis, t_fp, t_sys;
+  int32_t bits, group_size, dtype, reserved;        /* reserved must be 0 */
+  const void* q;
+  int64_t q_strides[3];                             /* batch row, token, head */
+  const int32_t* k_code;                            /* packed operands, layouts as in cq_decode_args */
+  const void* k_scale;
+  const void* k_mn;
+  const int32_t* v_code;
+  const void* v_scale;
+  const void* v_mn;
+  const void* k_fp;                                 /* token (b,h,t,:) at base + b*fp_stride_b + h*fp_stride_h + t*128 */
+  const void* v_fp;
+  int64_t fp_stride_b, fp_stride_h;
+  const void* mask;                                 /* optional additive mask [B, t_fp + t_vis] in `dtype`, key order */
+  int64_t mask_stride_b;                            /* [sys | visual | text]; NULL = none                             */
+  void* out;
+  int64_t out_strides[3];
+  float* lse;
+  const int32_t* t_fp_dev;                          /* optional device counter of live fp tokens, as in cq_decode_args: */
+                                                    /* t_fp is then the capacity; fewer than q_len live tokens: the     */
+                                                    /* first queries see no full-precision token                       */
+} cq_chunk_args;
+size_t cq_chunk_attn_workspace_bytes(const cq_chunk_args* args);
+int cq_chunk_attn(const cq_chunk_args* args, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * cq_key_weights: how much attention those queries paid to each key, summed over the queries and the query heads of a KV head:
+ *   w[b,hk,k] = w_in[b,hk,k] + sum over i and the heads h of hk of exp(s[i,k] - lse[b,h,i])        (s as above)
+ * with the lse that cq_chunk_attn gave.  A row whose lse is -infinity adds nothing.
+ *   args       as for cq_chunk_attn; v_code .. v_mn, v_fp, out are not used, lse is read
+ *   w_vis      fp32 [B,Hkv,t_vis]; w_fp fp32 [B,Hkv,w_capacity] with w_capacity >= t_fp: rows of keys that are not live keep w_in
+ *   *_in       the same shapes, may be the outputs themselves, or NULL: zeros
+ * Sums are fp32, in an order that depends on the sizes alone.
+ */
+size_t cq_key_weights_workspace_bytes(const cq_chunk_args* args);
+int cq_key_weights(const cq_chunk_args* args, const float* w_vis_in, const float* w_fp_in, float* w_vis, float* w_fp,
+                   int64_t w_capacity, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * cq_evict_groups: per (batch row, KV head) the `keep` groups of 32 visual tokens with the largest sum of weights (64-bit sums; ties to
+ * the lowest index; NaN counts as the largest) stay, in their order, as they are packed.
+ *   in   K code [B,H,D,t_vis*bits/32], scale, mn [B,H,D,t_vis/32]; V code [B,H,t_vis,D*bits/32], scale, mn [B,H,t_vis,4]; weights
+ *        fp32 [B,H,t_vis]
+ *   out  the same with 32*keep tokens; kept int64 [B,H,keep], ascending.  Outputs must not overlap inputs.
+ * bits in {1,2,4}, group_size 32, head_dim 128, 0 < keep <= t_vis/32 <= 16384, pointers 16-byte aligned.
+ *
+ * cq_evict_tokens: the same for single full-precision tokens: of t_fp tokens the first t_sys and the last `recent` stay whatever
+ * their weight, and those with the largest weights fill up to `keep`.
+ *   k, v     token (b,h,t,:) at base + b*stride_b + h*stride_h + t*128; weights fp32, row (b,h) at weights + (b*H + h)*w_stride
+ *   k_out, v_out [B,H,keep,128], w_out [B,H,keep], kept int64 [B,H,keep].  t_fp <= 24576.
+ */
+int cq_evict_groups(const int32_t* k_code, const void* k_scale, const void* k_mn, const int32_t* v_code, const void* v_scale,
+                    const void* v_mn, const float* weights, int batch, int heads, int head_dim, int t_vis, int keep, int bits,
+                    int group_size, int32_t* k_code_out, void* k_scale_out, void* k_mn_out, int32_t* v_code_out, void* v_scale_out,
+                    void* v_mn_out, float* w_out, int64_t* kept, void* stream);
+int cq_evict_tokens(const void* k, const void* v, int64_t stride_b, int64_t stride_h, const float* weights, int64_t w_stride,
+                    int batch, int heads, int head_dim, int t_fp, int keep, int t_sys, int recent, void* k_out, void* v_out,
+                    float* w_out, int64_t* kept, void* stream);
+
+/*
  * Sticky device status of the prefill kernel (no reference counterpart: the reference checks no
  * CUDA errors).  0, or CQ_ERR_TIMEOUT if one of its bounded barrier waits ever ran out on the
  * current device.  Synchronises the device.
