@@ -1,136 +1,607 @@
-// Attention of several new tokens over [system | visual (4-bit group format) | text], and what each key got of it: the simplest
-// form of both.  A warp per query row (attention) or per eight keys (weights); a lane holds four channels; scores are summed over
-// the lanes; softmax with a running maximum and sum.  All arithmetic in fp32.
+// Attention of several new tokens over [system | visual (4-bit group format) | text] on the 5th-generation tensor cores.
+//
+// Rows are (query, head) pairs of one KV head, query major.  A CTA works on one KV head of one request with two 128-row tiles A and B
+// (a TMEM lane per row):
+//   PAIR    A and B are adjacent rows and share every key tile (more than 128 rows);
+//   else    A and B are the SAME rows and take the even and the odd key tiles, two partial results.
+// The keys of a CTA are a part of the request's key tiles, visual ones first (`parts` on the grid); partial results are merged by
+// combine_kernel.  Roles:
+//   warps 0-3 / 4-7  softmax of A / B: thread = row; running maximum and sum, probabilities back to tensor memory
+//   warps 8-15       operands: codes from global memory (requested a tile ahead), unpacked into 16-bit tiles in a ring of five
+//                    shared-memory slots; full-precision rows into the same layout
+//   warp 16          issues the products
+// S = Q K^T with packed keys as two 16-bit terms (their sum is scale * code + minimum exactly), so scores carry no rounding but
+// that of fp32 sums; O += P V with P in tensor memory.  S_A [0,128) S_B [128,256) O_A [256,384) O_B [384,512) TMEM columns.
+// Every wait is bounded; one that runs out sets CQ_ERR_TIMEOUT in the workspace's first word, and the CTA ends.
 #include <math.h>
 
-#include "cq_chunk.cuh"
+#include "cq_chunk_tc.cuh"
 
 namespace cq {
 namespace chunk {
 
-constexpr int WARPS = 8;
+using namespace ptx;
+using namespace tc;
 
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, float (&v)[4]) {
-  const uint2 w = *reinterpret_cast<const uint2*>(p);
-  using T2 = typename Elem<T>::T2;
-  const float2 a = Elem<T>::to_f2(*reinterpret_cast<const T2*>(&w.x)), b = Elem<T>::to_f2(*reinterpret_cast<const T2*>(&w.y));
-  v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+constexpr int SLOTS = 5;
+constexpr int PRODUCERS = 8, MMA_WARP = 16, THREADS = 17 * 32;
+constexpr int SMEM_BYTES = (2 + SLOTS) * TILE_BYTES + 1024;
+constexpr uint32_t WAIT_TRIES = 1u << 22;
+constexpr long long WAIT_CYCLES = 1ll << 30;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct AttnParams {
+  Params p;
+  int parts;                 // partial results per row (1: the kernel writes the output itself)
+  float scale;               // 1 / sqrt(128)
+  uint32_t idesc_kmajor, idesc_mn;
+  float* part_o;             // [batch][KV head][row][part][128]
+  float2* part_ml;           // [batch][KV head][row][part]: maximum and sum
+  int* status;
+};
+
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
+__device__ __forceinline__ float max3(float a, float b, float c) {
+  float d;
+  asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+  return d;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  uint32_t r;
+  if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+__device__ __forceinline__ void tile_barrier(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
 
-// Keys key0 .. key0+7 in cache order [visual | fp], this lane's channels 4*lane .. +3; keys past the end are zeros.
-template <typename T>
-__device__ __forceinline__ void load_keys(const Params& p, int b, int hk, int key0, int n_keys, int lane, float (&k)[8][4]) {
-  if (key0 < p.t_vis) {
-    const int64_t row = ((int64_t)b * p.hkv + hk) * 128 + lane * 4;
-    for (int c = 0; c < 4; ++c) {
-      const uint32_t w = p.k_code[(row + c) * (p.t_vis / 8) + key0 / 8];
-      const float s = Elem<T>::to_f(static_cast<const T*>(p.k_scale)[(row + c) * (p.t_vis / 32) + key0 / 32]);
-      const float m = Elem<T>::to_f(static_cast<const T*>(p.k_mn)[(row + c) * (p.t_vis / 32) + key0 / 32]);
-      for (int j = 0; j < 8; ++j) k[j][c] = fmaf((float)((w >> (4 * j)) & 15u), s, m);
-    }
-  } else {
-    for (int j = 0; j < 8; ++j) {
-      if (key0 + j < n_keys)
-        load4(static_cast<const T*>(p.k_fp) + b * p.fp_sb + hk * p.fp_sh + (int64_t)(key0 + j - p.t_vis) * 128 + lane * 4, k[j]);
-      else
-        for (int c = 0; c < 4; ++c) k[j][c] = 0.f;
-    }
+// Ring position of a role: slot and how often it has come round.
+struct Ring {
+  uint32_t slot = 0, round = 0;
+  __device__ __forceinline__ void next() {
+    if (++slot == SLOTS) { slot = 0; ++round; }
   }
-}
+};
 
-// logits of a row against eight keys; -inf where a key takes no part
-template <typename T>
-__device__ __forceinline__ void logits(const Params& p, int b, int key0, int limit, const float (&q)[4], const float (&k)[8][4], float (&s)[8]) {
-  for (int j = 0; j < 8; ++j) {
-    float x = q[0] * k[j][0] + q[1] * k[j][1] + q[2] * k[j][2] + q[3] * k[j][3];
-    x = warp_sum(x) * 0.08838834764831845f;
-    const int key = key0 + j;
-    if (key >= limit) {
-      x = -INFINITY;
-    } else if (p.mask) {
-      const float m = Elem<T>::to_f(static_cast<const T*>(p.mask)[b * p.mask_sb + mask_index(p, key)]);
-      x = m == -INFINITY ? -INFINITY : x + m;
+// Key tiles of a CTA: visual tiles [0, nv), full-precision ones [nv, n_all); this CTA's are [t0, t0 + n).
+struct Range {
+  int nv, t0, n;
+};
+
+template <bool BF16, bool MASK, bool PAIR>
+__global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_constant__ AttnParams a) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  const Params& p = a.p;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t q_s = smem_u32(smem), ring_s = q_s + 2 * TILE_BYTES;
+  // bar_q (once); bar_full/free[slot]; bar_s[X] scores of X ready; bar_p[X][half] probabilities of keys 0-63 / 64-127 stored;
+  // bar_pv[X] the tile's P V done
+  __shared__ __align__(8) uint64_t bar_q, bar_full[SLOTS], bar_free[SLOTS], bar_s[2], bar_p[2][2], bar_pv[2];
+  __shared__ uint32_t tmem_base_s;
+  __shared__ __align__(16) T mask_s[MASK ? 2 : 1][MASK ? 2 : 1][MASK ? 128 : 8];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int hk = blockIdx.y % p.hkv, b = blockIdx.y / p.hkv, part = blockIdx.z;
+  const int64_t bh = (int64_t)b * p.hkv + hk;
+  const int row0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * (PAIR ? 256 : 128);      // rows that see most keys first
+
+  if (tid == 0) {
+    mbar_init(&bar_q, PRODUCERS);
+    for (int s = 0; s < SLOTS; ++s) {
+      mbar_init(&bar_full[s], PRODUCERS);
+      mbar_init(&bar_free[s], 1);
     }
-    s[j] = x;
+    for (int x = 0; x < 2; ++x) {
+      mbar_init(&bar_s[x], 1);
+      mbar_init(&bar_p[x][0], 128);
+      mbar_init(&bar_p[x][1], 128);
+      mbar_init(&bar_pv[x], 1);
+    }
+    mbar_fence_init();
   }
-}
+  pdl_launch_dependents();
+  const int live = live_tokens(p);
+  if (warp == MMA_WARP) tmem_alloc(&tmem_base_s, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_s;
 
-template <typename T>
-__global__ void __launch_bounds__(WARPS * 32) chunk_rows_kernel(Params p) {
-  const int lane = threadIdx.x & 31, row = blockIdx.x * WARPS + (threadIdx.x >> 5), hk = blockIdx.y, b = blockIdx.z;
-  if (row >= p.rows) return;
-  const int i = row / p.n_rep, h = hk * p.n_rep + row % p.n_rep;
-  float q[4];
-  load4(static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_st + h * p.q_sh + lane * 4, q);
-  const int limit = p.t_vis + max(0, live_tokens(p) - p.q_len + i + 1);
-  float m = -INFINITY, l = 0.f, o[4] = {};
-  for (int key0 = 0; key0 < limit; key0 += 8) {
-    float k[8][4], s[8];
-    load_keys<T>(p, b, hk, key0, limit, lane, k);
-    logits<T>(p, b, key0, limit, q, k, s);
-    float top = m;
-    for (int j = 0; j < 8; ++j) top = fmaxf(top, s[j]);
-    if (top == -INFINITY) continue;
-    const float a = expf(m - top);
-    l *= a;
-    for (int c = 0; c < 4; ++c) o[c] *= a;
-    m = top;
-    for (int j = 0; j < 8; ++j) {
-      if (s[j] == -INFINITY) continue;
-      const float pr = expf(s[j] - m);
-      const int key = key0 + j;
-      float v[4];
-      if (key < p.t_vis) {
-        const int64_t tok = ((int64_t)b * p.hkv + hk) * p.t_vis + key;
-        const uint32_t w = p.v_code[tok * 16 + lane / 2] >> (16 * (lane & 1));
-        const float sc = Elem<T>::to_f(static_cast<const T*>(p.v_scale)[tok * 4 + lane / 8]);
-        const float mn = Elem<T>::to_f(static_cast<const T*>(p.v_mn)[tok * 4 + lane / 8]);
-        for (int c = 0; c < 4; ++c) v[c] = fmaf((float)((w >> (4 * c)) & 15u), sc, mn);
-      } else {
-        load4(static_cast<const T*>(p.v_fp) + b * p.fp_sb + hk * p.fp_sh + (int64_t)(key - p.t_vis) * 128 + lane * 4, v);
+  Range k;
+  {
+    const int last = min(row0 + (PAIR ? 256 : 128), p.rows) - 1;
+    const int n_fp = max(0, live - p.q_len + last / p.n_rep + 1);      // full-precision tokens that the last row sees
+    k.nv = (p.t_vis + 127) >> 7;
+    const int n_all = k.nv + ((n_fp + 127) >> 7), grid_parts = gridDim.z, per = (n_all + grid_parts - 1) / grid_parts;
+    k.t0 = min(n_all, part * per);
+    k.n = min(n_all, k.t0 + per) - k.t0;
+  }
+
+  if (warp >= 8 && warp < MMA_WARP) {
+    // ================= operands =================
+    const int pw = warp - 8, ptid = tid - 256;
+    bool ok = true;
+    // the queries; rows past the end are zeros
+    for (int x = 0; x < (PAIR ? 2 : 1); ++x) {
+#pragma unroll 4
+      for (int it = 0; it < 8; ++it) {
+        const int r = it * 16 + (ptid >> 4), c = ptid & 15, row = row0 + x * 128 + r;
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (row < p.rows) {
+          const int i = row / p.n_rep, h = hk * p.n_rep + row % p.n_rep;
+          v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_st + h * p.q_sh + c * 8);
+        }
+        sts128(chunk_at(q_s + x * TILE_BYTES, r, c), v.x, v.y, v.z, v.w);
       }
-      l += pr;
-      for (int c = 0; c < 4; ++c) o[c] = fmaf(pr, v[c], o[c]);
+    }
+    fence_proxy_async_smem();
+    __syncwarp();
+    if (lane == 0) mbar_arrive(&bar_q);
+
+    Unit ku[2], vu[2];
+    // whether a key's mask lets it take part (its values are not looked at otherwise)
+    const auto taken = [&](int key) {
+      return !MASK || Elem<T>::to_f(static_cast<const T*>(p.mask)[b * p.mask_sb + mask_index(p, key)]) != -INFINITY;
+    };
+    const auto request_k = [&](int j) {
+      const int tile = k.t0 + j;
+      if (j < k.n && tile < k.nv) {
+        load_k_unit(p, bh, tile, pw, lane, ku[0]);
+        load_k_unit(p, bh, tile, pw + 8, lane, ku[1]);
+      }
+    };
+    const auto request_v = [&](int j) {
+      const int tile = k.t0 + j;
+      if (j < k.n && tile < k.nv) {
+        for (int u = 0; u < 2; ++u) {
+          const int key = tile * 128 + (pw + 8 * u) * 8 + (lane >> 2);
+          load_v_unit(p, bh, tile, pw + 8 * u, lane, key < p.t_vis && taken(key), vu[u]);
+        }
+      }
+    };
+    Ring ring;
+    const auto wait_free = [&]() {
+      if (ok && ring.round > 0) ok = mbar_wait_bounded(&bar_free[ring.slot], (ring.round - 1) & 1, WAIT_TRIES);
+      ok = __all_sync(0xffffffffu, ok);
+    };
+    const auto publish = [&](uint32_t slot) {
+      if (lane == 0) mbar_arrive(&bar_full[slot]);
+    };
+    const auto fp_tile = [&](const void* base, int tile, bool values) {      // into the ring's slot
+      const T* src = static_cast<const T*>(base) + b * p.fp_sb + hk * p.fp_sh;
+      const int t_first = (tile - k.nv) * 128;
+      const uint32_t dst = ring_s + ring.slot * TILE_BYTES;
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint4 v[4];
+#pragma unroll
+        for (int it = 0; it < 4; ++it) {
+          const int t = t_first + (half * 4 + it) * 16 + (ptid >> 4);
+          v[it] = make_uint4(0, 0, 0, 0);
+          if (t < live && (!values || taken(p.t_vis + t))) v[it] = *reinterpret_cast<const uint4*>(src + (int64_t)t * 128 + (ptid & 15) * 8);
+          if (values) order_values(v[it]);
+        }
+#pragma unroll
+        for (int it = 0; it < 4; ++it)
+          sts128(chunk_at(dst, (half * 4 + it) * 16 + (ptid >> 4), ptid & 15), v[it].x, v[it].y, v[it].z, v[it].w);
+      }
+    };
+    const auto produce_k = [&](int j) {
+      const int tile = k.t0 + j;
+      wait_free();
+      if (tile < k.nv) {
+        const uint32_t hi = ring.slot;
+        ring.next();
+        wait_free();
+        if (!ok) return;
+        const uint32_t lo = ring.slot;
+        store_k_unit<BF16>(ring_s + hi * TILE_BYTES, ring_s + lo * TILE_BYTES, ku[0], pw, lane);
+        store_k_unit<BF16>(ring_s + hi * TILE_BYTES, ring_s + lo * TILE_BYTES, ku[1], pw + 8, lane);
+        request_k(j + 1);
+        fence_proxy_async_smem();
+        __syncwarp();
+        publish(hi);
+        publish(lo);
+      } else {
+        if (!ok) return;
+        fp_tile(p.k_fp, tile, false);
+        fence_proxy_async_smem();
+        __syncwarp();
+        publish(ring.slot);
+      }
+      ring.next();
+    };
+    const auto produce_v = [&](int j) {
+      const int tile = k.t0 + j;
+      wait_free();
+      if (!ok) return;
+      if (tile < k.nv) {
+        store_v_unit<BF16>(ring_s + ring.slot * TILE_BYTES, vu[0], pw, lane);
+        store_v_unit<BF16>(ring_s + ring.slot * TILE_BYTES, vu[1], pw + 8, lane);
+        request_v(j + 1);
+      } else {
+        fp_tile(p.v_fp, tile, true);
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      publish(ring.slot);
+      ring.next();
+    };
+    request_k(0);
+    request_v(0);
+    // the order in which the issuer first touches them
+    if (!PAIR && k.n > 0) produce_k(0);
+    for (int j = 0; j < k.n && ok; ++j) {
+      if (PAIR) produce_k(j);
+      else if (j + 1 < k.n) produce_k(j + 1);
+      if (ok) produce_v(j);
+    }
+    if (!ok && lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
+  } else if (warp == MMA_WARP) {
+    // ================= products =================
+    // the whole warp runs the loop and one elected lane issues: control flow and operands are uniform
+    const uint32_t lead = elect_one();
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    constexpr uint64_t tile16 = TILE_BYTES >> 4;
+    const uint64_t qd = smem_desc(q_s, 16, 1024), kd = smem_desc(ring_s, 16, 1024), md = smem_desc(ring_s, PANEL_BYTES, 1024);
+    bool ok = true;
+    const auto all = [](bool r) { return __all_sync(0xffffffffu, r) != 0; };
+    Ring ring;
+    const auto acquire = [&]() {
+      ok = ok && all(mbar_wait_bounded(&bar_full[ring.slot], ring.round & 1, WAIT_TRIES));
+      const uint32_t s = ring.slot;
+      ring.next();
+      return s;
+    };
+    const auto commit = [&](uint64_t* bar) { if (lead) umma_commit(bar); };
+    uint32_t hi = 0, lo = 0;                  // slots of the key tile at hand; hi == lo: full precision
+    const auto take_k = [&](int j) {
+      hi = lo = acquire();
+      if (k.t0 + j < k.nv) lo = acquire();
+      tc_fence_after();
+    };
+    const auto issue_s = [&](int x) {         // S_x = Q_x K^T
+      if (!lead) return;
+      const uint32_t d = tm + (uint32_t)x * 128u;
+      const uint64_t q = qd + (PAIR && x ? tile16 : 0);
+      if (hi != lo) {
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          const uint64_t qo = (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
+          umma(d, q + qo, md + hi * tile16 + (uint64_t)(ks * 128), a.idesc_mn, ks > 0);
+        }
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          const uint64_t qo = (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
+          umma(d, q + qo, md + lo * tile16 + (uint64_t)(ks * 128), a.idesc_mn, 1);
+        }
+      } else {
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          const uint64_t qo = (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
+          umma(d, q + qo, kd + hi * tile16 + qo, a.idesc_kmajor, ks > 0);
+        }
+      }
+      umma_commit(&bar_s[x]);
+    };
+    const auto free_k = [&]() {
+      commit(&bar_free[hi]);
+      if (lo != hi) commit(&bar_free[lo]);
+    };
+    // O_x += P_x V, the probabilities of keys 0-63 first
+    const auto pv = [&](int x, uint32_t v, int count) {
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        ok = ok && all(mbar_wait_cycles(&bar_p[x][half], count & 1, WAIT_CYCLES));
+        if (!ok) return;
+        tc_fence_after();
+        if (lead) {
+#pragma unroll
+          for (int ks = 4 * half; ks < 4 * half + 4; ++ks)
+            umma_ts(tm + 256u + (uint32_t)x * 128u, tm + (uint32_t)x * 128u + (uint32_t)ks * 8u, md + v * tile16 + (uint64_t)(ks * 128), a.idesc_mn,
+                    (ks > 0 || count > 0) ? 1u : 0u);
+        }
+      }
+      commit(&bar_pv[x]);
+    };
+    ok = all(mbar_wait_bounded(&bar_q, 0, WAIT_TRIES));
+    if (PAIR) {
+      if (k.n > 0) {
+        take_k(0);
+        if (ok) { issue_s(0); issue_s(1); free_k(); }
+      }
+      for (int j = 0; j < k.n && ok; ++j) {
+        const uint32_t v = acquire();
+        const bool more = j + 1 < k.n;
+        if (ok) pv(0, v, j);
+        if (more && ok) take_k(j + 1);
+        if (more && ok) issue_s(0);
+        if (ok) pv(1, v, j);
+        if (ok) commit(&bar_free[v]);
+        if (more && ok) { issue_s(1); free_k(); }
+      }
+    } else {
+      for (int j = 0; j < min(2, k.n) && ok; ++j) {
+        take_k(j);
+        if (ok) { issue_s(j); free_k(); }
+      }
+      for (int j = 0; j < k.n && ok; ++j) {
+        const uint32_t v = acquire();
+        if (ok) pv(j & 1, v, j >> 1);
+        if (ok) commit(&bar_free[v]);
+        if (j + 2 < k.n && ok) take_k(j + 2);
+        if (j + 2 < k.n && ok) { issue_s(j & 1); free_k(); }
+      }
+    }
+    if (!ok && lead) atomicExch(a.status, CQ_ERR_TIMEOUT);
+    __syncwarp();
+  } else if (warp < 8) {
+    // ================= softmax: thread = row =================
+    const int x = warp >> 2, quarter = warp & 3, r_in = quarter * 32 + lane;
+    const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
+    const uint32_t tS = tmem + (uint32_t)x * 128u + lane_off, tO = tmem + 256u + (uint32_t)x * 128u + lane_off;
+    const int row = row0 + (PAIR ? x * 128 : 0) + r_in, i = row / p.n_rep;
+    const int limit = live - p.q_len + i + 1;                     // full-precision tokens that the row sees
+    const int n_x = PAIR ? k.n : (k.n + 1 - x) >> 1;
+    // Units: without a mask, scores as the tensor core gives them times `factor` are powers of two; with one they are scaled and
+    // masked first (a mask of the type's lowest value times log2 e would leave fp32's range).
+    const float factor = MASK ? LOG2E : a.scale * LOG2E;
+    bool ok = true;
+    float m_ref = -INFINITY, l_run = 0.f;
+    const auto mask_of = [&](int j) {                              // of column r_in of this tile's j-th key tile
+      const int tile = k.t0 + (PAIR ? j : 2 * j + x);
+      const int key = tile < k.nv ? tile * 128 + r_in : p.t_vis + (tile - k.nv) * 128 + r_in;
+      if (j >= n_x || (tile < k.nv ? key >= p.t_vis : key - p.t_vis >= live)) return Elem<T>::from_f(-INFINITY);
+      return static_cast<const T*>(p.mask)[b * p.mask_sb + mask_index(p, key)];
+    };
+    T mask_next = MASK ? mask_of(0) : Elem<T>::from_f(0.f);
+    for (int j = 0; j < n_x; ++j) {
+      const int tile = k.t0 + (PAIR ? j : 2 * j + x);
+      const int lim = min(128, tile < k.nv ? p.t_vis - tile * 128 : limit - (tile - k.nv) * 128);      // columns from lim on are not seen
+      const T* mk = mask_s[MASK ? x : 0][MASK ? j & 1 : 0];
+      if (MASK) {
+        mask_s[x][j & 1][r_in] = mask_next;
+        mask_next = mask_of(j + 1);
+        tile_barrier(1 + x);
+      }
+      const bool need = __any_sync(0xffffffffu, lim < 128);
+      if (ok) ok = mbar_wait_cycles(&bar_s[x], j & 1, WAIT_CYCLES);
+      tc_fence_after();
+      const auto scores = [&](int cc, uint32_t (&s)[32]) {         // 32 of them
+        tmem_ld32(tS + cc * 32, s);
+        if (MASK) {
+#pragma unroll
+          for (int c = 0; c < 32; c += 4) {
+            const uint2 m4 = *reinterpret_cast<const uint2*>(mk + cc * 32 + c);
+            const uint16_t m16[4] = {(uint16_t)m4.x, (uint16_t)(m4.x >> 16), (uint16_t)m4.y, (uint16_t)(m4.y >> 16)};
+            const float m[4] = {number<BF16>(m16[0]), number<BF16>(m16[1]), number<BF16>(m16[2]), number<BF16>(m16[3])};
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              s[c + e] = m[e] == -INFINITY ? 0xff800000u : __float_as_uint(fmaf(__uint_as_float(s[c + e]), a.scale, m[e]));
+          }
+        }
+        if (need) {
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (cc * 32 + c >= lim) s[c] = 0xff800000u;
+        }
+      };
+      float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int cc = 0; cc < 4; ++cc) {
+        uint32_t s[32];
+        scores(cc, s);
+#pragma unroll
+        for (int c = 0; c < 32; c += 2) mx4[(c >> 1) & 3] = max3(mx4[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+      }
+      const float m_true = fmaxf(m_ref, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
+      // a row keeps its reference until the true maximum is 2^8 above it (probabilities stay below 256), or for the first time
+      const bool grow = (m_true - m_ref) * factor > 8.f;
+      if (j > 0 && __any_sync(0xffffffffu, grow)) {
+        if (ok) ok = mbar_wait_bounded(&bar_pv[x], (j - 1) & 1, WAIT_TRIES);
+        tc_fence_after();
+        const float alpha = grow ? exp2f((m_ref - m_true) * factor) : 1.f;
+#pragma unroll 1
+        for (int cc = 0; cc < 4; ++cc) {
+          uint32_t r[32];
+          tmem_ld32(tO + cc * 32, r);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(__uint_as_float(r[c]) * alpha);
+          tmem_st32(tO + cc * 32, r);
+        }
+        l_run *= alpha;
+      }
+      if (grow) m_ref = m_true;
+      const float m_use = m_ref == -INFINITY ? 0.f : m_ref, neg = -m_use * factor;
+      float rs[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        uint32_t w[32];
+#pragma unroll
+        for (int cc = 0; cc < 2; ++cc) {
+          uint32_t s[32];
+          scores(half * 2 + cc, s);
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) {
+            float e0, e1;
+            if (MASK) {
+              e0 = ex2_approx((__uint_as_float(s[c]) - m_use) * factor);
+              e1 = ex2_approx((__uint_as_float(s[c + 1]) - m_use) * factor);
+            } else {
+              e0 = ex2_approx(fmaf(__uint_as_float(s[c]), factor, neg));
+              e1 = ex2_approx(fmaf(__uint_as_float(s[c + 1]), factor, neg));
+            }
+            rs[c & 2] += e0;
+            rs[(c & 2) + 1] += e1;
+            w[cc * 16 + (c >> 1)] = pack16<BF16>(e0, e1);
+          }
+        }
+        tmem_st32(tS + half * 32, w);               // over scores that have been read
+        tmem_st_wait();
+        tc_fence_before();
+        mbar_arrive(&bar_p[x][half]);
+      }
+      l_run += (rs[0] + rs[1]) + (rs[2] + rs[3]);
+    }
+    if (n_x > 0 && ok) ok = mbar_wait_bounded(&bar_pv[x], (n_x - 1) & 1, WAIT_TRIES);
+    ok = __all_sync(0xffffffffu, ok);
+    if (!ok && lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
+    tc_fence_after();
+    const int h = hk * p.n_rep + row % p.n_rep;
+    const float nat = MASK ? 1.f : a.scale;         // reference maximum in natural units
+    if (a.parts == 1) {
+      // the tile's rows through its query tile in shared memory (no product reads that any more), then 16 lanes a row
+      const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+      if (ok && row < p.rows && p.lse)
+        p.lse[((int64_t)b * p.hq + h) * p.q_len + i] = l_run > 0.f ? m_ref * nat + logf(l_run) : -INFINITY;
+      const uint32_t stage = q_s + (uint32_t)x * TILE_BYTES;
+      if (ok) {
+#pragma unroll 1
+        for (int cc = 0; cc < 4; ++cc) {
+          uint32_t r[32];
+          if (n_x > 0) tmem_ld32(tO + cc * 32, r);
+#pragma unroll
+          for (int c = 0; c < 32; ++c) r[c] = n_x > 0 ? __float_as_uint(__uint_as_float(r[c]) * inv) : 0u;
+#pragma unroll
+          for (int c = 0; c < 32; c += 8) {         // columns 0 4 1 5 2 6 3 7 of eight channels
+            const auto f = [&](int e) { return __uint_as_float(r[c + e]); };
+            sts128(chunk_at(stage, r_in, cc * 4 + (c >> 3)), pack16<BF16>(f(0), f(2)), pack16<BF16>(f(4), f(6)), pack16<BF16>(f(1), f(3)),
+                   pack16<BF16>(f(5), f(7)));
+          }
+        }
+        __syncwarp();
+        for (int it = 0; it < 16; ++it) {
+          const int rr = quarter * 32 + it * 2 + (lane >> 4), rw = row0 + x * 128 + rr;
+          if (rw < p.rows) {
+            const uint4 v = lds128(chunk_at(stage, rr, lane & 15));
+            T* dst = static_cast<T*>(p.out) + b * p.o_sb + (int64_t)(rw / p.n_rep) * p.o_st + (int64_t)(hk * p.n_rep + rw % p.n_rep) * p.o_sh;
+            *reinterpret_cast<uint4*>(dst + (lane & 15) * 8) = v;
+          }
+        }
+      }
+    } else if (row0 + (PAIR ? x * 128 : 0) + quarter * 32 < p.rows) {
+      // a partial result, the channels in their order
+      const int64_t at = (bh * p.rows + row) * a.parts + (PAIR ? part : 2 * part + x);
+      if (row < p.rows) a.part_ml[at] = make_float2(ok ? (n_x > 0 ? m_ref * nat : -INFINITY) : 0.f, ok ? l_run : NAN);
+      if (n_x > 0 && ok) {
+#pragma unroll 1
+        for (int cc = 0; cc < 4; ++cc) {
+          uint32_t r[32];
+          tmem_ld32(tO + cc * 32, r);
+          if (row < p.rows) {
+            float4* dst = reinterpret_cast<float4*>(a.part_o + at * 128 + cc * 32);
+#pragma unroll
+            for (int c = 0; c < 32; c += 8) {
+              const auto f = [&](int e) { return __uint_as_float(r[c + e]); };
+              dst[c >> 2] = make_float4(f(0), f(2), f(4), f(6));
+              dst[(c >> 2) + 1] = make_float4(f(1), f(3), f(5), f(7));
+            }
+          }
+        }
+      }
     }
   }
-  const float inv = l > 0.f ? 1.f / l : 0.f;
-  T* out = static_cast<T*>(p.out) + b * p.o_sb + i * p.o_st + h * p.o_sh + lane * 4;
-  for (int c = 0; c < 4; ++c) out[c] = Elem<T>::from_f(o[c] * inv);
-  if (p.lse && lane == 0) p.lse[((int64_t)b * p.hq + h) * p.q_len + i] = l > 0.f ? m + logf(l) : -INFINITY;
+  tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(WARPS * 32) key_weights_kernel(Params p, const float* vis_in, const float* fp_in, float* vis, float* fp,
-                                                                 int64_t capacity) {
-  const int lane = threadIdx.x & 31, key0 = (blockIdx.x * WARPS + (threadIdx.x >> 5)) * 8, hk = blockIdx.y, b = blockIdx.z;
-  const int live = live_tokens(p), n_keys = p.t_vis + live;
-  if (key0 >= p.t_vis + capacity) return;
-  float w[8] = {};
-  if (key0 < n_keys) {
-    float k[8][4];
-    load_keys<T>(p, b, hk, key0, n_keys, lane, k);
-    for (int row = 0; row < p.rows; ++row) {
-      const int i = row / p.n_rep, h = hk * p.n_rep + row % p.n_rep;
-      const float lse = p.lse[((int64_t)b * p.hq + h) * p.q_len + i];
-      if (lse == -INFINITY) continue;
-      float q[4], s[8];
-      load4(static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_st + h * p.q_sh + lane * 4, q);
-      logits<T>(p, b, key0, p.t_vis + max(0, live - p.q_len + i + 1), q, k, s);
-      for (int j = 0; j < 8; ++j)
-        if (s[j] != -INFINITY) w[j] += expf(s[j] - lse);
-    }
+// Merge of a row's partial results: a warp per row, a lane per four channels.
+template <bool BF16>
+__global__ void __launch_bounds__(256) chunk_combine_kernel(AttnParams a, int64_t all_rows) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  const Params& p = a.p;
+  const int lane = threadIdx.x & 31;
+  const int64_t at = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  pdl_wait();
+  if (at >= all_rows) return;
+  const float2* ml = a.part_ml + at * a.parts;
+  float m = -INFINITY;
+  bool bad = false;
+  for (int s = 0; s < a.parts; ++s) {
+    const float2 v = ml[s];
+    bad |= v.y != v.y;
+    if (v.y > 0.f) m = fmaxf(m, v.x);
   }
-  if (lane == 0) {
-    const int64_t bh = (int64_t)b * p.hkv + hk;
-    for (int j = 0; j < 8; ++j) {
-      const int key = key0 + j;
-      if (key < p.t_vis)
-        vis[bh * p.t_vis + key] = (vis_in ? vis_in[bh * p.t_vis + key] : 0.f) + w[j];
-      else if (key < p.t_vis + capacity)
-        fp[bh * capacity + key - p.t_vis] = (fp_in ? fp_in[bh * capacity + key - p.t_vis] : 0.f) + w[j];
-    }
+  float l = 0.f, o[4] = {};
+  for (int s = 0; s < a.parts; ++s) {
+    const float2 v = ml[s];
+    if (!(v.y > 0.f)) continue;
+    const float f = exp2f((v.x - m) * LOG2E);
+    const float4 x = *reinterpret_cast<const float4*>(a.part_o + (at * a.parts + s) * 128 + lane * 4);
+    l = fmaf(v.y, f, l);
+    o[0] = fmaf(x.x, f, o[0]); o[1] = fmaf(x.y, f, o[1]); o[2] = fmaf(x.z, f, o[2]); o[3] = fmaf(x.w, f, o[3]);
   }
+  const float inv = bad ? NAN : l > 0.f ? 1.f / l : 0.f;
+  const int row = (int)(at % p.rows), i = row / p.n_rep;
+  const int64_t bh = at / p.rows, b = bh / p.hkv, h = (bh % p.hkv) * p.n_rep + row % p.n_rep;
+  T* dst = static_cast<T*>(p.out) + b * p.o_sb + i * p.o_st + h * p.o_sh + lane * 4;
+  *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<BF16>(o[0] * inv, o[1] * inv), pack16<BF16>(o[2] * inv, o[3] * inv));
+  if (p.lse && lane == 0) p.lse[(b * p.hq + h) * p.q_len + i] = bad ? NAN : l > 0.f ? m + logf(l) : -INFINITY;
+}
+
+// ---- host ---------------------------------------------------------------------------------------------------------
+struct Plan {
+  bool pair;
+  int row_blocks, grid_parts, parts;
+};
+// Split of the key tiles: as many CTAs as fill the SMs, in whole rounds where there are several; a CTA costs about three key tiles beside
+// its own (its start, and its partial result).
+static Plan make_plan(const cq_chunk_args* a) {
+  const int64_t rows = (int64_t)a->q_len * (a->n_q_heads / a->n_kv_heads);
+  Plan pl;
+  pl.pair = rows > 128;
+  pl.row_blocks = (int)((rows + (pl.pair ? 255 : 127)) / (pl.pair ? 256 : 128));
+  const int64_t items = (int64_t)a->batch * a->n_kv_heads * pl.row_blocks;
+  const int tiles = (a->t_vis + 127) / 128 + (a->t_fp + 127) / 128, sms = sm_count();
+  int best = 1;
+  double cost = 1e300;
+  for (int s = 1; s <= 64 && s <= tiles; ++s) {
+    const int per = (tiles + s - 1) / s;
+    if (s > 1 && (tiles + per - 1) / per != s) continue;      // leaves a part empty
+    const double c = (double)((items * s + sms - 1) / sms) * (per * (pl.pair ? 2 : 1) + 3 + (s > 1 && pl.pair ? 2 : 0));
+    if (c < cost) { cost = c; best = s; }
+  }
+  pl.grid_parts = best;
+  pl.parts = pl.pair ? best : 2 * best;
+  return pl;
+}
+static size_t workspace_bytes(const cq_chunk_args* a, const Plan& pl) {
+  if (pl.parts == 1) return 256;
+  const size_t rows = (size_t)a->batch * a->n_q_heads * a->q_len;
+  return 256 + rows * pl.parts * (128 * sizeof(float) + sizeof(float2));
+}
+
+template <bool BF16, bool MASK, bool PAIR>
+static int launch_attn(const AttnParams& p, const Plan& pl, int batch, cudaStream_t st) {
+  static bool configured[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CQ_ERR_LAUNCH;
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(chunk_attn_kernel<BF16, MASK, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return CQ_ERR_LAUNCH;
+    configured[dev] = true;
+  }
+  const dim3 grid(pl.row_blocks, batch * p.p.hkv, pl.grid_parts);
+  chunk_attn_kernel<BF16, MASK, PAIR><<<grid, THREADS, SMEM_BYTES, st>>>(p);
+  if (const int rc = check_launch()) return rc;
+  if (pl.parts == 1) return CQ_OK;
+  const int64_t rows = (int64_t)batch * p.p.hkv * p.p.rows;
+  return launched(launch_pdl(chunk_combine_kernel<BF16>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p, rows));
+}
+
+static bool attn_valid(const cq_chunk_args* a) {
+  if (!valid(a) || !a->out || !aligned16(a->out) || !a->v_fp || !aligned16(a->v_fp)) return false;
+  for (int i = 0; i < 3; ++i)
+    if (a->out_strides[i] % 8) return false;
+  return !a->t_vis || (a->v_code && a->v_scale && a->v_mn && aligned16(a->v_code) && aligned16(a->v_scale) && aligned16(a->v_mn));
+}
+static bool attn_supported(const cq_chunk_args* a) {
+  return supported(a) && (int64_t)a->batch * a->n_kv_heads <= 65535;
 }
 
 }  // namespace chunk
@@ -138,46 +609,31 @@ __global__ void __launch_bounds__(WARPS * 32) key_weights_kernel(Params p, const
 
 using namespace cq;
 
-static bool chunk_valid(const cq_chunk_args* a) {
-  if (!chunk::valid(a) || !a->out || !aligned16(a->out) || !a->v_fp || !aligned16(a->v_fp)) return false;
-  for (int i = 0; i < 3; ++i)
-    if (a->out_strides[i] % 8) return false;
-  return !a->t_vis || (a->v_code && a->v_scale && a->v_mn && aligned16(a->v_code) && aligned16(a->v_scale) && aligned16(a->v_mn));
-}
-
 extern "C" size_t cq_chunk_attn_workspace_bytes(const cq_chunk_args* a) {
-  return chunk_valid(a) && chunk::supported(a) ? 256 : 0;
+  if (!chunk::attn_valid(a) || !chunk::attn_supported(a)) return 0;
+  return chunk::workspace_bytes(a, chunk::make_plan(a));
 }
 
 extern "C" int cq_chunk_attn(const cq_chunk_args* a, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!chunk_valid(a)) return CQ_ERR_BAD_ARG;
-  if (!chunk::supported(a)) return CQ_ERR_UNSUPPORTED;
-  if (!workspace || workspace_bytes < cq_chunk_attn_workspace_bytes(a)) return CQ_ERR_WORKSPACE;
+  if (!chunk::attn_valid(a)) return CQ_ERR_BAD_ARG;
+  if (!chunk::attn_supported(a)) return CQ_ERR_UNSUPPORTED;
+  const chunk::Plan pl = chunk::make_plan(a);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < chunk::workspace_bytes(a, pl)) return CQ_ERR_WORKSPACE;
   if (a->batch == 0) return CQ_OK;
-  const chunk::Params p = chunk::make_params(a);
-  const dim3 grid((p.rows + chunk::WARPS - 1) / chunk::WARPS, p.hkv, a->batch);
+  chunk::AttnParams p = {};
+  p.p = chunk::make_params(a);
+  p.parts = pl.parts;
+  p.scale = 0.08838834764831845f;
+  const int bf16 = a->dtype == CQ_DTYPE_BF16;
+  p.idesc_kmajor = chunk::idesc_of(bf16, 0, 0, 128, 128);
+  p.idesc_mn = chunk::idesc_of(bf16, 0, 1, 128, 128);
+  const size_t rows = (size_t)a->batch * a->n_q_heads * a->q_len;
+  p.status = static_cast<int*>(workspace);
+  p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+  p.part_ml = reinterpret_cast<float2*>(p.part_o + rows * pl.parts * 128);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->dtype == CQ_DTYPE_BF16) chunk::chunk_rows_kernel<__nv_bfloat16><<<grid, chunk::WARPS * 32, 0, st>>>(p);
-  else chunk::chunk_rows_kernel<__half><<<grid, chunk::WARPS * 32, 0, st>>>(p);
-  return check_launch();
-}
-
-extern "C" size_t cq_key_weights_workspace_bytes(const cq_chunk_args* a) {
-  return chunk::valid(a) && a->lse && chunk::supported(a) ? 256 : 0;
-}
-
-extern "C" int cq_key_weights(const cq_chunk_args* a, const float* w_vis_in, const float* w_fp_in, float* w_vis, float* w_fp,
-                              int64_t w_capacity, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!chunk::valid(a) || !a->lse || (a->t_vis && !w_vis) || !w_fp || w_capacity < a->t_fp) return CQ_ERR_BAD_ARG;
-  if (!chunk::supported(a) || a->t_vis + w_capacity >= (1ll << 30)) return CQ_ERR_UNSUPPORTED;
-  if (!workspace || workspace_bytes < cq_key_weights_workspace_bytes(a)) return CQ_ERR_WORKSPACE;
-  if (a->batch == 0) return CQ_OK;
-  const chunk::Params p = chunk::make_params(a);
-  const dim3 grid((unsigned)((p.t_vis + w_capacity + chunk::WARPS * 8 - 1) / (chunk::WARPS * 8)), p.hkv, a->batch);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->dtype == CQ_DTYPE_BF16)
-    chunk::key_weights_kernel<__nv_bfloat16><<<grid, chunk::WARPS * 32, 0, st>>>(p, w_vis_in, w_fp_in, w_vis, w_fp, w_capacity);
-  else
-    chunk::key_weights_kernel<__half><<<grid, chunk::WARPS * 32, 0, st>>>(p, w_vis_in, w_fp_in, w_vis, w_fp, w_capacity);
-  return check_launch();
+#define CQ_RUN(B, M) (pl.pair ? chunk::launch_attn<B, M, true>(p, pl, a->batch, st) : chunk::launch_attn<B, M, false>(p, pl, a->batch, st))
+  if (bf16) return a->mask ? CQ_RUN(true, true) : CQ_RUN(true, false);
+  return a->mask ? CQ_RUN(false, true) : CQ_RUN(false, false);
+#undef CQ_RUN
 }
