@@ -151,7 +151,7 @@ SIGNATURES = {
     "cq_workspace_status": (_c.c_int, [_vp, _vp]),
     "cq_chunk_attn_workspace_bytes": (_sz, [_c.POINTER(ChunkArgs)]),
     "cq_chunk_attn": (_c.c_int, [_c.POINTER(ChunkArgs), _vp, _sz, _vp]),
-    "cq_key_weights_workspace_bytes": (_sz, [_c.POINTER(ChunkArgs)]),
+    "cq_key_weights_workspace_bytes": (_sz, [_c.POINTER(ChunkArgs), _i64]),
     "cq_key_weights": (_c.c_int, [_c.POINTER(ChunkArgs), _vp, _vp, _vp, _vp, _i64, _vp, _sz, _vp]),
     "cq_evict_groups": (_c.c_int, [_vp, _vp, _vp, _vp, _vp, _vp, _vp, _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int, _c.c_int,
                                    _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _vp]),

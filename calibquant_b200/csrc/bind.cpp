@@ -948,7 +948,7 @@ PyObject* py_key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
     out[1] = empty({d.batch, d.n_kv_heads, given ? in[1].size(2) : d.t_fp}, c.q, at::kFloat);
   }
   if (d.batch > 0) {
-    const size_t nbytes = cq_key_weights_workspace_bytes(&d);
+    const size_t nbytes = cq_key_weights_workspace_bytes(&d, out[1].size(2));
     if (nbytes == 0) {
       const int rc = cq_key_weights(&d, nullptr, nullptr, out[0].data_ptr<float>(), out[1].data_ptr<float>(), out[1].size(2), nullptr, 0, call.stream);
       check(rc ? rc : CQ_ERR_WORKSPACE, "cq_key_weights");

@@ -1,114 +1,371 @@
-// How much attention each key got: the simplest form.  A warp per eight keys, a lane holds four channels; scores are summed over the
-// lanes.  All arithmetic in fp32.
+// How much attention the queries of a chunk paid to each key: column sums of exp(score - log-sum-exp), on tcgen05.
+//
+// The scores are formed the other way round than for the attention, S^T = K Q^T: a TMEM lane per key, so that a key's sum over the queries
+// stays in one thread and no exchange is needed.  A CTA holds two key tiles of 128 (packed keys as two 16-bit terms, exact as there) and
+// goes over the query rows of their KV head in blocks of NB.  Roles:
+//   warps 0-3 / 4-7  sums of key tile 0 / 1: thread = key
+//   warps 8-15       operands: the key tiles once, then the query blocks through two slots (requested a block ahead)
+//   warp 16          issues the products
+// TMEM: tile X's scores in columns X * 256 + buffer * 128.  Where the key tiles are fewer than the SMs, the rows are cut into parts whose
+// sums finish_kernel adds in their order.
 #include <math.h>
 
-#include "cq_chunk.cuh"
+#include <type_traits>
+
+#include "cq_chunk_tc.cuh"
 
 namespace cq {
 namespace chunk {
 
-constexpr int WARPS = 8;
+using namespace ptx;
+using namespace tc;
 
-template <typename T>
-__device__ __forceinline__ void load4(const T* p, float (&v)[4]) {
-  const uint2 w = *reinterpret_cast<const uint2*>(p);
-  using T2 = typename Elem<T>::T2;
-  const float2 a = Elem<T>::to_f2(*reinterpret_cast<const T2*>(&w.x)), b = Elem<T>::to_f2(*reinterpret_cast<const T2*>(&w.y));
-  v[0] = a.x; v[1] = a.y; v[2] = b.x; v[3] = b.y;
+namespace kw {
+
+constexpr int PRODUCERS = 8, MMA_WARP = 16, THREADS = 17 * 32;
+constexpr int SMEM_BYTES = 6 * TILE_BYTES + 1024;
+constexpr uint32_t WAIT_TRIES = 1u << 22;
+constexpr long long WAIT_CYCLES = 1ll << 30;
+constexpr float LOG2E = 1.4426950408889634f;
+
+struct WeightParams {
+  Params p;
+  const float *vis_in, *fp_in;
+  float *vis, *fp;
+  int64_t capacity;          // full-precision weights per (batch row, KV head)
+  int64_t batch;
+  int parts;
+  float* part;               // [part][batch][KV head][t_vis + capacity]
+  float scale;
+  uint32_t idesc_kmajor, idesc_mn;
+  int* status;
+};
+
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+__device__ __forceinline__ void tile_barrier(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+// (x0, x1) = (a0, a1) * (b, b) + (c0, c1)
+__device__ __forceinline__ void fma_pair(float& x0, float& x1, float a0, float a1, float b, float c0, float c1) {
+  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %4};\n\tmov.b64 rc, {%5, %6};\n\t"
+      "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(x0), "=f"(x1) : "f"(a0), "f"(a1), "f"(b), "f"(c0), "f"(c1));
+}
+__device__ __forceinline__ void add_pair(float& s0, float& s1, float a0, float a1) {
+  asm("{\n\t.reg .b64 ra, rs;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rs, {%0, %1};\n\tadd.rn.f32x2 rs, rs, ra;\n\tmov.b64 {%0, %1}, rs;\n\t}"
+      : "+f"(s0), "+f"(s1) : "f"(a0), "f"(a1));
 }
 
-// Keys key0 .. key0+7 in cache order [visual | fp], this lane's channels 4*lane .. +3; keys past the end are zeros.
-template <typename T>
-__device__ __forceinline__ void load_keys(const Params& p, int b, int hk, int key0, int n_keys, int lane, float (&k)[8][4]) {
-  if (key0 < p.t_vis) {
-    const int64_t row = ((int64_t)b * p.hkv + hk) * 128 + lane * 4;
-    for (int c = 0; c < 4; ++c) {
-      const uint32_t w = p.k_code[(row + c) * (p.t_vis / 8) + key0 / 8];
-      const float s = Elem<T>::to_f(static_cast<const T*>(p.k_scale)[(row + c) * (p.t_vis / 32) + key0 / 32]);
-      const float m = Elem<T>::to_f(static_cast<const T*>(p.k_mn)[(row + c) * (p.t_vis / 32) + key0 / 32]);
-      for (int j = 0; j < 8; ++j) k[j][c] = fmaf((float)((w >> (4 * j)) & 15u), s, m);
-    }
-  } else {
-    for (int j = 0; j < 8; ++j) {
-      if (key0 + j < n_keys)
-        load4(static_cast<const T*>(p.k_fp) + b * p.fp_sb + hk * p.fp_sh + (int64_t)(key0 + j - p.t_vis) * 128 + lane * 4, k[j]);
-      else
-        for (int c = 0; c < 4; ++c) k[j][c] = 0.f;
-    }
-  }
+// result of key `key` (cache order [visual | fp]) of KV head bh
+__device__ __forceinline__ void put(const WeightParams& a, int64_t bh, int64_t key, float w) {
+  const int64_t vis = bh * a.p.t_vis + key, fp = bh * a.capacity + key - a.p.t_vis;
+  if (key < a.p.t_vis) a.vis[vis] = (a.vis_in ? a.vis_in[vis] : 0.f) + w;
+  else a.fp[fp] = (a.fp_in ? a.fp_in[fp] : 0.f) + w;
 }
 
-// logits of a row against eight keys; -inf where a key takes no part
-template <typename T>
-__device__ __forceinline__ void logits(const Params& p, int b, int key0, int limit, const float (&q)[4], const float (&k)[8][4], float (&s)[8]) {
-  for (int j = 0; j < 8; ++j) {
-    float x = q[0] * k[j][0] + q[1] * k[j][1] + q[2] * k[j][2] + q[3] * k[j][3];
-    x = warp_sum(x) * 0.08838834764831845f;
-    const int key = key0 + j;
-    if (key >= limit) {
-      x = -INFINITY;
-    } else if (p.mask) {
-      const float m = Elem<T>::to_f(static_cast<const T*>(p.mask)[b * p.mask_sb + mask_index(p, key)]);
-      x = m == -INFINITY ? -INFINITY : x + m;
+template <bool BF16, bool MASK, int NB>
+__global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_constant__ WeightParams a) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  const Params& p = a.p;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t k_s = smem_u32(smem), q_s = k_s + 4 * TILE_BYTES;      // key tiles [X][hi, lo], query slots
+  // bar_k the key tiles are there; bar_q/free[slot] query blocks; bar_d/dfree[X][buffer] scores ready / read
+  __shared__ __align__(8) uint64_t bar_k, bar_q[2], bar_free[2], bar_d[2][2], bar_dfree[2][2];
+  __shared__ uint32_t tmem_base_s;
+  __shared__ __align__(16) float lse_s[2][2][NB];
+
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int hk = blockIdx.y % p.hkv, b = blockIdx.y / p.hkv;
+  const int64_t bh = (int64_t)b * p.hkv + hk;
+  const int live = live_tokens(p), nv = (p.t_vis + 127) >> 7;
+  // first key of tile X; keys of a tile that are there; first row that sees one of them
+  const int tile0 = (int)blockIdx.x * 2;
+  const auto first_key = [&](int x) { return tile0 + x < nv ? (tile0 + x) * 128 : p.t_vis + (tile0 + x - nv) * 128; };
+  const auto alive = [&](int x) { return tile0 + x < nv || (tile0 + x - nv) * 128 < live; };
+  const auto first_row = [&](int t) { return (int64_t)max(0, t - live + p.q_len) * p.n_rep; };      // of full-precision token t
+  const int blocks_all = (p.rows + NB - 1) / NB, per = (blocks_all + (int)gridDim.z - 1) / (int)gridDim.z;
+  int blk0 = min(blocks_all, (int)blockIdx.z * per);
+  const int blk1 = min(blocks_all, blk0 + per);
+  if (tile0 >= nv) blk0 = max(blk0, (int)min((int64_t)blk1, first_row((tile0 - nv) * 128) / NB));
+  const int n_x = !alive(0) ? 0 : alive(1) ? 2 : 1, nb = n_x ? blk1 - blk0 : 0;
+  pdl_launch_dependents();
+
+  if (tid == 0) {
+    mbar_init(&bar_k, PRODUCERS);
+    for (int s = 0; s < 2; ++s) {
+      mbar_init(&bar_q[s], PRODUCERS);
+      mbar_init(&bar_free[s], 1);
+      for (int x = 0; x < 2; ++x) {
+        mbar_init(&bar_d[x][s], 1);
+        mbar_init(&bar_dfree[x][s], 128);
+      }
     }
-    s[j] = x;
+    mbar_fence_init();
   }
+  if (warp == MMA_WARP) tmem_alloc(&tmem_base_s, 512);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = tmem_base_s;
+
+  if (warp >= 8 && warp < MMA_WARP) {
+    // ================= operands =================
+    const int pw = warp - 8, ptid = tid - 256;
+    constexpr int CH = NB / 16;                  // chunks of a block per thread
+    uint4 v[CH];
+    const auto request = [&](int blk) {
+#pragma unroll
+      for (int it = 0; it < CH; ++it) {
+        const int row = blk * NB + it * 16 + (ptid >> 4);
+        v[it] = make_uint4(0, 0, 0, 0);
+        if (row < p.rows) {
+          const int i = row / p.n_rep, h = hk * p.n_rep + row % p.n_rep;
+          v[it] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_st + h * p.q_sh + (ptid & 15) * 8);
+        }
+      }
+    };
+    if (nb > 0) {
+      for (int x = 0; x < n_x; ++x) {
+        const uint32_t hi = k_s + x * 2 * TILE_BYTES, lo = hi + TILE_BYTES;
+        if (tile0 + x < nv) {
+          Unit u[2];
+          load_k_unit(p, bh, tile0 + x, pw, lane, u[0]);
+          load_k_unit(p, bh, tile0 + x, pw + 8, lane, u[1]);
+          store_k_unit<BF16>(hi, lo, u[0], pw, lane);
+          store_k_unit<BF16>(hi, lo, u[1], pw + 8, lane);
+        } else {
+          const T* src = static_cast<const T*>(p.k_fp) + b * p.fp_sb + hk * p.fp_sh;
+#pragma unroll
+          for (int it = 0; it < 8; ++it) {
+            const int r = it * 16 + (ptid >> 4), t = (tile0 + x - nv) * 128 + r;
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (t < live) w = *reinterpret_cast<const uint4*>(src + (int64_t)t * 128 + (ptid & 15) * 8);
+            sts128(chunk_at(hi, r, ptid & 15), w.x, w.y, w.z, w.w);
+          }
+        }
+      }
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar_k);
+      request(blk0);
+    }
+    bool ok = true;
+    for (int n = 0; n < nb && ok; ++n) {
+      const int s = n & 1;
+      if (n >= 2) ok = mbar_wait_bounded(&bar_free[s], ((n >> 1) - 1) & 1, WAIT_TRIES);
+      ok = __all_sync(0xffffffffu, ok);
+      if (!ok) break;
+#pragma unroll
+      for (int it = 0; it < CH; ++it)
+        sts128(chunk_at(q_s + s * TILE_BYTES, it * 16 + (ptid >> 4), ptid & 15), v[it].x, v[it].y, v[it].z, v[it].w);
+      if (n + 1 < nb) request(blk0 + n + 1);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar_q[s]);
+    }
+    if (!ok && lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
+  } else if (warp == MMA_WARP) {
+    // ================= products =================
+    const uint32_t lead = elect_one();
+    const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
+    constexpr uint64_t tile16 = TILE_BYTES >> 4;
+    const uint64_t kd = smem_desc(k_s, 16, 1024), md = smem_desc(k_s, PANEL_BYTES, 1024), qd = smem_desc(q_s, 16, 1024);
+    const auto all = [](bool r) { return __all_sync(0xffffffffu, r) != 0; };
+    bool ok = nb == 0 || all(mbar_wait_bounded(&bar_k, 0, WAIT_TRIES));
+    for (int n = 0; n < nb && ok; ++n) {
+      const int s = n & 1;
+      ok = all(mbar_wait_bounded(&bar_q[s], (n >> 1) & 1, WAIT_TRIES));
+      for (int x = 0; x < n_x && ok; ++x) {
+        if (n >= 2) ok = all(mbar_wait_cycles(&bar_dfree[x][s], ((n >> 1) - 1) & 1, WAIT_CYCLES));
+        if (!ok) break;
+        tc_fence_after();
+        if (lead) {
+          const uint32_t d = tm + (uint32_t)(x * 256 + s * 128);
+          const bool packed = tile0 + x < nv;
+#pragma unroll
+          for (int ks = 0; ks < 8; ++ks) {
+            const uint64_t qo = (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4), q = qd + s * tile16 + qo;
+            if (packed) umma(d, md + 2 * x * tile16 + (uint64_t)(ks * 128), q, a.idesc_mn, ks > 0);
+            else umma(d, kd + 2 * x * tile16 + qo, q, a.idesc_kmajor, ks > 0);
+          }
+          if (packed) {
+#pragma unroll
+            for (int ks = 0; ks < 8; ++ks)
+              umma(d, md + (2 * x + 1) * tile16 + (uint64_t)(ks * 128), qd + s * tile16 + (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4), a.idesc_mn, 1);
+          }
+          umma_commit(&bar_d[x][s]);
+        }
+      }
+      if (ok && lead) umma_commit(&bar_free[s]);
+    }
+    if (!ok && lead) atomicExch(a.status, CQ_ERR_TIMEOUT);
+    __syncwarp();
+  } else if (warp < 8) {
+    // ================= sums: thread = key =================
+    const int x = warp >> 2, r_in = (warp & 3) * 32 + lane;
+    const int64_t key = first_key(x) + r_in;
+    const bool vis = tile0 + x < nv;
+    const int t = (int)(key - p.t_vis);                                 // full-precision token
+    const bool there = vis ? key < p.t_vis : t < live;
+    float m = 0.f;
+    if (MASK && there) m = Elem<T>::to_f(static_cast<const T*>(p.mask)[b * p.mask_sb + mask_index(p, (int)key)]);
+    const int64_t rmin = vis ? 0 : first_row(t);                        // the first row that sees the key
+    const uint32_t tD = tmem + (uint32_t)x * 256u + ((uint32_t)((warp & 3) * 32) << 16);
+    const float c1 = a.scale * LOG2E;
+    bool ok = true;
+    float acc[4] = {};
+    // minus the rows' log-sum-exp in units of the exponent (log-sum-exp as it is with a mask); a row that adds nothing: -inf
+    const auto lse_of = [&](int n) {
+      const int row = (blk0 + n) * NB + r_in;
+      if (r_in >= NB || n >= nb || row >= p.rows) return MASK ? INFINITY : -INFINITY;
+      const float v = p.lse[((int64_t)b * p.hq + hk * p.n_rep + row % p.n_rep) * p.q_len + row / p.n_rep];
+      if (v == -INFINITY) return MASK ? INFINITY : -INFINITY;
+      return MASK ? v : -v * LOG2E;
+    };
+    if (x < n_x && nb > 0) {
+      float next = lse_of(0);
+      for (int n = 0; n < nb; ++n) {
+        const int s = n & 1;
+        if (r_in < NB) lse_s[x][s][r_in] = next;
+        next = lse_of(n + 1);
+        tile_barrier(1 + x);
+        if (ok) ok = mbar_wait_cycles(&bar_d[x][s], (n >> 1) & 1, WAIT_CYCLES);
+        tc_fence_after();
+        const int64_t r0 = (int64_t)(blk0 + n) * NB;
+        const bool need = __any_sync(0xffffffffu, rmin > r0);
+        const int hidden = (int)min((int64_t)NB, rmin - r0);            // columns below are not seen
+#pragma unroll
+        for (int cc = 0; cc < NB / 32; ++cc) {
+          uint32_t d[32];
+          tmem_ld32(tD + s * 128 + cc * 32, d);
+          if (cc == NB / 32 - 1) {
+            tc_fence_before();
+            mbar_arrive(&bar_dfree[x][s]);
+          }
+#pragma unroll
+          for (int c = 0; c < 32; c += 4) {
+            const float4 l = *reinterpret_cast<const float4*>(&lse_s[x][s][cc * 32 + c]);
+            float e[4];
+            if (MASK) {
+              e[0] = (fmaf(__uint_as_float(d[c]), a.scale, m) - l.x) * LOG2E;
+              e[1] = (fmaf(__uint_as_float(d[c + 1]), a.scale, m) - l.y) * LOG2E;
+              e[2] = (fmaf(__uint_as_float(d[c + 2]), a.scale, m) - l.z) * LOG2E;
+              e[3] = (fmaf(__uint_as_float(d[c + 3]), a.scale, m) - l.w) * LOG2E;
+            } else {
+              fma_pair(e[0], e[1], __uint_as_float(d[c]), __uint_as_float(d[c + 1]), c1, l.x, l.y);
+              fma_pair(e[2], e[3], __uint_as_float(d[c + 2]), __uint_as_float(d[c + 3]), c1, l.z, l.w);
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              e[i] = ex2_approx(e[i]);
+              if (need && cc * 32 + c + i < hidden) e[i] = 0.f;
+            }
+            add_pair(acc[0], acc[1], e[0], e[1]);
+            add_pair(acc[2], acc[3], e[2], e[3]);
+          }
+        }
+      }
+      if (!__all_sync(0xffffffffu, ok) && lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
+    }
+    float w = (acc[0] + acc[1]) + (acc[2] + acc[3]);
+    if (!ok) w = NAN;
+    if (!there || (MASK && m == -INFINITY)) w = 0.f;
+    const int64_t end = vis ? p.t_vis : p.t_vis + a.capacity;
+    if (key < end) {
+      if (a.parts == 1) put(a, bh, key, w);
+      else a.part[((int64_t)blockIdx.z * a.batch * p.hkv + bh) * (p.t_vis + a.capacity) + key] = w;
+    }
+  }
+  tc_fence_before();
+  __syncthreads();
+  if (warp == MMA_WARP) tmem_dealloc(tmem, 512);
 }
 
-template <typename T>
-__global__ void __launch_bounds__(WARPS * 32) key_weights_kernel(Params p, const float* vis_in, const float* fp_in, float* vis, float* fp,
-                                                                 int64_t capacity) {
-  const int lane = threadIdx.x & 31, key0 = (blockIdx.x * WARPS + (threadIdx.x >> 5)) * 8, hk = blockIdx.y, b = blockIdx.z;
-  const int live = live_tokens(p), n_keys = p.t_vis + live;
-  if (key0 >= p.t_vis + capacity) return;
-  float w[8] = {};
-  if (key0 < n_keys) {
-    float k[8][4];
-    load_keys<T>(p, b, hk, key0, n_keys, lane, k);
-    for (int row = 0; row < p.rows; ++row) {
-      const int i = row / p.n_rep, h = hk * p.n_rep + row % p.n_rep;
-      const float lse = p.lse[((int64_t)b * p.hq + h) * p.q_len + i];
-      if (lse == -INFINITY) continue;
-      float q[4], s[8];
-      load4(static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_st + h * p.q_sh + lane * 4, q);
-      logits<T>(p, b, key0, p.t_vis + max(0, live - p.q_len + i + 1), q, k, s);
-      for (int j = 0; j < 8; ++j)
-        if (s[j] != -INFINITY) w[j] += expf(s[j] - lse);
-    }
-  }
-  if (lane == 0) {
-    const int64_t bh = (int64_t)b * p.hkv + hk;
-    for (int j = 0; j < 8; ++j) {
-      const int key = key0 + j;
-      if (key < p.t_vis)
-        vis[bh * p.t_vis + key] = (vis_in ? vis_in[bh * p.t_vis + key] : 0.f) + w[j];
-      else if (key < p.t_vis + capacity)
-        fp[bh * capacity + key - p.t_vis] = (fp_in ? fp_in[bh * capacity + key - p.t_vis] : 0.f) + w[j];
-    }
-  }
+// sums of the parts, in their order
+__global__ void __launch_bounds__(256) key_weights_finish_kernel(WeightParams a) {
+  const int64_t key = (int64_t)blockIdx.x * 256 + threadIdx.x, bh = blockIdx.y, keys = a.p.t_vis + a.capacity;
+  pdl_wait();
+  if (key >= keys) return;
+  float w = 0.f;
+  for (int s = 0; s < a.parts; ++s) w += a.part[((int64_t)s * gridDim.y + bh) * keys + key];
+  put(a, bh, key, w);
 }
 
+// ---- host ---------------------------------------------------------------------------------------------------------
+struct Plan {
+  int nb, pairs, parts;
+};
+static Plan make_plan(const cq_chunk_args* a, int64_t capacity) {
+  Plan pl;
+  const int64_t rows = (int64_t)a->q_len * (a->n_q_heads / a->n_kv_heads);
+  pl.nb = rows <= 32 ? 32 : 128;
+  pl.pairs = (int)(((a->t_vis + 127) / 128 + (capacity + 127) / 128 + 1) / 2);
+  // CTAs for the keys alone leave SMs idle: rows in parts, each of four blocks at least
+  const int64_t ctas = (int64_t)a->batch * a->n_kv_heads * pl.pairs, blocks = (rows + pl.nb - 1) / pl.nb;
+  int64_t parts = ctas > 0 ? sm_count() / ctas : 1;
+  if (parts > blocks / 4) parts = blocks / 4;
+  pl.parts = (int)(parts < 1 ? 1 : parts > 16 ? 16 : parts);
+  return pl;
+}
+static size_t bytes_of(const cq_chunk_args* a, int64_t capacity, const Plan& pl) {
+  return 256 + (pl.parts > 1 ? (size_t)pl.parts * a->batch * a->n_kv_heads * (a->t_vis + capacity) * sizeof(float) : 0);
+}
+
+template <bool BF16, bool MASK, int NB>
+static int run(const WeightParams& p, const Plan& pl, cudaStream_t st) {
+  static bool configured[64] = {};
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CQ_ERR_LAUNCH;
+  if (!configured[dev]) {
+    if (cudaFuncSetAttribute(key_weights_kernel<BF16, MASK, NB>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return CQ_ERR_LAUNCH;
+    configured[dev] = true;
+  }
+  const unsigned bh = (unsigned)(p.batch * p.p.hkv);
+  key_weights_kernel<BF16, MASK, NB><<<dim3(pl.pairs, bh, pl.parts), THREADS, SMEM_BYTES, st>>>(p);
+  if (const int rc = check_launch()) return rc;
+  if (pl.parts == 1) return CQ_OK;
+  return launched(launch_pdl(key_weights_finish_kernel, dim3((unsigned)((p.p.t_vis + p.capacity + 255) / 256), bh), dim3(256), 0, st, p));
+}
+
+}  // namespace kw
 }  // namespace chunk
 }  // namespace cq
 
 using namespace cq;
 
-extern "C" size_t cq_key_weights_workspace_bytes(const cq_chunk_args* a) {
-  return chunk::valid(a) && a->lse && chunk::supported(a) ? 256 : 0;
+static bool weights_supported(const cq_chunk_args* a, int64_t capacity) {
+  return chunk::supported(a) && a->t_vis + capacity < (1ll << 30) && (int64_t)a->batch * a->n_kv_heads <= 65535;
+}
+
+extern "C" size_t cq_key_weights_workspace_bytes(const cq_chunk_args* a, int64_t w_capacity) {
+  if (!chunk::valid(a) || !a->lse || w_capacity < a->t_fp || !weights_supported(a, w_capacity)) return 0;
+  return chunk::kw::bytes_of(a, w_capacity, chunk::kw::make_plan(a, w_capacity));
 }
 
 extern "C" int cq_key_weights(const cq_chunk_args* a, const float* w_vis_in, const float* w_fp_in, float* w_vis, float* w_fp,
                               int64_t w_capacity, void* workspace, size_t workspace_bytes, void* stream) {
+  using namespace chunk::kw;
   if (!chunk::valid(a) || !a->lse || (a->t_vis && !w_vis) || !w_fp || w_capacity < a->t_fp) return CQ_ERR_BAD_ARG;
-  if (!chunk::supported(a) || a->t_vis + w_capacity >= (1ll << 30)) return CQ_ERR_UNSUPPORTED;
-  if (!workspace || workspace_bytes < cq_key_weights_workspace_bytes(a)) return CQ_ERR_WORKSPACE;
+  if (!weights_supported(a, w_capacity)) return CQ_ERR_UNSUPPORTED;
+  const Plan pl = make_plan(a, w_capacity);
+  if (!workspace || !aligned16(workspace) || workspace_bytes < bytes_of(a, w_capacity, pl)) return CQ_ERR_WORKSPACE;
   if (a->batch == 0) return CQ_OK;
-  const chunk::Params p = chunk::make_params(a);
-  const dim3 grid((unsigned)((p.t_vis + w_capacity + chunk::WARPS * 8 - 1) / (chunk::WARPS * 8)), p.hkv, a->batch);
+  const int bf16 = a->dtype == CQ_DTYPE_BF16;
+  WeightParams p = {};
+  p.p = chunk::make_params(a);
+  p.vis_in = w_vis_in; p.fp_in = w_fp_in; p.vis = w_vis; p.fp = w_fp;
+  p.capacity = w_capacity; p.batch = a->batch; p.parts = pl.parts;
+  p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+  p.scale = 0.08838834764831845f;
+  p.idesc_kmajor = chunk::idesc_of(bf16, 0, 0, 128, pl.nb);
+  p.idesc_mn = chunk::idesc_of(bf16, 1, 0, 128, pl.nb);
+  p.status = static_cast<int*>(workspace);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (a->dtype == CQ_DTYPE_BF16)
-    chunk::key_weights_kernel<__nv_bfloat16><<<grid, chunk::WARPS * 32, 0, st>>>(p, w_vis_in, w_fp_in, w_vis, w_fp, w_capacity);
-  else
-    chunk::key_weights_kernel<__half><<<grid, chunk::WARPS * 32, 0, st>>>(p, w_vis_in, w_fp_in, w_vis, w_fp, w_capacity);
-  return check_launch();
+#define CQ_RUN(B, M) (pl.nb == 32 ? run<B, M, 32>(p, pl, st) : run<B, M, 128>(p, pl, st))
+  if (bf16) return a->mask ? CQ_RUN(true, true) : CQ_RUN(true, false);
+  return a->mask ? CQ_RUN(false, true) : CQ_RUN(false, false);
+#undef CQ_RUN
 }

@@ -549,7 +549,7 @@ int cq_chunk_attn(const cq_chunk_args* args, void* workspace, size_t workspace_b
  *   *_in       the same shapes, may be the outputs themselves, or NULL: zeros
  * Sums are fp32, in an order that depends on the sizes alone.
  */
-size_t cq_key_weights_workspace_bytes(const cq_chunk_args* args);
+size_t cq_key_weights_workspace_bytes(const cq_chunk_args* args, int64_t w_capacity);
 int cq_key_weights(const cq_chunk_args* args, const float* w_vis_in, const float* w_fp_in, float* w_vis, float* w_fp,
                    int64_t w_capacity, void* workspace, size_t workspace_bytes, void* stream);
 
