@@ -804,6 +804,8 @@ void chunk_common(Chunk& c, PyObject* q, PyObject* k_pack, PyObject* k_fp, PyObj
   want_dims(tensor(q), 4, "q");
   want_dims(tensor(k_fp), 4, "k_fp");
   c.q = with_rows(tensor(q));
+  for (int i = 0; i < 3; ++i)
+    if (c.q.stride(i) == 0 && c.q.size(i) > 1) { c.q = c.q.contiguous(); break; }      // an expanded one
   c.k_fp = tensor(k_fp);
   const int64_t B = c.q.size(0), L = c.q.size(1), Hq = c.q.size(2), D = c.q.size(3), Hkv = c.k_fp.size(1);
   if (Hq % divisor(Hkv, "the number of KV heads")) raise(PyExc_ValueError, "query heads must be a multiple of KV heads");

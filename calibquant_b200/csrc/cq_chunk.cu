@@ -24,7 +24,9 @@ using namespace ptx;
 using namespace tc;
 
 constexpr int SLOTS = 5;
-constexpr int PRODUCERS = 8, MMA_WARP = 16, THREADS = 17 * 32;
+constexpr int PRODUCERS = 8, MMA_WARP = 16, THREADS = 20 * 32;
+// registers: 256 x 120 + 256 x 88 + 128 x 64 = the launch's 640 x 96
+constexpr int SOFTMAX_REGS = 120, PRODUCER_REGS = 88, CONTROL_REGS = 64;
 constexpr int SMEM_BYTES = (2 + SLOTS) * TILE_BYTES + 1024;
 constexpr uint32_t WAIT_TRIES = 1u << 22;
 constexpr long long WAIT_CYCLES = 1ll << 30;
@@ -45,6 +47,9 @@ __device__ __forceinline__ float ex2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
+// register split between warpgroups; every warp of a group runs it
+template <int N> __device__ __forceinline__ void setmaxnreg_inc() { asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(N)); }
+template <int N> __device__ __forceinline__ void setmaxnreg_dec() { asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(N)); }
 __device__ __forceinline__ float max3(float a, float b, float c) {
   float d;
   asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
@@ -124,6 +129,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
 
   if (warp >= 8 && warp < MMA_WARP) {
     // ================= operands =================
+    setmaxnreg_dec<PRODUCER_REGS>();
     const int pw = warp - 8, ptid = tid - 256;
     bool ok = true;
     // the queries; rows past the end are zeros
@@ -242,8 +248,10 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
       if (ok) produce_v(j);
     }
     if (!ok && lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
-  } else if (warp == MMA_WARP) {
+  } else if (warp >= MMA_WARP) {
     // ================= products =================
+    setmaxnreg_dec<CONTROL_REGS>();
+    if (warp == MMA_WARP) {
     // the whole warp runs the loop and one elected lane issues: control flow and operands are uniform
     const uint32_t lead = elect_one();
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
@@ -273,12 +281,12 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
           const uint64_t qo = (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
-          umma(d, q + qo, md + hi * tile16 + (uint64_t)(ks * 128), a.idesc_mn, ks > 0);
+          umma(d, q + qo, md + lo * tile16 + (uint64_t)(ks * 128), a.idesc_mn, ks > 0);      // the small terms first: sums are cut off, not rounded
         }
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
           const uint64_t qo = (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
-          umma(d, q + qo, md + lo * tile16 + (uint64_t)(ks * 128), a.idesc_mn, 1);
+          umma(d, q + qo, md + hi * tile16 + (uint64_t)(ks * 128), a.idesc_mn, 1);
         }
       } else {
 #pragma unroll
@@ -340,8 +348,10 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
     }
     if (!ok && lead) atomicExch(a.status, CQ_ERR_TIMEOUT);
     __syncwarp();
-  } else if (warp < 8) {
+    }
+  } else {
     // ================= softmax: thread = row =================
+    setmaxnreg_inc<SOFTMAX_REGS>();
     const int x = warp >> 2, quarter = warp & 3, r_in = quarter * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t tS = tmem + (uint32_t)x * 128u + lane_off, tO = tmem + 256u + (uint32_t)x * 128u + lane_off;
@@ -372,8 +382,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
       const bool need = __any_sync(0xffffffffu, lim < 128);
       if (ok) ok = mbar_wait_cycles(&bar_s[x], j & 1, WAIT_CYCLES);
       tc_fence_after();
-      const auto scores = [&](int cc, uint32_t (&s)[32]) {         // 32 of them
-        tmem_ld32(tS + cc * 32, s);
+      const auto shown = [&](int cc, uint32_t (&s)[32]) {          // 32 scores with the mask
         if (MASK) {
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
@@ -393,11 +402,17 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
       };
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int cc = 0; cc < 4; ++cc) {
-        uint32_t s[32];
-        scores(cc, s);
+      for (int half = 0; half < 2; ++half) {
+        uint32_t s[2][32];
+        tmem_ld32_nowait(tS + half * 64, s[0]);
+        tmem_ld32_nowait(tS + half * 64 + 32, s[1]);
+        tmem_ld_wait();
 #pragma unroll
-        for (int c = 0; c < 32; c += 2) mx4[(c >> 1) & 3] = max3(mx4[(c >> 1) & 3], __uint_as_float(s[c]), __uint_as_float(s[c + 1]));
+        for (int cc = 0; cc < 2; ++cc) {
+          shown(half * 2 + cc, s[cc]);
+#pragma unroll
+          for (int c = 0; c < 32; c += 2) mx4[(c >> 1) & 3] = max3(mx4[(c >> 1) & 3], __uint_as_float(s[cc][c]), __uint_as_float(s[cc][c + 1]));
+        }
       }
       const float m_true = fmaxf(m_ref, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
       // a row keeps its reference until the true maximum is 2^8 above it (probabilities stay below 256), or for the first time
@@ -421,23 +436,25 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
       float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        uint32_t w[32];
+        uint32_t w[32], s[2][32];
+        tmem_ld32_nowait(tS + half * 64, s[0]);
+        tmem_ld32_nowait(tS + half * 64 + 32, s[1]);
+        tmem_ld_wait();
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
-          uint32_t s[32];
-          scores(half * 2 + cc, s);
+          shown(half * 2 + cc, s[cc]);
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
-            float e0, e1;
+            float e0 = __uint_as_float(s[cc][c]), e1 = __uint_as_float(s[cc][c + 1]);
             if (MASK) {
-              e0 = ex2_approx((__uint_as_float(s[c]) - m_use) * factor);
-              e1 = ex2_approx((__uint_as_float(s[c + 1]) - m_use) * factor);
+              e0 = (e0 - m_use) * factor;
+              e1 = (e1 - m_use) * factor;
             } else {
-              e0 = ex2_approx(fmaf(__uint_as_float(s[c]), factor, neg));
-              e1 = ex2_approx(fmaf(__uint_as_float(s[c + 1]), factor, neg));
+              fma_pair(e0, e1, e0, e1, factor, factor, neg, neg);
             }
-            rs[c & 2] += e0;
-            rs[(c & 2) + 1] += e1;
+            e0 = ex2_approx(e0);
+            e1 = ex2_approx(e1);
+            add_pair(rs[c & 2], rs[(c & 2) + 1], e0, e1);
             w[cc * 16 + (c >> 1)] = pack16<BF16>(e0, e1);
           }
         }

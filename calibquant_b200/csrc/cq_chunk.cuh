@@ -38,14 +38,15 @@ inline bool valid(const cq_chunk_args* a) {
     return false;
   if (!a->q || !a->k_fp || !aligned16(a->q) || !aligned16(a->k_fp) || a->fp_stride_b % 8 || a->fp_stride_h % 8) return false;
   for (int i = 0; i < 3; ++i)
-    if (a->q_strides[i] % 8) return false;
+    if (a->q_strides[i] % 8 || a->q_strides[i] < 0) return false;
+  if ((a->q_strides[0] == 0 && a->batch > 1) || (a->q_strides[1] == 0 && a->q_len > 1) || (a->q_strides[2] == 0 && a->n_q_heads > 1)) return false;
   if (a->mask && reinterpret_cast<uintptr_t>(a->mask) % 2) return false;
   if (a->t_vis && (!a->k_code || !a->k_scale || !a->k_mn || !aligned16(a->k_code) || !aligned16(a->k_scale) || !aligned16(a->k_mn))) return false;
   return true;
 }
 inline bool supported(const cq_chunk_args* a) {
   return a->head_dim == kHeadDim && a->group_size == kGroup && a->bits == 4 && a->t_vis % kGroup == 0 &&
-         a->batch <= 65535 && a->n_kv_heads <= 65535 &&
+         a->batch <= 65535 && a->n_kv_heads <= 65535 && a->n_q_heads / a->n_kv_heads <= 128 &&
          (int64_t)a->q_len * (a->n_q_heads / a->n_kv_heads) < (1ll << 30) && (int64_t)a->t_vis + a->t_fp < (1ll << 30);
 }
 

@@ -5,6 +5,8 @@
 // chunk of a row, and four words share scale and minimum.  Full-precision rows have a token per row.
 #pragma once
 
+#include <cuda.h>
+
 #include "cq_chunk.cuh"
 #include "cq_ptx.cuh"
 #include "cq_tc.cuh"
@@ -34,36 +36,52 @@ __device__ __forceinline__ float number(uint16_t bits) {
   return BF16 ? __uint_as_float((uint32_t)bits << 16) : __half2float(__ushort_as_half(bits));
 }
 
+// (x0, x1) = (a0, a1) * (b0, b1) + (c0, c1)
+__device__ __forceinline__ void fma_pair(float& x0, float& x1, float a0, float a1, float b0, float b1, float c0, float c1) {
+  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %5};\n\tmov.b64 rc, {%6, %7};\n\t"
+      "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
+      : "=f"(x0), "=f"(x1) : "f"(a0), "f"(a1), "f"(b0), "f"(b1), "f"(c0), "f"(c1));
+}
+// (s0, s1) += (a0, a1)
+__device__ __forceinline__ void add_pair(float& s0, float& s1, float a0, float a1) {
+  asm("{\n\t.reg .b64 ra, rs;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rs, {%0, %1};\n\tadd.rn.f32x2 rs, rs, ra;\n\tmov.b64 {%0, %1}, rs;\n\t}"
+      : "+f"(s0), "+f"(s1) : "f"(a0), "f"(a1));
+}
+
 // Two numbers as 16-bit pairs whose sum they are: hi is the number cut off, lo the rest rounded.  A value scale * code + minimum has
 // up to 16 bits in all cases but those where the minimum is hundreds of scales away from zero, and is exact then.
 template <bool BF16>
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
   if (BF16) {
     hi = ptx::prmt(__float_as_uint(a), __float_as_uint(b), 0x7632);
-    const float ra = a - __uint_as_float(__float_as_uint(a) & 0xffff0000u), rb = b - __uint_as_float(__float_as_uint(b) & 0xffff0000u);
-    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(rb), "f"(ra));
+    fma_pair(a, b, __uint_as_float(__float_as_uint(a) & 0xffff0000u), __uint_as_float(__float_as_uint(b) & 0xffff0000u), -1.f, -1.f, a, b);
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(b), "f"(a));
   } else {
     asm("cvt.rz.f16x2.f32 %0, %1, %2;" : "=r"(hi) : "f"(b), "f"(a));
     const float2 h = __half22float2(*reinterpret_cast<const __half2*>(&hi));
-    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(b - h.y), "f"(a - h.x));
+    fma_pair(a, b, h.x, h.y, -1.f, -1.f, a, b);
+    asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(lo) : "f"(b), "f"(a));
   }
 }
 
-// code N (0..7) of a word as the float 16 + code
+// Code N (0..7) of a word as the float 128 + code
 template <int N>
-__device__ __forceinline__ float code16(uint32_t w) {
-  constexpr int sh = 19 - 4 * N;
+__device__ __forceinline__ float code128(uint32_t w) {
+  constexpr int sh = 16 - 4 * N;
   const uint32_t s = sh >= 0 ? w << (sh >= 0 ? sh : 0) : w >> (sh < 0 ? -sh : 0);
-  return __uint_as_float((s & 0x00780000u) | 0x41800000u);
+  return __uint_as_float((s & 0x000f0000u) | 0x43000000u);
 }
-
-// Eight keys of a channel, scale * code + minimum exactly in fp32, as chunks of the two tiles whose sum they are.
+// Eight keys of a channel, scale * code + minimum in fp32, as chunks of the two tiles whose sum they are; off = minimum - 128 scale.  The
+// products are exact, the offset is unless the minimum is thousands of times smaller than the scale (then 2^-17 scales off).
 template <bool BF16>
-__device__ __forceinline__ void keys_of_word(uint32_t w, float s, float off, uint32_t (&hi)[4], uint32_t (&lo)[4]) {      // off = minimum - 16 scale
-  split_pair<BF16>(fmaf(code16<0>(w), s, off), fmaf(code16<1>(w), s, off), hi[0], lo[0]);
-  split_pair<BF16>(fmaf(code16<2>(w), s, off), fmaf(code16<3>(w), s, off), hi[1], lo[1]);
-  split_pair<BF16>(fmaf(code16<4>(w), s, off), fmaf(code16<5>(w), s, off), hi[2], lo[2]);
-  split_pair<BF16>(fmaf(code16<6>(w), s, off), fmaf(code16<7>(w), s, off), hi[3], lo[3]);
+__device__ __forceinline__ void keys_of_word(uint32_t w, float s, float off, uint32_t (&hi)[4], uint32_t (&lo)[4]) {
+  float k[8];
+  fma_pair(k[0], k[1], code128<0>(w), code128<1>(w), s, s, off, off);
+  fma_pair(k[2], k[3], code128<2>(w), code128<3>(w), s, s, off, off);
+  fma_pair(k[4], k[5], code128<4>(w), code128<5>(w), s, s, off, off);
+  fma_pair(k[6], k[7], code128<6>(w), code128<7>(w), s, s, off, off);
+#pragma unroll
+  for (int j = 0; j < 4; ++j) split_pair<BF16>(k[2 * j], k[2 * j + 1], hi[j], lo[j]);
 }
 
 // Eight values of a token, scale * code + minimum rounded once, in the order 0 4 1 5 2 6 3 7 (codes four nibbles apart come out of a
@@ -120,7 +138,7 @@ template <bool BF16>
 __device__ __forceinline__ void store_k_unit(uint32_t hi_tile, uint32_t lo_tile, const Unit& x, int u, int lane) {
   const int r = u * 8 + (lane >> 2), g = lane & 3, flip = g & 2;
   const uint32_t w[4] = {flip ? x.w.z : x.w.x, flip ? x.w.w : x.w.y, flip ? x.w.x : x.w.z, flip ? x.w.y : x.w.w};
-  const float s = number<BF16>(x.scale), off = fmaf(-16.f, s, number<BF16>(x.mn));
+  const float s = number<BF16>(x.scale), off = fmaf(-128.f, s, number<BF16>(x.mn));
 #pragma unroll
   for (int k = 0; k < 4; ++k) {
     uint32_t hi[4], lo[4];
@@ -141,6 +159,35 @@ __device__ __forceinline__ void store_v_unit(uint32_t tile, const Unit& x, int u
     values_of_word<BF16>(w[k], s2, m2, v);
     sts128(chunk_at(tile, r, g * 4 + (k ^ flip)), v[0], v[1], v[2], v[3]);
   }
+}
+
+__device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int c0, int c1, int c2, int c3, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.4d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4, %5}], [%6];"
+      ::"r"(dst), "l"(tmap), "r"(c0), "r"(c1), "r"(c2), "r"(c3), "r"(ptx::smem_u32(bar))
+      : "memory");
+}
+
+// Queries [B,L,Hq,128] as a map (channel, head, query, batch row) whose box is 64 channels of the heads of a KV head for
+// `queries` queries: rows of 128 bytes in query-major order, the panel layout above.
+inline bool query_map(CUtensorMap* m, const cq_chunk_args* a, int queries) {
+  typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+  static const Encode encode = []() -> Encode {
+    void* p = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
+    return reinterpret_cast<Encode>(p);
+  }();
+  if (!encode) return false;
+  const cuuint64_t dims[4] = {128, (cuuint64_t)a->n_q_heads, (cuuint64_t)a->q_len, (cuuint64_t)a->batch};
+  const int64_t step[3] = {a->q_strides[2], a->q_strides[1], a->q_strides[0]};
+  cuuint64_t strides[3];
+  for (int i = 0; i < 3; ++i) strides[i] = dims[i + 1] == 1 ? 256 : (cuuint64_t)step[i] * 2;      // an extent of one: any
+  const cuuint32_t box[4] = {64, (cuuint32_t)(a->n_q_heads / a->n_kv_heads), (cuuint32_t)queries, 1}, one[4] = {1, 1, 1, 1};
+  return encode(m, a->dtype == CQ_DTYPE_BF16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT16, 4, const_cast<void*>(a->q), dims,
+                strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 // Instruction descriptor with the majors of both operands (0: K, 1: M or N contiguous).

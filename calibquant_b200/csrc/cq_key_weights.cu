@@ -4,10 +4,12 @@
 // stays in one thread and no exchange is needed.  A CTA holds two key tiles of 128 (packed keys as two 16-bit terms, exact as there) and
 // goes over the query rows of their KV head in blocks of NB.  Roles:
 //   warps 0-3 / 4-7  sums of key tile 0 / 1: thread = key
-//   warps 8-15       operands: the key tiles once, then the query blocks through two slots (requested a block ahead)
+//   warps 8-15       the key tiles, once; then one lane has TMA bring the query blocks into two slots
 //   warp 16          issues the products
+// A block is the query heads of the KV head for as many queries as NB rows hold: a row of a block is the same head for every block.
 // TMEM: tile X's scores in columns X * 256 + buffer * 128.  Where the key tiles are fewer than the SMs, the rows are cut into parts whose
 // sums finish_kernel adds in their order.
+#include <cuda.h>
 #include <math.h>
 
 #include <type_traits>
@@ -34,7 +36,7 @@ struct WeightParams {
   float *vis, *fp;
   int64_t capacity;          // full-precision weights per (batch row, KV head)
   int64_t batch;
-  int parts;
+  int parts, block_rows, block_queries;      // block_rows = block_queries * n_rep <= NB
   float* part;               // [part][batch][KV head][t_vis + capacity]
   float scale;
   uint32_t idesc_kmajor, idesc_mn;
@@ -47,17 +49,6 @@ __device__ __forceinline__ float ex2_approx(float x) {
   return y;
 }
 __device__ __forceinline__ void tile_barrier(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
-// (x0, x1) = (a0, a1) * (b, b) + (c0, c1)
-__device__ __forceinline__ void fma_pair(float& x0, float& x1, float a0, float a1, float b, float c0, float c1) {
-  asm("{\n\t.reg .b64 ra, rb, rc, rd;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rb, {%4, %4};\n\tmov.b64 rc, {%5, %6};\n\t"
-      "fma.rn.f32x2 rd, ra, rb, rc;\n\tmov.b64 {%0, %1}, rd;\n\t}"
-      : "=f"(x0), "=f"(x1) : "f"(a0), "f"(a1), "f"(b), "f"(c0), "f"(c1));
-}
-__device__ __forceinline__ void add_pair(float& s0, float& s1, float a0, float a1) {
-  asm("{\n\t.reg .b64 ra, rs;\n\tmov.b64 ra, {%2, %3};\n\tmov.b64 rs, {%0, %1};\n\tadd.rn.f32x2 rs, rs, ra;\n\tmov.b64 {%0, %1}, rs;\n\t}"
-      : "+f"(s0), "+f"(s1) : "f"(a0), "f"(a1));
-}
-
 // result of key `key` (cache order [visual | fp]) of KV head bh
 __device__ __forceinline__ void put(const WeightParams& a, int64_t bh, int64_t key, float w) {
   const int64_t vis = bh * a.p.t_vis + key, fp = bh * a.capacity + key - a.p.t_vis;
@@ -66,7 +57,7 @@ __device__ __forceinline__ void put(const WeightParams& a, int64_t bh, int64_t k
 }
 
 template <bool BF16, bool MASK, int NB>
-__global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_constant__ WeightParams a) {
+__global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ WeightParams a) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   const Params& p = a.p;
   extern __shared__ unsigned char smem_raw[];
@@ -86,17 +77,17 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
   const auto first_key = [&](int x) { return tile0 + x < nv ? (tile0 + x) * 128 : p.t_vis + (tile0 + x - nv) * 128; };
   const auto alive = [&](int x) { return tile0 + x < nv || (tile0 + x - nv) * 128 < live; };
   const auto first_row = [&](int t) { return (int64_t)max(0, t - live + p.q_len) * p.n_rep; };      // of full-precision token t
-  const int blocks_all = (p.rows + NB - 1) / NB, per = (blocks_all + (int)gridDim.z - 1) / (int)gridDim.z;
+  const int blocks_all = (p.q_len + a.block_queries - 1) / a.block_queries, per = (blocks_all + (int)gridDim.z - 1) / (int)gridDim.z;
   int blk0 = min(blocks_all, (int)blockIdx.z * per);
   const int blk1 = min(blocks_all, blk0 + per);
-  if (tile0 >= nv) blk0 = max(blk0, (int)min((int64_t)blk1, first_row((tile0 - nv) * 128) / NB));
+  if (tile0 >= nv) blk0 = max(blk0, (int)min((int64_t)blk1, first_row((tile0 - nv) * 128) / a.block_rows));
   const int n_x = !alive(0) ? 0 : alive(1) ? 2 : 1, nb = n_x ? blk1 - blk0 : 0;
   pdl_launch_dependents();
 
   if (tid == 0) {
     mbar_init(&bar_k, PRODUCERS);
     for (int s = 0; s < 2; ++s) {
-      mbar_init(&bar_q[s], PRODUCERS);
+      mbar_init(&bar_q[s], 1);
       mbar_init(&bar_free[s], 1);
       for (int x = 0; x < 2; ++x) {
         mbar_init(&bar_d[x][s], 1);
@@ -114,19 +105,6 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
   if (warp >= 8 && warp < MMA_WARP) {
     // ================= operands =================
     const int pw = warp - 8, ptid = tid - 256;
-    constexpr int CH = NB / 16;                  // chunks of a block per thread
-    uint4 v[CH];
-    const auto request = [&](int blk) {
-#pragma unroll
-      for (int it = 0; it < CH; ++it) {
-        const int row = blk * NB + it * 16 + (ptid >> 4);
-        v[it] = make_uint4(0, 0, 0, 0);
-        if (row < p.rows) {
-          const int i = row / p.n_rep, h = hk * p.n_rep + row % p.n_rep;
-          v[it] = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_st + h * p.q_sh + (ptid & 15) * 8);
-        }
-      }
-    };
     if (nb > 0) {
       for (int x = 0; x < n_x; ++x) {
         const uint32_t hi = k_s + x * 2 * TILE_BYTES, lo = hi + TILE_BYTES;
@@ -147,26 +125,27 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
           }
         }
       }
+      // rows of a block that no query fills are zeros for good
+      for (int c = a.block_rows * 8 + ptid; c < NB * 8; c += 256)
+        for (int s = 0; s < 4; ++s) sts128(q_s + s * PANEL_BYTES + c * 16, 0, 0, 0, 0);
       fence_proxy_async_smem();
       __syncwarp();
       if (lane == 0) mbar_arrive(&bar_k);
-      request(blk0);
     }
-    bool ok = true;
-    for (int n = 0; n < nb && ok; ++n) {
-      const int s = n & 1;
-      if (n >= 2) ok = mbar_wait_bounded(&bar_free[s], ((n >> 1) - 1) & 1, WAIT_TRIES);
-      ok = __all_sync(0xffffffffu, ok);
-      if (!ok) break;
-#pragma unroll
-      for (int it = 0; it < CH; ++it)
-        sts128(chunk_at(q_s + s * TILE_BYTES, it * 16 + (ptid >> 4), ptid & 15), v[it].x, v[it].y, v[it].z, v[it].w);
-      if (n + 1 < nb) request(blk0 + n + 1);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar_q[s]);
+    if (pw == 0 && lane == 0) {
+      bool ok = true;
+      for (int n = 0; n < nb && ok; ++n) {
+        const int s = n & 1;
+        if (n >= 2) ok = mbar_wait_bounded(&bar_free[s], ((n >> 1) - 1) & 1, WAIT_TRIES);
+        if (!ok) break;
+        mbar_expect_tx(&bar_q[s], 256 * a.block_rows);
+        const int i0 = (blk0 + n) * a.block_queries;
+        tma_load_4d(q_s + s * TILE_BYTES, &tm_q, 0, hk * p.n_rep, i0, b, &bar_q[s]);
+        tma_load_4d(q_s + s * TILE_BYTES + PANEL_BYTES, &tm_q, 64, hk * p.n_rep, i0, b, &bar_q[s]);
+      }
+      if (!ok) atomicExch(a.status, CQ_ERR_TIMEOUT);
     }
-    if (!ok && lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
+    __syncwarp();
   } else if (warp == MMA_WARP) {
     // ================= products =================
     const uint32_t lead = elect_one();
@@ -184,17 +163,17 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
         tc_fence_after();
         if (lead) {
           const uint32_t d = tm + (uint32_t)(x * 256 + s * 128);
-          const bool packed = tile0 + x < nv;
+          const bool packed = tile0 + x < nv;      // its small terms first: sums are cut off, not rounded
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
             const uint64_t qo = (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4), q = qd + s * tile16 + qo;
-            if (packed) umma(d, md + 2 * x * tile16 + (uint64_t)(ks * 128), q, a.idesc_mn, ks > 0);
+            if (packed) umma(d, md + (2 * x + 1) * tile16 + (uint64_t)(ks * 128), q, a.idesc_mn, ks > 0);
             else umma(d, kd + 2 * x * tile16 + qo, q, a.idesc_kmajor, ks > 0);
           }
           if (packed) {
 #pragma unroll
             for (int ks = 0; ks < 8; ++ks)
-              umma(d, md + (2 * x + 1) * tile16 + (uint64_t)(ks * 128), qd + s * tile16 + (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4), a.idesc_mn, 1);
+              umma(d, md + 2 * x * tile16 + (uint64_t)(ks * 128), qd + s * tile16 + (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4), a.idesc_mn, 1);
           }
           umma_commit(&bar_d[x][s]);
         }
@@ -218,10 +197,12 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
     bool ok = true;
     float acc[4] = {};
     // minus the rows' log-sum-exp in units of the exponent (log-sum-exp as it is with a mask); a row that adds nothing: -inf
+    const int i_in = r_in / p.n_rep;
+    const float* lse_row = p.lse + ((int64_t)b * p.hq + hk * p.n_rep + r_in % p.n_rep) * p.q_len;
     const auto lse_of = [&](int n) {
-      const int row = (blk0 + n) * NB + r_in;
-      if (r_in >= NB || n >= nb || row >= p.rows) return MASK ? INFINITY : -INFINITY;
-      const float v = p.lse[((int64_t)b * p.hq + hk * p.n_rep + row % p.n_rep) * p.q_len + row / p.n_rep];
+      const int i = (blk0 + n) * a.block_queries + i_in;
+      if (r_in >= a.block_rows || n >= nb || i >= p.q_len) return MASK ? INFINITY : -INFINITY;
+      const float v = lse_row[i];
       if (v == -INFINITY) return MASK ? INFINITY : -INFINITY;
       return MASK ? v : -v * LOG2E;
     };
@@ -234,7 +215,7 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
         tile_barrier(1 + x);
         if (ok) ok = mbar_wait_cycles(&bar_d[x][s], (n >> 1) & 1, WAIT_CYCLES);
         tc_fence_after();
-        const int64_t r0 = (int64_t)(blk0 + n) * NB;
+        const int64_t r0 = (int64_t)(blk0 + n) * a.block_rows;
         const bool need = __any_sync(0xffffffffu, rmin > r0);
         const int hidden = (int)min((int64_t)NB, rmin - r0);            // columns below are not seen
 #pragma unroll
@@ -255,8 +236,8 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
               e[2] = (fmaf(__uint_as_float(d[c + 2]), a.scale, m) - l.z) * LOG2E;
               e[3] = (fmaf(__uint_as_float(d[c + 3]), a.scale, m) - l.w) * LOG2E;
             } else {
-              fma_pair(e[0], e[1], __uint_as_float(d[c]), __uint_as_float(d[c + 1]), c1, l.x, l.y);
-              fma_pair(e[2], e[3], __uint_as_float(d[c + 2]), __uint_as_float(d[c + 3]), c1, l.z, l.w);
+              fma_pair(e[0], e[1], __uint_as_float(d[c]), __uint_as_float(d[c + 1]), c1, c1, l.x, l.y);
+              fma_pair(e[2], e[3], __uint_as_float(d[c + 2]), __uint_as_float(d[c + 3]), c1, c1, l.z, l.w);
             }
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -296,15 +277,17 @@ __global__ void __launch_bounds__(256) key_weights_finish_kernel(WeightParams a)
 
 // ---- host ---------------------------------------------------------------------------------------------------------
 struct Plan {
-  int nb, pairs, parts;
+  int nb, queries, pairs, parts;      // queries of a block
 };
 static Plan make_plan(const cq_chunk_args* a, int64_t capacity) {
   Plan pl;
   const int64_t rows = (int64_t)a->q_len * (a->n_q_heads / a->n_kv_heads);
+  const int n_rep = a->n_q_heads / a->n_kv_heads;
   pl.nb = rows <= 32 ? 32 : 128;
+  pl.queries = pl.nb / n_rep;
   pl.pairs = (int)(((a->t_vis + 127) / 128 + (capacity + 127) / 128 + 1) / 2);
   // CTAs for the keys alone leave SMs idle: rows in parts, each of four blocks at least
-  const int64_t ctas = (int64_t)a->batch * a->n_kv_heads * pl.pairs, blocks = (rows + pl.nb - 1) / pl.nb;
+  const int64_t ctas = (int64_t)a->batch * a->n_kv_heads * pl.pairs, blocks = (a->q_len + pl.queries - 1) / pl.queries;
   int64_t parts = ctas > 0 ? sm_count() / ctas : 1;
   if (parts > blocks / 4) parts = blocks / 4;
   pl.parts = (int)(parts < 1 ? 1 : parts > 16 ? 16 : parts);
@@ -315,7 +298,7 @@ static size_t bytes_of(const cq_chunk_args* a, int64_t capacity, const Plan& pl)
 }
 
 template <bool BF16, bool MASK, int NB>
-static int run(const WeightParams& p, const Plan& pl, cudaStream_t st) {
+static int run(const CUtensorMap& tm, const WeightParams& p, const Plan& pl, cudaStream_t st) {
   static bool configured[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CQ_ERR_LAUNCH;
@@ -324,7 +307,7 @@ static int run(const WeightParams& p, const Plan& pl, cudaStream_t st) {
     configured[dev] = true;
   }
   const unsigned bh = (unsigned)(p.batch * p.p.hkv);
-  key_weights_kernel<BF16, MASK, NB><<<dim3(pl.pairs, bh, pl.parts), THREADS, SMEM_BYTES, st>>>(p);
+  key_weights_kernel<BF16, MASK, NB><<<dim3(pl.pairs, bh, pl.parts), THREADS, SMEM_BYTES, st>>>(tm, p);
   if (const int rc = check_launch()) return rc;
   if (pl.parts == 1) return CQ_OK;
   return launched(launch_pdl(key_weights_finish_kernel, dim3((unsigned)((p.p.t_vis + p.capacity + 255) / 256), bh), dim3(256), 0, st, p));
@@ -360,11 +343,14 @@ extern "C" int cq_key_weights(const cq_chunk_args* a, const float* w_vis_in, con
   p.capacity = w_capacity; p.batch = a->batch; p.parts = pl.parts;
   p.part = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
   p.scale = 0.08838834764831845f;
+  p.block_queries = pl.queries; p.block_rows = pl.queries * p.p.n_rep;
+  CUtensorMap tm;
+  if (!chunk::query_map(&tm, a, pl.queries)) return CQ_ERR_LAUNCH;
   p.idesc_kmajor = chunk::idesc_of(bf16, 0, 0, 128, pl.nb);
   p.idesc_mn = chunk::idesc_of(bf16, 1, 0, 128, pl.nb);
   p.status = static_cast<int*>(workspace);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define CQ_RUN(B, M) (pl.nb == 32 ? run<B, M, 32>(p, pl, st) : run<B, M, 128>(p, pl, st))
+#define CQ_RUN(B, M) (pl.nb == 32 ? run<B, M, 32>(tm, p, pl, st) : run<B, M, 128>(tm, p, pl, st))
   if (bf16) return a->mask ? CQ_RUN(true, true) : CQ_RUN(true, false);
   return a->mask ? CQ_RUN(false, true) : CQ_RUN(false, false);
 #undef CQ_RUN

@@ -507,10 +507,11 @@ int cq_qjl_gqa_score(const uint8_t* key_quant, const uint8_t* key_outlier_quant,
  * A key whose mask is -infinity takes no part, whatever its key and value hold; a row without keys gives out 0, lse -infinity.
  * The scores are exact but for their fp32 sums (packed keys are multiplied as two terms), values and probabilities are rounded to
  * `dtype` for the second product.  No calibration of logits (calibrate = 0 of cq_decode_attn).
- *   q, out  element (b,i,h,d) at base + b*strides[0] + i*strides[1] + h*strides[2] + d (strides in elements, multiples of 8)
+ *   q, out  element (b,i,h,d) at base + b*strides[0] + i*strides[1] + h*strides[2] + d (strides in elements, multiples of 8, above
+ *           zero where the extent is above one)
  *   lse     fp32 [B,Hq,q_len], or NULL
  * bits == 4, group_size == 32, head_dim == 128, t_vis a multiple of 32 (0: no packed operands), 0 < q_len <= t_fp, every
- * pointer 16-byte aligned (mask 2-byte), any number of query heads per KV head.
+ * pointer 16-byte aligned (mask 2-byte), up to 128 query heads per KV head.
  * The first word of the workspace is a sticky status word as in cq_decode_attn; two calls that overlap on the GPU need two workspaces.
  */
 typedef struct cq_chunk_args {
