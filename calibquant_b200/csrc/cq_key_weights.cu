@@ -3,9 +3,10 @@
 // The scores are formed the other way round than for the attention, S^T = K Q^T: a TMEM lane per key, so that a key's sum over the queries
 // stays in one thread and no exchange is needed.  A CTA holds two key tiles of 128 (packed keys as two 16-bit terms, exact as there) and
 // goes over the query rows of their KV head in blocks of NB.  Roles:
-//   warps 0-3 / 4-7  sums of key tile 0 / 1: thread = key
-//   warps 8-15       the key tiles, once; then one lane has TMA bring the query blocks into two slots
-//   warp 16          issues the products
+//   warps 0-15  the key tiles, once; then the sums: a thread has a key and every other 32 (16) of a block's rows, warps 0-3, 8-11 tile 0,
+//               4-7, 12-15 tile 1
+//   warp 16     issues the products
+//   warp 17     has TMA bring the query blocks into two slots
 // A block is the query heads of the KV head for as many queries as NB rows hold: a row of a block is the same head for every block.
 // TMEM: tile X's scores in columns X * 256 + buffer * 128.  Where the key tiles are fewer than the SMs, the rows are cut into parts whose
 // sums finish_kernel adds in their order.
@@ -24,7 +25,8 @@ using namespace tc;
 
 namespace kw {
 
-constexpr int PRODUCERS = 8, MMA_WARP = 16, THREADS = 17 * 32;
+constexpr int WORKERS = 16, MMA_WARP = 16, TMA_WARP = 17, THREADS = 18 * 32;
+constexpr int LSE_BLOCKS = 16;             // blocks whose rows' log-sum-exp are in shared memory at a time
 constexpr int SMEM_BYTES = 6 * TILE_BYTES + 1024;
 constexpr uint32_t WAIT_TRIES = 1u << 22;
 constexpr long long WAIT_CYCLES = 1ll << 30;
@@ -48,7 +50,7 @@ __device__ __forceinline__ float ex2_approx(float x) {
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
-__device__ __forceinline__ void tile_barrier(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+__device__ __forceinline__ void worker_barrier() { asm volatile("bar.sync 1, 512;" ::: "memory"); }
 // result of key `key` (cache order [visual | fp]) of KV head bh
 __device__ __forceinline__ void put(const WeightParams& a, int64_t bh, int64_t key, float w) {
   const int64_t vis = bh * a.p.t_vis + key, fp = bh * a.capacity + key - a.p.t_vis;
@@ -66,7 +68,8 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
   // bar_k the key tiles are there; bar_q/free[slot] query blocks; bar_d/dfree[X][buffer] scores ready / read
   __shared__ __align__(8) uint64_t bar_k, bar_q[2], bar_free[2], bar_d[2][2], bar_dfree[2][2];
   __shared__ uint32_t tmem_base_s;
-  __shared__ __align__(16) float lse_s[2][2][NB];
+  __shared__ __align__(16) float lse_s[LSE_BLOCKS * NB];
+  __shared__ float half_s[256];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hk = blockIdx.y % p.hkv, b = blockIdx.y / p.hkv;
@@ -85,13 +88,13 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
   pdl_launch_dependents();
 
   if (tid == 0) {
-    mbar_init(&bar_k, PRODUCERS);
+    mbar_init(&bar_k, WORKERS);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bar_q[s], 1);
       mbar_init(&bar_free[s], 1);
       for (int x = 0; x < 2; ++x) {
         mbar_init(&bar_d[x][s], 1);
-        mbar_init(&bar_dfree[x][s], 128);
+        mbar_init(&bar_dfree[x][s], 256);
       }
     }
     mbar_fence_init();
@@ -102,40 +105,13 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
   tc_fence_after();
   const uint32_t tmem = tmem_base_s;
 
-  if (warp >= 8 && warp < MMA_WARP) {
-    // ================= operands =================
-    const int pw = warp - 8, ptid = tid - 256;
-    if (nb > 0) {
-      for (int x = 0; x < n_x; ++x) {
-        const uint32_t hi = k_s + x * 2 * TILE_BYTES, lo = hi + TILE_BYTES;
-        if (tile0 + x < nv) {
-          Unit u[2];
-          load_k_unit(p, bh, tile0 + x, pw, lane, u[0]);
-          load_k_unit(p, bh, tile0 + x, pw + 8, lane, u[1]);
-          store_k_unit<BF16>(hi, lo, u[0], pw, lane);
-          store_k_unit<BF16>(hi, lo, u[1], pw + 8, lane);
-        } else {
-          const T* src = static_cast<const T*>(p.k_fp) + b * p.fp_sb + hk * p.fp_sh;
-#pragma unroll
-          for (int it = 0; it < 8; ++it) {
-            const int r = it * 16 + (ptid >> 4), t = (tile0 + x - nv) * 128 + r;
-            uint4 w = make_uint4(0, 0, 0, 0);
-            if (t < live) w = *reinterpret_cast<const uint4*>(src + (int64_t)t * 128 + (ptid & 15) * 8);
-            sts128(chunk_at(hi, r, ptid & 15), w.x, w.y, w.z, w.w);
-          }
-        }
-      }
-      // rows of a block that no query fills are zeros for good
-      for (int c = a.block_rows * 8 + ptid; c < NB * 8; c += 256)
-        for (int s = 0; s < 4; ++s) sts128(q_s + s * PANEL_BYTES + c * 16, 0, 0, 0, 0);
-      fence_proxy_async_smem();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&bar_k);
-    }
-    if (pw == 0 && lane == 0) {
+  if (warp == TMA_WARP) {
+    // ================= query blocks =================
+    if (lane == 0) {
       bool ok = true;
       for (int n = 0; n < nb && ok; ++n) {
         const int s = n & 1;
+        // rows of a block that no query fills are zeros for good: written before bar_k
         if (n >= 2) ok = mbar_wait_bounded(&bar_free[s], ((n >> 1) - 1) & 1, WAIT_TRIES);
         if (!ok) break;
         mbar_expect_tx(&bar_q[s], 256 * a.block_rows);
@@ -182,9 +158,36 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
     }
     if (!ok && lead) atomicExch(a.status, CQ_ERR_TIMEOUT);
     __syncwarp();
-  } else if (warp < 8) {
+  } else {
+    // ================= the key tiles =================
+    if (nb > 0) {
+      for (int x = 0; x < n_x; ++x) {
+        const uint32_t hi = k_s + x * 2 * TILE_BYTES, lo = hi + TILE_BYTES;
+        if (tile0 + x < nv) {
+          Unit u;
+          load_k_unit(p, bh, tile0 + x, warp, lane, u);
+          store_k_unit<BF16>(hi, lo, u, warp, lane);
+        } else {
+          const T* src = static_cast<const T*>(p.k_fp) + b * p.fp_sb + hk * p.fp_sh;
+#pragma unroll
+          for (int it = 0; it < 4; ++it) {
+            const int r = it * 32 + (tid >> 4), t = (tile0 + x - nv) * 128 + r;
+            uint4 w = make_uint4(0, 0, 0, 0);
+            if (t < live) w = *reinterpret_cast<const uint4*>(src + (int64_t)t * 128 + (tid & 15) * 8);
+            sts128(chunk_at(hi, r, tid & 15), w.x, w.y, w.z, w.w);
+          }
+        }
+      }
+      // rows of a block that no query fills
+      for (int c = a.block_rows * 8 + tid; c < NB * 8; c += 512)
+        for (int s = 0; s < 4; ++s) sts128(q_s + s * PANEL_BYTES + c * 16, 0, 0, 0, 0);
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&bar_k);
+    }
     // ================= sums: thread = key =================
-    const int x = warp >> 2, r_in = (warp & 3) * 32 + lane;
+    constexpr int COLS = NB / 4;                                        // columns at a time; a half takes the even or the odd ones of four
+    const int x = (warp >> 2) & 1, half = warp >> 3, r_in = (warp & 3) * 32 + lane;
     const int64_t key = first_key(x) + r_in;
     const bool vis = tile0 + x < nv;
     const int t = (int)(key - p.t_vis);                                 // full-precision token
@@ -196,68 +199,79 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
     const float c1 = a.scale * LOG2E;
     bool ok = true;
     float acc[4] = {};
-    // minus the rows' log-sum-exp in units of the exponent (log-sum-exp as it is with a mask); a row that adds nothing: -inf
-    const int i_in = r_in / p.n_rep;
-    const float* lse_row = p.lse + ((int64_t)b * p.hq + hk * p.n_rep + r_in % p.n_rep) * p.q_len;
-    const auto lse_of = [&](int n) {
-      const int i = (blk0 + n) * a.block_queries + i_in;
-      if (r_in >= a.block_rows || n >= nb || i >= p.q_len) return MASK ? INFINITY : -INFINITY;
-      const float v = lse_row[i];
-      if (v == -INFINITY) return MASK ? INFINITY : -INFINITY;
-      return MASK ? v : -v * LOG2E;
-    };
-    if (x < n_x && nb > 0) {
-      float next = lse_of(0);
-      for (int n = 0; n < nb; ++n) {
+    for (int n0 = 0; n0 < nb; n0 += LSE_BLOCKS) {
+      // minus the rows' log-sum-exp in units of the exponent (log-sum-exp as it is with a mask); a row that adds nothing: -inf
+      worker_barrier();
+      for (int c = tid; c < LSE_BLOCKS * NB; c += 512) {
+        const int r = c % NB, i = (blk0 + n0 + c / NB) * a.block_queries + r / p.n_rep;
+        float v = -INFINITY;
+        if (r < a.block_rows && n0 + c / NB < nb && i < p.q_len) v = p.lse[((int64_t)b * p.hq + hk * p.n_rep + r % p.n_rep) * p.q_len + i];
+        lse_s[c] = v == -INFINITY ? (MASK ? INFINITY : -INFINITY) : MASK ? v : -v * LOG2E;
+      }
+      worker_barrier();
+      if (x >= n_x) continue;
+      for (int n = n0; n < min(nb, n0 + LSE_BLOCKS); ++n) {
         const int s = n & 1;
-        if (r_in < NB) lse_s[x][s][r_in] = next;
-        next = lse_of(n + 1);
-        tile_barrier(1 + x);
         if (ok) ok = mbar_wait_cycles(&bar_d[x][s], (n >> 1) & 1, WAIT_CYCLES);
         tc_fence_after();
-        const int64_t r0 = (int64_t)(blk0 + n) * a.block_rows;
-        const bool need = __any_sync(0xffffffffu, rmin > r0);
-        const int hidden = (int)min((int64_t)NB, rmin - r0);            // columns below are not seen
-#pragma unroll
-        for (int cc = 0; cc < NB / 32; ++cc) {
-          uint32_t d[32];
-          tmem_ld32(tD + s * 128 + cc * 32, d);
-          if (cc == NB / 32 - 1) {
-            tc_fence_before();
-            mbar_arrive(&bar_dfree[x][s]);
-          }
-#pragma unroll
-          for (int c = 0; c < 32; c += 4) {
-            const float4 l = *reinterpret_cast<const float4*>(&lse_s[x][s][cc * 32 + c]);
-            float e[4];
-            if (MASK) {
-              e[0] = (fmaf(__uint_as_float(d[c]), a.scale, m) - l.x) * LOG2E;
-              e[1] = (fmaf(__uint_as_float(d[c + 1]), a.scale, m) - l.y) * LOG2E;
-              e[2] = (fmaf(__uint_as_float(d[c + 2]), a.scale, m) - l.z) * LOG2E;
-              e[3] = (fmaf(__uint_as_float(d[c + 3]), a.scale, m) - l.w) * LOG2E;
-            } else {
-              fma_pair(e[0], e[1], __uint_as_float(d[c]), __uint_as_float(d[c + 1]), c1, c1, l.x, l.y);
-              fma_pair(e[2], e[3], __uint_as_float(d[c + 2]), __uint_as_float(d[c + 3]), c1, c1, l.z, l.w);
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              e[i] = ex2_approx(e[i]);
-              if (need && cc * 32 + c + i < hidden) e[i] = 0.f;
-            }
-            add_pair(acc[0], acc[1], e[0], e[1]);
-            add_pair(acc[2], acc[3], e[2], e[3]);
-          }
+        uint32_t d[2][COLS];
+        if constexpr (COLS == 32) {
+          tmem_ld32_nowait(tD + s * 128 + half * 32, d[0]);
+          tmem_ld32_nowait(tD + s * 128 + half * 32 + 64, d[1]);
+        } else {
+          tmem_ld8_nowait(tD + s * 128 + half * 8, d[0]);
+          tmem_ld8_nowait(tD + s * 128 + half * 8 + 16, d[1]);
         }
+        tmem_ld_wait();
+        tc_fence_before();
+        mbar_arrive(&bar_dfree[x][s]);
+        const int64_t hidden = rmin - (int64_t)(blk0 + n) * a.block_rows;      // columns below are not seen
+        const auto sum = [&](auto diagonal) {
+#pragma unroll
+          for (int cc = 0; cc < 2; ++cc) {
+            const int col0 = cc * 2 * COLS + half * COLS;
+            const float* l_s = lse_s + (n - n0) * NB + col0;
+#pragma unroll
+            for (int c = 0; c < COLS; c += 4) {
+              const float4 l = *reinterpret_cast<const float4*>(l_s + c);
+              const float f[4] = {__uint_as_float(d[cc][c]), __uint_as_float(d[cc][c + 1]), __uint_as_float(d[cc][c + 2]), __uint_as_float(d[cc][c + 3])};
+              float e[4];
+              if (MASK) {
+                e[0] = (fmaf(f[0], a.scale, m) - l.x) * LOG2E;
+                e[1] = (fmaf(f[1], a.scale, m) - l.y) * LOG2E;
+                e[2] = (fmaf(f[2], a.scale, m) - l.z) * LOG2E;
+                e[3] = (fmaf(f[3], a.scale, m) - l.w) * LOG2E;
+              } else {
+                fma_pair(e[0], e[1], f[0], f[1], c1, c1, l.x, l.y);
+                fma_pair(e[2], e[3], f[2], f[3], c1, c1, l.z, l.w);
+              }
+#pragma unroll
+              for (int i = 0; i < 4; ++i) {
+                e[i] = ex2_approx(e[i]);
+                if (decltype(diagonal)::value && col0 + c + i < hidden) e[i] = 0.f;
+              }
+              add_pair(acc[0], acc[1], e[0], e[1]);
+              add_pair(acc[2], acc[3], e[2], e[3]);
+            }
+          }
+        };
+        if (__any_sync(0xffffffffu, hidden > 0)) sum(std::true_type{});
+        else sum(std::false_type{});
       }
-      if (!__all_sync(0xffffffffu, ok) && lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
     }
+    if (!__all_sync(0xffffffffu, ok) && lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
     float w = (acc[0] + acc[1]) + (acc[2] + acc[3]);
     if (!ok) w = NAN;
-    if (!there || (MASK && m == -INFINITY)) w = 0.f;
-    const int64_t end = vis ? p.t_vis : p.t_vis + a.capacity;
-    if (key < end) {
-      if (a.parts == 1) put(a, bh, key, w);
-      else a.part[((int64_t)blockIdx.z * a.batch * p.hkv + bh) * (p.t_vis + a.capacity) + key] = w;
+    if (half == 1) half_s[x * 128 + r_in] = w;
+    worker_barrier();
+    if (half == 0) {
+      w += half_s[x * 128 + r_in];
+      if (!there || (MASK && m == -INFINITY)) w = 0.f;
+      const int64_t end = vis ? p.t_vis : p.t_vis + a.capacity;
+      if (key < end) {
+        if (a.parts == 1) put(a, bh, key, w);
+        else a.part[((int64_t)blockIdx.z * a.batch * p.hkv + bh) * (p.t_vis + a.capacity) + key] = w;
+      }
     }
   }
   tc_fence_before();
