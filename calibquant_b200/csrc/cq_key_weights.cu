@@ -129,32 +129,48 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
     constexpr uint64_t tile16 = TILE_BYTES >> 4;
     const uint64_t kd = smem_desc(k_s, 16, 1024), md = smem_desc(k_s, PANEL_BYTES, 1024), qd = smem_desc(q_s, 16, 1024);
     const auto all = [](bool r) { return __all_sync(0xffffffffu, r) != 0; };
-    bool ok = nb == 0 || all(mbar_wait_bounded(&bar_k, 0, WAIT_TRIES));
-    for (int n = 0; n < nb && ok; ++n) {
-      const int s = n & 1;
-      ok = all(mbar_wait_bounded(&bar_q[s], (n >> 1) & 1, WAIT_TRIES));
-      for (int x = 0; x < n_x && ok; ++x) {
-        if (n >= 2) ok = all(mbar_wait_cycles(&bar_dfree[x][s], ((n >> 1) - 1) & 1, WAIT_CYCLES));
-        if (!ok) break;
-        tc_fence_after();
-        if (lead) {
-          const uint32_t d = tm + (uint32_t)(x * 256 + s * 128);
-          const bool packed = tile0 + x < nv;      // its small terms first: sums are cut off, not rounded
+    // slot and tile as constants: with both as indices the issuing lane's address arithmetic held up the tensor pipe
+    const auto issue = [&](auto xc, auto sc, bool packed) {
+      constexpr int x = decltype(xc)::value, s = decltype(sc)::value;
+      if (lead) {
+        if (packed) {
+          // its small terms first: sums are cut off, not rounded
+#pragma unroll
+          for (int ks = 0; ks < 16; ++ks) {
+            constexpr uint64_t lo = (2 * x + 1) * tile16, hi = 2 * x * tile16;
+            const uint64_t qo = (uint64_t)((((ks & 7) >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
+            umma(tm + (uint32_t)(x * 256 + s * 128), md + ((ks < 8 ? lo : hi) + (uint64_t)((ks & 7) * 128)), qd + (s * tile16 + qo), a.idesc_mn, ks > 0);
+          }
+        } else {
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
-            const uint64_t qo = (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4), q = qd + s * tile16 + qo;
-            if (packed) umma(d, md + (2 * x + 1) * tile16 + (uint64_t)(ks * 128), q, a.idesc_mn, ks > 0);
-            else umma(d, kd + 2 * x * tile16 + qo, q, a.idesc_kmajor, ks > 0);
+            const uint64_t qo = (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
+            umma(tm + (uint32_t)(x * 256 + s * 128), kd + (2 * x * tile16 + qo), qd + (s * tile16 + qo), a.idesc_kmajor, ks > 0);
           }
-          if (packed) {
-#pragma unroll
-            for (int ks = 0; ks < 8; ++ks)
-              umma(d, md + 2 * x * tile16 + (uint64_t)(ks * 128), qd + s * tile16 + (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4), a.idesc_mn, 1);
-          }
-          umma_commit(&bar_d[x][s]);
         }
+        umma_commit(&bar_d[x][s]);
       }
-      if (ok && lead) umma_commit(&bar_free[s]);
+    };
+    const bool packed0 = tile0 < nv, packed1 = tile0 + 1 < nv;
+    bool ok = nb == 0 || all(mbar_wait_bounded(&bar_k, 0, WAIT_TRIES));
+    const auto block = [&](auto sc, int n) {
+      constexpr int s = decltype(sc)::value;
+      ok = all(mbar_wait_bounded(&bar_q[s], (n >> 1) & 1, WAIT_TRIES));
+      if (ok && n >= 2) ok = all(mbar_wait_cycles(&bar_dfree[0][s], ((n >> 1) - 1) & 1, WAIT_CYCLES));
+      if (!ok) return;
+      tc_fence_after();
+      issue(std::integral_constant<int, 0>{}, sc, packed0);
+      if (n_x > 1) {
+        if (n >= 2) ok = all(mbar_wait_cycles(&bar_dfree[1][s], ((n >> 1) - 1) & 1, WAIT_CYCLES));
+        if (!ok) return;
+        tc_fence_after();
+        issue(std::integral_constant<int, 1>{}, sc, packed1);
+      }
+      if (lead) umma_commit(&bar_free[s]);
+    };
+    for (int n = 0; n < nb && ok; n += 2) {
+      block(std::integral_constant<int, 0>{}, n);
+      if (n + 1 < nb && ok) block(std::integral_constant<int, 1>{}, n + 1);
     }
     if (!ok && lead) atomicExch(a.status, CQ_ERR_TIMEOUT);
     __syncwarp();
