@@ -1,19 +1,22 @@
 // Attention of several new tokens over [system | visual (4-bit group format) | text] on the 5th-generation tensor cores.
 //
-// Rows are (query, head) pairs of one KV head, query major.  A CTA works on one KV head of one request with two 128-row tiles A and B
-// (a TMEM lane per row):
-//   PAIR    A and B are adjacent rows and share every key tile (more than 128 rows);
+// Rows are (query, head) pairs of one KV head, query major.  A tile holds as many whole queries as 128 rows take (a TMEM lane per row),
+// and a CTA works on one KV head of one request with two tiles A and B:
+//   PAIR    A and B are adjacent tiles and share every key tile (more queries than one tile takes);
 //   else    A and B are the SAME rows and take the even and the odd key tiles, two partial results.
 // The keys of a CTA are a part of the request's key tiles, visual ones first (`parts` on the grid); partial results are merged by
 // combine_kernel.  Roles:
 //   warps 0-3 / 4-7  softmax of A / B: thread = row; running maximum and sum, probabilities back to tensor memory
-//   warps 8-15       operands: codes from global memory (requested a tile ahead), unpacked into 16-bit tiles in a ring of five
-//                    shared-memory slots; full-precision rows into the same layout
+//   warps 8-15       operands: codes from global memory (requested two tiles ahead), unpacked into 16-bit tiles in shared memory: two
+//                    buffers of keys (two terms each) and one of values, two where there is one query tile; full-precision
+//                    rows into the same layout
 //   warp 16          issues the products
 // S = Q K^T with packed keys as two 16-bit terms (their sum is scale * code + minimum exactly), so scores carry no rounding but
 // that of fp32 sums; O += P V with P in tensor memory.  S_A [0,128) S_B [128,256) O_A [256,384) O_B [384,512) TMEM columns.
 // Every wait is bounded; one that runs out sets CQ_ERR_TIMEOUT in the workspace's first word, and the CTA ends.
 #include <math.h>
+
+#include <type_traits>
 
 #include "cq_chunk_tc.cuh"
 
@@ -23,17 +26,17 @@ namespace chunk {
 using namespace ptx;
 using namespace tc;
 
-constexpr int SLOTS = 5;
 constexpr int PRODUCERS = 8, MMA_WARP = 16, THREADS = 20 * 32;
 // registers: 256 x 120 + 256 x 88 + 128 x 64 = the launch's 640 x 96
 constexpr int SOFTMAX_REGS = 120, PRODUCER_REGS = 88, CONTROL_REGS = 64;
-constexpr int SMEM_BYTES = (2 + SLOTS) * TILE_BYTES + 1024;
+constexpr int SMEM_BYTES = 7 * TILE_BYTES + 1024;
 constexpr uint32_t WAIT_TRIES = 1u << 22;
 constexpr long long WAIT_CYCLES = 1ll << 30;
 constexpr float LOG2E = 1.4426950408889634f;
 
 struct AttnParams {
   Params p;
+  int tile_queries, tile_rows;      // of a tile
   int parts;                 // partial results per row (1: the kernel writes the output itself)
   float scale;               // 1 / sqrt(128)
   uint32_t idesc_kmajor, idesc_mn;
@@ -64,44 +67,37 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
 }
 __device__ __forceinline__ void tile_barrier(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
 
-// Ring position of a role: slot and how often it has come round.
-struct Ring {
-  uint32_t slot = 0, round = 0;
-  __device__ __forceinline__ void next() {
-    if (++slot == SLOTS) { slot = 0; ++round; }
-  }
-};
-
 // Key tiles of a CTA: visual tiles [0, nv), full-precision ones [nv, n_all); this CTA's are [t0, t0 + n).
 struct Range {
   int nv, t0, n;
 };
 
 template <bool BF16, bool MASK, bool PAIR>
-__global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_constant__ AttnParams a) {
+__global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ AttnParams a) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   const Params& p = a.p;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  const uint32_t q_s = smem_u32(smem), ring_s = q_s + 2 * TILE_BYTES;
-  // bar_q (once); bar_full/free[slot]; bar_s[X] scores of X ready; bar_p[X][half] probabilities of keys 0-63 / 64-127 stored;
+  constexpr int QT = PAIR ? 2 : 1;      // query tiles
+  const uint32_t q_s = smem_u32(smem), k_s = q_s + QT * TILE_BYTES, v_s = k_s + 4 * TILE_BYTES;      // keys: [buffer][large terms, small ones]
+  // bar_q (once); bar_k / bar_v[buffer] full, bar_kfree / bar_vfree read; bar_s[X] scores of X ready; bar_p[X][half] probabilities of keys 0-63 / 64-127 stored;
   // bar_pv[X] the tile's P V done
-  __shared__ __align__(8) uint64_t bar_q, bar_full[SLOTS], bar_free[SLOTS], bar_s[2], bar_p[2][2], bar_pv[2];
+  __shared__ __align__(8) uint64_t bar_q, bar_k[2], bar_kfree[2], bar_v[2], bar_vfree[2], bar_s[2], bar_p[2][2], bar_pv[2];
   __shared__ uint32_t tmem_base_s;
   __shared__ __align__(16) T mask_s[MASK ? 2 : 1][MASK ? 2 : 1][MASK ? 128 : 8];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hk = blockIdx.y % p.hkv, b = blockIdx.y / p.hkv, part = blockIdx.z;
   const int64_t bh = (int64_t)b * p.hkv + hk;
-  const int row0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * (PAIR ? 256 : 128);      // rows that see most keys first
+  const int i0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * (PAIR ? 2 : 1) * a.tile_queries;      // first query; those that see most keys first
 
   if (tid == 0) {
-    mbar_init(&bar_q, PRODUCERS);
-    for (int s = 0; s < SLOTS; ++s) {
-      mbar_init(&bar_full[s], PRODUCERS);
-      mbar_init(&bar_free[s], 1);
-    }
+    mbar_init(&bar_q, PRODUCERS + 1);
     for (int x = 0; x < 2; ++x) {
+      mbar_init(&bar_k[x], PRODUCERS);
+      mbar_init(&bar_kfree[x], 1);
+      mbar_init(&bar_v[x], PRODUCERS);
+      mbar_init(&bar_vfree[x], 1);
       mbar_init(&bar_s[x], 1);
       mbar_init(&bar_p[x][0], 128);
       mbar_init(&bar_p[x][1], 128);
@@ -119,8 +115,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
 
   Range k;
   {
-    const int last = min(row0 + (PAIR ? 256 : 128), p.rows) - 1;
-    const int n_fp = max(0, live - p.q_len + last / p.n_rep + 1);      // full-precision tokens that the last row sees
+    const int last = min(i0 + (PAIR ? 2 : 1) * a.tile_queries, p.q_len) - 1;
+    const int n_fp = max(0, live - p.q_len + last + 1);      // full-precision tokens that the last query sees
     k.nv = (p.t_vis + 127) >> 7;
     const int n_all = k.nv + ((n_fp + 127) >> 7), grid_parts = gridDim.z, per = (n_all + grid_parts - 1) / grid_parts;
     k.t0 = min(n_all, part * per);
@@ -132,56 +128,47 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
     setmaxnreg_dec<PRODUCER_REGS>();
     const int pw = warp - 8, ptid = tid - 256;
     bool ok = true;
-    // the queries; rows past the end are zeros
-    for (int x = 0; x < (PAIR ? 2 : 1); ++x) {
-#pragma unroll 4
-      for (int it = 0; it < 8; ++it) {
-        const int r = it * 16 + (ptid >> 4), c = ptid & 15, row = row0 + x * 128 + r;
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (row < p.rows) {
-          const int i = row / p.n_rep, h = hk * p.n_rep + row % p.n_rep;
-          v = *reinterpret_cast<const uint4*>(static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_st + h * p.q_sh + c * 8);
-        }
-        sts128(chunk_at(q_s + x * TILE_BYTES, r, c), v.x, v.y, v.z, v.w);
-      }
-    }
+    // rows of a tile that hold no query are zeros; TMA brings the others
+    for (int c = a.tile_rows * 8 + ptid; c < 128 * 8; c += 256)
+      for (int s = 0; s < 2 * QT; ++s) sts128(q_s + s * PANEL_BYTES + c * 16, 0, 0, 0, 0);
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&bar_q);
 
-    Unit ku[2], vu[2];
     // whether a key's mask lets it take part (its values are not looked at otherwise)
     const auto taken = [&](int key) {
       return !MASK || Elem<T>::to_f(static_cast<const T*>(p.mask)[b * p.mask_sb + mask_index(p, key)]) != -INFINITY;
     };
-    const auto request_k = [&](int j) {
+    Unit ku[2][2], vu[2][2];                  // requested: [tile of two][unit of the warp's two]
+    const auto request_k = [&](int j, Unit (&x)[2]) {
       const int tile = k.t0 + j;
       if (j < k.n && tile < k.nv) {
-        load_k_unit(p, bh, tile, pw, lane, ku[0]);
-        load_k_unit(p, bh, tile, pw + 8, lane, ku[1]);
+        load_k_unit(p, bh, tile, pw, lane, x[0]);
+        load_k_unit(p, bh, tile, pw + 8, lane, x[1]);
       }
     };
-    const auto request_v = [&](int j) {
+    const auto request_v = [&](int j, Unit (&x)[2]) {
       const int tile = k.t0 + j;
       if (j < k.n && tile < k.nv) {
+#pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int key = tile * 128 + (pw + 8 * u) * 8 + (lane >> 2);
-          load_v_unit(p, bh, tile, pw + 8 * u, lane, key < p.t_vis && taken(key), vu[u]);
+          load_v_unit(p, bh, tile, pw + 8 * u, lane, key < p.t_vis && taken(key), x[u]);
         }
       }
     };
-    Ring ring;
-    const auto wait_free = [&]() {
-      if (ok && ring.round > 0) ok = mbar_wait_bounded(&bar_free[ring.slot], (ring.round - 1) & 1, WAIT_TRIES);
+    const auto wait_free = [&](uint64_t* bar, int use) {      // the buffer's use-th use is about to start
+      if (ok && use > 0) ok = mbar_wait_bounded(bar, (use - 1) & 1, WAIT_TRIES);
       ok = __all_sync(0xffffffffu, ok);
     };
-    const auto publish = [&](uint32_t slot) {
-      if (lane == 0) mbar_arrive(&bar_full[slot]);
+    const auto publish = [&](uint64_t* bar) {
+      fence_proxy_async_smem();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(bar);
     };
-    const auto fp_tile = [&](const void* base, int tile, bool values) {      // into the ring's slot
+    const auto fp_tile = [&](const void* base, int tile, bool values, uint32_t dst) {
       const T* src = static_cast<const T*>(base) + b * p.fp_sb + hk * p.fp_sh;
       const int t_first = (tile - k.nv) * 128;
-      const uint32_t dst = ring_s + ring.slot * TILE_BYTES;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         uint4 v[4];
@@ -197,112 +184,101 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
           sts128(chunk_at(dst, (half * 4 + it) * 16 + (ptid >> 4), ptid & 15), v[it].x, v[it].y, v[it].z, v[it].w);
       }
     };
-    const auto produce_k = [&](int j) {
-      const int tile = k.t0 + j;
-      wait_free();
-      if (tile < k.nv) {
-        const uint32_t hi = ring.slot;
-        ring.next();
-        wait_free();
-        if (!ok) return;
-        const uint32_t lo = ring.slot;
-        store_k_unit<BF16>(ring_s + hi * TILE_BYTES, ring_s + lo * TILE_BYTES, ku[0], pw, lane);
-        store_k_unit<BF16>(ring_s + hi * TILE_BYTES, ring_s + lo * TILE_BYTES, ku[1], pw + 8, lane);
-        request_k(j + 1);
-        fence_proxy_async_smem();
-        __syncwarp();
-        publish(hi);
-        publish(lo);
-      } else {
-        if (!ok) return;
-        fp_tile(p.k_fp, tile, false);
-        fence_proxy_async_smem();
-        __syncwarp();
-        publish(ring.slot);
-      }
-      ring.next();
-    };
-    const auto produce_v = [&](int j) {
-      const int tile = k.t0 + j;
-      wait_free();
+    const auto produce_k = [&](int j, Unit (&x)[2]) {
+      if (j >= k.n || !ok) return;
+      const int tile = k.t0 + j, buf = j & 1;
+      const uint32_t hi = k_s + buf * 2 * TILE_BYTES, lo = hi + TILE_BYTES;
+      wait_free(&bar_kfree[buf], j >> 1);
       if (!ok) return;
       if (tile < k.nv) {
-        store_v_unit<BF16>(ring_s + ring.slot * TILE_BYTES, vu[0], pw, lane);
-        store_v_unit<BF16>(ring_s + ring.slot * TILE_BYTES, vu[1], pw + 8, lane);
-        request_v(j + 1);
+        store_k_unit<BF16>(hi, lo, x[0], pw, lane);
+        store_k_unit<BF16>(hi, lo, x[1], pw + 8, lane);
       } else {
-        fp_tile(p.v_fp, tile, true);
+        fp_tile(p.k_fp, tile, false, hi);
       }
-      fence_proxy_async_smem();
-      __syncwarp();
-      publish(ring.slot);
-      ring.next();
+      publish(&bar_k[buf]);
+      request_k(j + 2, x);                    // behind the fence, which would wait for what is under way
     };
-    request_k(0);
-    request_v(0);
-    // the order in which the issuer first touches them
-    if (!PAIR && k.n > 0) produce_k(0);
-    for (int j = 0; j < k.n && ok; ++j) {
-      if (PAIR) produce_k(j);
-      else if (j + 1 < k.n) produce_k(j + 1);
-      if (ok) produce_v(j);
+    const auto produce_v = [&](int j, Unit (&x)[2]) {
+      if (j >= k.n || !ok) return;
+      const int tile = k.t0 + j, buf = PAIR ? 0 : j & 1;
+      const uint32_t dst = v_s + buf * TILE_BYTES;
+      wait_free(&bar_vfree[buf], PAIR ? j : j >> 1);
+      if (!ok) return;
+      if (tile < k.nv) {
+        store_v_unit<BF16>(dst, x[0], pw, lane);
+        store_v_unit<BF16>(dst, x[1], pw + 8, lane);
+      } else {
+        fp_tile(p.v_fp, tile, true, dst);
+      }
+      publish(&bar_v[buf]);
+      request_v(j + 2, x);
+    };
+    request_k(0, ku[0]);
+    request_k(1, ku[1]);
+    request_v(0, vu[0]);
+    request_v(1, vu[1]);
+    // keys one tile ahead of values: scores come first
+    produce_k(0, ku[0]);
+    for (int j = 0; j < k.n && ok; j += 2) {
+      produce_k(j + 1, ku[1]);
+      produce_v(j, vu[0]);
+      produce_k(j + 2, ku[0]);
+      produce_v(j + 1, vu[1]);
     }
     if (!ok && lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
   } else if (warp >= MMA_WARP) {
     // ================= products =================
     setmaxnreg_dec<CONTROL_REGS>();
     if (warp == MMA_WARP) {
-    // the whole warp runs the loop and one elected lane issues: control flow and operands are uniform
+    // The whole warp runs the loop and one elected lane issues.  Loop bounds and tile numbers come out of a shuffle, so that the compiler
+    // knows them to be the warp's: operands that it holds per lane cost the issuing lane 104 cycles a product, of which the pipe takes 64.
+    const auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    const Range kr = k;
+    const Range k = {uniform(kr.nv), uniform(kr.t0), uniform(kr.n)};
     const uint32_t lead = elect_one();
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     constexpr uint64_t tile16 = TILE_BYTES >> 4;
-    const uint64_t qd = smem_desc(q_s, 16, 1024), kd = smem_desc(ring_s, 16, 1024), md = smem_desc(ring_s, PANEL_BYTES, 1024);
+    const uint64_t qd = smem_desc(q_s, 16, 1024), kd = smem_desc(k_s, 16, 1024), kmd = smem_desc(k_s, PANEL_BYTES, 1024), vd = smem_desc(v_s, PANEL_BYTES, 1024);
     bool ok = true;
     const auto all = [](bool r) { return __all_sync(0xffffffffu, r) != 0; };
-    Ring ring;
-    const auto acquire = [&]() {
-      ok = ok && all(mbar_wait_bounded(&bar_full[ring.slot], ring.round & 1, WAIT_TRIES));
-      const uint32_t s = ring.slot;
-      ring.next();
-      return s;
-    };
+    if (lead) {
+      mbar_expect_tx(&bar_q, 256 * a.tile_rows * QT);
+      for (int s = 0; s < 2 * QT; ++s)      // both halves of the channels; queries past the end are zeros
+        tma_load_4d(q_s + s * PANEL_BYTES, &tm_q, (s & 1) * 64, hk * p.n_rep, i0 + (s >> 1) * a.tile_queries, b, &bar_q);
+    }
     const auto commit = [&](uint64_t* bar) { if (lead) umma_commit(bar); };
-    uint32_t hi = 0, lo = 0;                  // slots of the key tile at hand; hi == lo: full precision
-    const auto take_k = [&](int j) {
-      hi = lo = acquire();
-      if (k.t0 + j < k.nv) lo = acquire();
+    using C0 = std::integral_constant<int, 0>;
+    using C1 = std::integral_constant<int, 1>;
+    // tile and buffer are constants of the code
+    const auto take_k = [&](auto bc, int j) {
+      constexpr int buf = decltype(bc)::value;
+      ok = ok && all(mbar_wait_bounded(&bar_k[buf], (j >> 1) & 1, WAIT_TRIES));
       tc_fence_after();
     };
-    const auto issue_s = [&](int x) {         // S_x = Q_x K^T
+    const auto issue_s = [&](auto xc, auto bc, int j) {      // S_x = Q_x K^T of key tile j
+      constexpr int x = decltype(xc)::value, buf = decltype(bc)::value;
+      constexpr uint64_t q0 = PAIR && x ? tile16 : 0, hi = 2 * buf * tile16, lo = hi + tile16;
       if (!lead) return;
       const uint32_t d = tm + (uint32_t)x * 128u;
-      const uint64_t q = qd + (PAIR && x ? tile16 : 0);
-      if (hi != lo) {
+      if (k.t0 + j < k.nv) {                                 // the small terms first: sums are cut off, not rounded
 #pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          const uint64_t qo = (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
-          umma(d, q + qo, md + lo * tile16 + (uint64_t)(ks * 128), a.idesc_mn, ks > 0);      // the small terms first: sums are cut off, not rounded
-        }
-#pragma unroll
-        for (int ks = 0; ks < 8; ++ks) {
-          const uint64_t qo = (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
-          umma(d, q + qo, md + hi * tile16 + (uint64_t)(ks * 128), a.idesc_mn, 1);
+        for (int ks = 0; ks < 16; ++ks) {
+          const uint64_t qo = (uint64_t)((((ks & 7) >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
+          umma(d, qd + (q0 + qo), kmd + ((ks < 8 ? lo : hi) + (uint64_t)((ks & 7) * 128)), a.idesc_mn, ks > 0);
         }
       } else {
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
           const uint64_t qo = (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
-          umma(d, q + qo, kd + hi * tile16 + qo, a.idesc_kmajor, ks > 0);
+          umma(d, qd + (q0 + qo), kd + (hi + qo), a.idesc_kmajor, ks > 0);
         }
       }
       umma_commit(&bar_s[x]);
     };
-    const auto free_k = [&]() {
-      commit(&bar_free[hi]);
-      if (lo != hi) commit(&bar_free[lo]);
-    };
-    // O_x += P_x V, the probabilities of keys 0-63 first
-    const auto pv = [&](int x, uint32_t v, int count) {
+    // O_x += P_x V, the probabilities of keys 0-63 first; `count` key tiles of x before
+    const auto pv = [&](auto xc, auto vc, int count) {
+      constexpr int x = decltype(xc)::value, buf = decltype(vc)::value;
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         ok = ok && all(mbar_wait_cycles(&bar_p[x][half], count & 1, WAIT_CYCLES));
@@ -311,7 +287,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
         if (lead) {
 #pragma unroll
           for (int ks = 4 * half; ks < 4 * half + 4; ++ks)
-            umma_ts(tm + 256u + (uint32_t)x * 128u, tm + (uint32_t)x * 128u + (uint32_t)ks * 8u, md + v * tile16 + (uint64_t)(ks * 128), a.idesc_mn,
+            umma_ts(tm + 256u + (uint32_t)x * 128u, tm + (uint32_t)x * 128u + (uint32_t)ks * 8u, vd + (buf * tile16 + (uint64_t)(ks * 128)), a.idesc_mn,
                     (ks > 0 || count > 0) ? 1u : 0u);
         }
       }
@@ -320,30 +296,52 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
     ok = all(mbar_wait_bounded(&bar_q, 0, WAIT_TRIES));
     if (PAIR) {
       if (k.n > 0) {
-        take_k(0);
-        if (ok) { issue_s(0); issue_s(1); free_k(); }
+        take_k(C0{}, 0);
+        if (ok) { issue_s(C0{}, C0{}, 0); issue_s(C1{}, C0{}, 0); commit(&bar_kfree[0]); }
       }
-      for (int j = 0; j < k.n && ok; ++j) {
-        const uint32_t v = acquire();
+      const auto step = [&](auto next, int j) {              // next: the buffer of key tile j + 1
+        constexpr int nb = decltype(next)::value;
+        if (j >= k.n || !ok) return;
         const bool more = j + 1 < k.n;
-        if (ok) pv(0, v, j);
-        if (more && ok) take_k(j + 1);
-        if (more && ok) issue_s(0);
-        if (ok) pv(1, v, j);
-        if (ok) commit(&bar_free[v]);
-        if (more && ok) { issue_s(1); free_k(); }
+        ok = all(mbar_wait_bounded(&bar_v[0], j & 1, WAIT_TRIES));
+        if (ok) pv(C0{}, C0{}, j);
+        if (more && ok) take_k(next, j + 1);
+        if (more && ok) issue_s(C0{}, next, j + 1);
+        if (ok) pv(C1{}, C0{}, j);
+        if (!ok) return;
+        commit(&bar_vfree[0]);
+        if (more) {
+          issue_s(C1{}, next, j + 1);
+          commit(&bar_kfree[nb]);
+        }
+      };
+      for (int j = 0; j < k.n && ok; j += 2) {
+        step(C1{}, j);
+        step(C0{}, j + 1);
       }
     } else {
-      for (int j = 0; j < min(2, k.n) && ok; ++j) {
-        take_k(j);
-        if (ok) { issue_s(j); free_k(); }
-      }
-      for (int j = 0; j < k.n && ok; ++j) {
-        const uint32_t v = acquire();
-        if (ok) pv(j & 1, v, j >> 1);
-        if (ok) commit(&bar_free[v]);
-        if (j + 2 < k.n && ok) take_k(j + 2);
-        if (j + 2 < k.n && ok) { issue_s(j & 1); free_k(); }
+      const auto first = [&](auto xc) {                      // x, its buffers and key tile are one number here
+        constexpr int x = decltype(xc)::value;
+        if (x >= k.n || !ok) return;
+        take_k(xc, x);
+        if (ok) { issue_s(xc, xc, x); commit(&bar_kfree[x]); }
+      };
+      const auto step = [&](auto xc, int j) {
+        constexpr int x = decltype(xc)::value;
+        if (j >= k.n || !ok) return;
+        ok = all(mbar_wait_bounded(&bar_v[x], (j >> 1) & 1, WAIT_TRIES));
+        if (ok) pv(xc, xc, j >> 1);
+        if (!ok) return;
+        commit(&bar_vfree[x]);
+        if (j + 2 >= k.n) return;
+        take_k(xc, j + 2);
+        if (ok) { issue_s(xc, xc, j + 2); commit(&bar_kfree[x]); }
+      };
+      first(C0{});
+      first(C1{});
+      for (int j = 0; j < k.n && ok; j += 2) {
+        step(C0{}, j);
+        step(C1{}, j + 1);
       }
     }
     if (!ok && lead) atomicExch(a.status, CQ_ERR_TIMEOUT);
@@ -355,7 +353,8 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
     const int x = warp >> 2, quarter = warp & 3, r_in = quarter * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t tS = tmem + (uint32_t)x * 128u + lane_off, tO = tmem + 256u + (uint32_t)x * 128u + lane_off;
-    const int row = row0 + (PAIR ? x * 128 : 0) + r_in, i = row / p.n_rep;
+    const int q_first = i0 + (PAIR ? x * a.tile_queries : 0), i_in = r_in / p.n_rep, i = q_first + i_in;
+    const bool valid_row = r_in < a.tile_rows && i < p.q_len;
     const int limit = live - p.q_len + i + 1;                     // full-precision tokens that the row sees
     const int n_x = PAIR ? k.n : (k.n + 1 - x) >> 1;
     // Units: without a mask, scores as the tensor core gives them times `factor` are powers of two; with one they are scaled and
@@ -469,12 +468,12 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
     ok = __all_sync(0xffffffffu, ok);
     if (!ok && lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
     tc_fence_after();
-    const int h = hk * p.n_rep + row % p.n_rep;
+    const int h = hk * p.n_rep + r_in - i_in * p.n_rep;
     const float nat = MASK ? 1.f : a.scale;         // reference maximum in natural units
     if (a.parts == 1) {
       // the tile's rows through its query tile in shared memory (no product reads that any more), then 16 lanes a row
       const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
-      if (ok && row < p.rows && p.lse)
+      if (ok && valid_row && p.lse)
         p.lse[((int64_t)b * p.hq + h) * p.q_len + i] = l_run > 0.f ? m_ref * nat + logf(l_run) : -INFINITY;
       const uint32_t stage = q_s + (uint32_t)x * TILE_BYTES;
       if (ok) {
@@ -493,24 +492,24 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
         }
         __syncwarp();
         for (int it = 0; it < 16; ++it) {
-          const int rr = quarter * 32 + it * 2 + (lane >> 4), rw = row0 + x * 128 + rr;
-          if (rw < p.rows) {
+          const int rr = quarter * 32 + it * 2 + (lane >> 4), ii = rr / p.n_rep;
+          if (rr < a.tile_rows && q_first + ii < p.q_len) {
             const uint4 v = lds128(chunk_at(stage, rr, lane & 15));
-            T* dst = static_cast<T*>(p.out) + b * p.o_sb + (int64_t)(rw / p.n_rep) * p.o_st + (int64_t)(hk * p.n_rep + rw % p.n_rep) * p.o_sh;
+            T* dst = static_cast<T*>(p.out) + b * p.o_sb + (int64_t)(q_first + ii) * p.o_st + (int64_t)(hk * p.n_rep + rr - ii * p.n_rep) * p.o_sh;
             *reinterpret_cast<uint4*>(dst + (lane & 15) * 8) = v;
           }
         }
       }
-    } else if (row0 + (PAIR ? x * 128 : 0) + quarter * 32 < p.rows) {
+    } else if (__any_sync(0xffffffffu, valid_row)) {
       // a partial result, the channels in their order
-      const int64_t at = (bh * p.rows + row) * a.parts + (PAIR ? part : 2 * part + x);
-      if (row < p.rows) a.part_ml[at] = make_float2(ok ? (n_x > 0 ? m_ref * nat : -INFINITY) : 0.f, ok ? l_run : NAN);
+      const int64_t at = (bh * p.rows + (int64_t)i * p.n_rep + (h - hk * p.n_rep)) * a.parts + (PAIR ? part : 2 * part + x);
+      if (valid_row) a.part_ml[at] = make_float2(ok ? (n_x > 0 ? m_ref * nat : -INFINITY) : 0.f, ok ? l_run : NAN);
       if (n_x > 0 && ok) {
 #pragma unroll 1
         for (int cc = 0; cc < 4; ++cc) {
           uint32_t r[32];
           tmem_ld32(tO + cc * 32, r);
-          if (row < p.rows) {
+          if (valid_row) {
             float4* dst = reinterpret_cast<float4*>(a.part_o + at * 128 + cc * 32);
 #pragma unroll
             for (int c = 0; c < 32; c += 8) {
@@ -565,15 +564,16 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(AttnParams a, int64_
 // ---- host ---------------------------------------------------------------------------------------------------------
 struct Plan {
   bool pair;
-  int row_blocks, grid_parts, parts;
+  int queries, row_blocks, grid_parts, parts;      // queries of a tile
 };
 // Split of the key tiles: as many CTAs as fill the SMs, in whole rounds where there are several; a CTA costs about three key tiles beside
 // its own (its start, and its partial result).
 static Plan make_plan(const cq_chunk_args* a) {
-  const int64_t rows = (int64_t)a->q_len * (a->n_q_heads / a->n_kv_heads);
   Plan pl;
-  pl.pair = rows > 128;
-  pl.row_blocks = (int)((rows + (pl.pair ? 255 : 127)) / (pl.pair ? 256 : 128));
+  pl.queries = 128 / (a->n_q_heads / a->n_kv_heads);
+  pl.pair = a->q_len > pl.queries;
+  const int block = pl.queries * (pl.pair ? 2 : 1);
+  pl.row_blocks = (a->q_len + block - 1) / block;
   const int64_t items = (int64_t)a->batch * a->n_kv_heads * pl.row_blocks;
   const int tiles = (a->t_vis + 127) / 128 + (a->t_fp + 127) / 128, sms = sm_count();
   int best = 1;
@@ -595,7 +595,7 @@ static size_t workspace_bytes(const cq_chunk_args* a, const Plan& pl) {
 }
 
 template <bool BF16, bool MASK, bool PAIR>
-static int launch_attn(const AttnParams& p, const Plan& pl, int batch, cudaStream_t st) {
+static int launch_attn(const CUtensorMap& tm, const AttnParams& p, const Plan& pl, int batch, cudaStream_t st) {
   static bool configured[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CQ_ERR_LAUNCH;
@@ -604,7 +604,7 @@ static int launch_attn(const AttnParams& p, const Plan& pl, int batch, cudaStrea
     configured[dev] = true;
   }
   const dim3 grid(pl.row_blocks, batch * p.p.hkv, pl.grid_parts);
-  chunk_attn_kernel<BF16, MASK, PAIR><<<grid, THREADS, SMEM_BYTES, st>>>(p);
+  chunk_attn_kernel<BF16, MASK, PAIR><<<grid, THREADS, SMEM_BYTES, st>>>(tm, p);
   if (const int rc = check_launch()) return rc;
   if (pl.parts == 1) return CQ_OK;
   const int64_t rows = (int64_t)batch * p.p.hkv * p.p.rows;
@@ -641,6 +641,9 @@ extern "C" int cq_chunk_attn(const cq_chunk_args* a, void* workspace, size_t wor
   p.p = chunk::make_params(a);
   p.parts = pl.parts;
   p.scale = 0.08838834764831845f;
+  p.tile_queries = pl.queries; p.tile_rows = pl.queries * p.p.n_rep;
+  CUtensorMap tm;
+  if (!chunk::query_map(&tm, a, pl.queries)) return CQ_ERR_LAUNCH;
   const int bf16 = a->dtype == CQ_DTYPE_BF16;
   p.idesc_kmajor = chunk::idesc_of(bf16, 0, 0, 128, 128);
   p.idesc_mn = chunk::idesc_of(bf16, 0, 1, 128, 128);
@@ -649,7 +652,7 @@ extern "C" int cq_chunk_attn(const cq_chunk_args* a, void* workspace, size_t wor
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
   p.part_ml = reinterpret_cast<float2*>(p.part_o + rows * pl.parts * 128);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define CQ_RUN(B, M) (pl.pair ? chunk::launch_attn<B, M, true>(p, pl, a->batch, st) : chunk::launch_attn<B, M, false>(p, pl, a->batch, st))
+#define CQ_RUN(B, M) (pl.pair ? chunk::launch_attn<B, M, true>(tm, p, pl, a->batch, st) : chunk::launch_attn<B, M, false>(tm, p, pl, a->batch, st))
   if (bf16) return a->mask ? CQ_RUN(true, true) : CQ_RUN(true, false);
   return a->mask ? CQ_RUN(false, true) : CQ_RUN(false, false);
 #undef CQ_RUN

@@ -124,6 +124,10 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
     __syncwarp();
   } else if (warp == MMA_WARP) {
     // ================= products =================
+    // loop bounds come out of a shuffle, so that the compiler knows them to be the warp's and keeps the operands in uniform registers
+    const auto uniform = [](int v) { return __shfl_sync(0xffffffffu, v, 0); };
+    const int nb_lane = nb, n_x_lane = n_x;
+    const int nb = uniform(nb_lane), n_x = uniform(n_x_lane);
     const uint32_t lead = elect_one();
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
     constexpr uint64_t tile16 = TILE_BYTES >> 4;
@@ -151,7 +155,7 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
         umma_commit(&bar_d[x][s]);
       }
     };
-    const bool packed0 = tile0 < nv, packed1 = tile0 + 1 < nv;
+    const bool packed0 = uniform(tile0 < nv), packed1 = uniform(tile0 + 1 < nv);
     bool ok = nb == 0 || all(mbar_wait_bounded(&bar_k, 0, WAIT_TRIES));
     const auto block = [&](auto sc, int n) {
       constexpr int s = decltype(sc)::value;
