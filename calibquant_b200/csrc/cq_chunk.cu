@@ -26,9 +26,14 @@ namespace chunk {
 using namespace ptx;
 using namespace tc;
 
-constexpr int PRODUCERS = 8, MMA_WARP = 16, THREADS = 20 * 32;
-// registers: 256 x 120 + 256 x 88 + 128 x 64 = the launch's 640 x 96
-constexpr int SOFTMAX_REGS = 120, PRODUCER_REGS = 88, CONTROL_REGS = 64;
+constexpr int PRODUCERS = 8;
+// Threads and registers.  Without images: 8 softmax warps, 8 producers, the issuer's warpgroup; 256 x 120 + 256 x 88 + 128 x 64 = the launch's
+// 640 x 96.  With images: 8 softmax warps, which hold a row's 128 scores at once, and the issuer's warpgroup; 256 x 200 + 128 x 96
+// = 63 488 of the launch's 384 x 168.
+template <bool IMAGE> struct Roles {
+  static constexpr int MMA_WARP = IMAGE ? 8 : 16, THREADS = IMAGE ? 384 : 640;
+  static constexpr int SOFTMAX_REGS = IMAGE ? 200 : 120, CONTROL_REGS = IMAGE ? 96 : 64, PRODUCER_REGS = 88;
+};
 constexpr int SMEM_BYTES = 7 * TILE_BYTES + 1024;
 constexpr uint32_t WAIT_TRIES = 1u << 22;
 constexpr long long WAIT_CYCLES = 1ll << 30;
@@ -40,6 +45,8 @@ struct AttnParams {
   int parts;                 // partial results per row (1: the kernel writes the output itself)
   float scale;               // 1 / sqrt(128)
   uint32_t idesc_kmajor, idesc_mn;
+  unsigned char* image;      // unpacked tiles, see unpack_kernel
+  int image_fp_tiles;
   float* part_o;             // [batch][KV head][row][part][128]
   float2* part_ml;           // [batch][KV head][row][part]: maximum and sum
   int* status;
@@ -72,13 +79,96 @@ struct Range {
   int nv, t0, n;
 };
 
-template <bool BF16, bool MASK, bool PAIR>
-__global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ AttnParams a) {
+// Unpacked tiles of a KV head as they lie in shared memory, one after the other: per visual tile both terms of the keys and the values, per
+// full-precision tile keys and values.
+__host__ __device__ __forceinline__ size_t image_bytes(int nv, int nf) { return (size_t)(3 * nv + 2 * nf) * TILE_BYTES; }
+
+// whether a key's mask lets it take part (its values are not looked at otherwise)
+template <bool BF16, bool MASK>
+__device__ __forceinline__ bool takes_part(const Params& p, int b, int key) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  return !MASK || Elem<T>::to_f(static_cast<const T*>(p.mask)[b * p.mask_sb + mask_index(p, key)]) != -INFINITY;
+}
+
+// A full-precision tile, rows that are not live (values: or that the mask takes out) as zeros; 256 threads.
+template <bool BF16, bool MASK>
+__device__ __forceinline__ void fill_fp_tile(const Params& p, const void* base, int b, int hk, int t_first, int live, bool values, uint32_t dst, int ptid) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  const T* src = static_cast<const T*>(base) + b * p.fp_sb + hk * p.fp_sh;
+#pragma unroll
+  for (int half = 0; half < 2; ++half) {
+    uint4 v[4];
+#pragma unroll
+    for (int it = 0; it < 4; ++it) {
+      const int t = t_first + (half * 4 + it) * 16 + (ptid >> 4);
+      v[it] = make_uint4(0, 0, 0, 0);
+      if (t < live && (!values || takes_part<BF16, MASK>(p, b, p.t_vis + t))) v[it] = *reinterpret_cast<const uint4*>(src + (int64_t)t * 128 + (ptid & 15) * 8);
+      if (values) order_values(v[it]);
+    }
+#pragma unroll
+    for (int it = 0; it < 4; ++it)
+      sts128(chunk_at(dst, (half * 4 + it) * 16 + (ptid >> 4), ptid & 15), v[it].x, v[it].y, v[it].z, v[it].w);
+  }
+}
+
+__device__ __forceinline__ void bulk_store_1d(void* dst, uint32_t src, uint32_t bytes) {
+  asm volatile("cp.async.bulk.global.shared::cta.bulk_group [%0], [%1], %2;" ::"l"(dst), "r"(src), "r"(bytes) : "memory");
+}
+
+// Unpacks every key tile once, for calls whose rows would have the attention unpack it many times: a CTA per tile.
+template <bool BF16, bool MASK>
+__global__ void __launch_bounds__(256) chunk_unpack_kernel(const __grid_constant__ AttnParams a) {
+  const Params& p = a.p;
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
+  const uint32_t s0 = smem_u32(smem);
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nv = (p.t_vis + 127) >> 7, tile = blockIdx.x;
+  const int hk = blockIdx.y % p.hkv, b = blockIdx.y / p.hkv;
+  const int64_t bh = (int64_t)b * p.hkv + hk;
+  const int live = live_tokens(p);
+  pdl_launch_dependents();
+  unsigned char* dst = a.image + bh * image_bytes(nv, a.image_fp_tiles);
+  int n;
+  if (tile < nv) {
+    Unit k[2], v[2];
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      const int key = tile * 128 + (warp + 8 * u) * 8 + (lane >> 2);
+      load_k_unit(p, bh, tile, warp + 8 * u, lane, k[u]);
+      load_v_unit(p, bh, tile, warp + 8 * u, lane, key < p.t_vis && takes_part<BF16, MASK>(p, b, key), v[u]);
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      store_k_unit<BF16>(s0, s0 + TILE_BYTES, k[u], warp + 8 * u, lane);
+      store_v_unit<BF16>(s0 + 2 * TILE_BYTES, v[u], warp + 8 * u, lane);
+    }
+    dst += (size_t)tile * 3 * TILE_BYTES;
+    n = 3;
+  } else {
+    const int t_first = (tile - nv) * 128;
+    if (t_first >= live) return;
+    fill_fp_tile<BF16, MASK>(p, p.k_fp, b, hk, t_first, live, false, s0, tid);
+    fill_fp_tile<BF16, MASK>(p, p.v_fp, b, hk, t_first, live, true, s0 + TILE_BYTES, tid);
+    dst += image_bytes(nv, tile - nv);
+    n = 2;
+  }
+  fence_proxy_async_smem();
+  __syncthreads();
+  if (tid == 0) {
+    bulk_store_1d(dst, s0, n * TILE_BYTES);
+    asm volatile("cp.async.bulk.commit_group;" ::: "memory");
+    asm volatile("cp.async.bulk.wait_group 0;" ::: "memory");
+  }
+}
+
+template <bool BF16, bool MASK, bool PAIR, bool IMAGE>
+__global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(const __grid_constant__ CUtensorMap tm_q, const __grid_constant__ AttnParams a) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   const Params& p = a.p;
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
-  constexpr int QT = PAIR ? 2 : 1;      // query tiles
+  static_assert(PAIR || !IMAGE, "images are for many rows");
+  constexpr int QT = PAIR ? 2 : 1, MMA_WARP = Roles<IMAGE>::MMA_WARP;      // query tiles
   const uint32_t q_s = smem_u32(smem), k_s = q_s + QT * TILE_BYTES, v_s = k_s + 4 * TILE_BYTES;      // keys: [buffer][large terms, small ones]
   // bar_q (once); bar_k / bar_v[buffer] full, bar_kfree / bar_vfree read; bar_s[X] scores of X ready; bar_p[X][half] probabilities of keys 0-63 / 64-127 stored;
   // bar_pv[X] the tile's P V done
@@ -92,11 +182,11 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
   const int i0 = ((int)gridDim.x - 1 - (int)blockIdx.x) * (PAIR ? 2 : 1) * a.tile_queries;      // first query; those that see most keys first
 
   if (tid == 0) {
-    mbar_init(&bar_q, PRODUCERS + 1);
+    mbar_init(&bar_q, 1 + (IMAGE ? 1 : PRODUCERS));
     for (int x = 0; x < 2; ++x) {
-      mbar_init(&bar_k[x], PRODUCERS);
+      mbar_init(&bar_k[x], IMAGE ? 1 : PRODUCERS);
       mbar_init(&bar_kfree[x], 1);
-      mbar_init(&bar_v[x], PRODUCERS);
+      mbar_init(&bar_v[x], IMAGE ? 1 : PRODUCERS);
       mbar_init(&bar_vfree[x], 1);
       mbar_init(&bar_s[x], 1);
       mbar_init(&bar_p[x][0], 128);
@@ -105,6 +195,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
     }
     mbar_fence_init();
   }
+  if (IMAGE) pdl_wait();                      // the images are the launch's before this one
   pdl_launch_dependents();
   const int live = live_tokens(p);
   if (warp == MMA_WARP) tmem_alloc(&tmem_base_s, 512);
@@ -123,22 +214,22 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
     k.n = min(n_all, k.t0 + per) - k.t0;
   }
 
-  if (warp >= 8 && warp < MMA_WARP) {
-    // ================= operands =================
-    setmaxnreg_dec<PRODUCER_REGS>();
-    const int pw = warp - 8, ptid = tid - 256;
-    bool ok = true;
-    // rows of a tile that hold no query are zeros; TMA brings the others
-    for (int c = a.tile_rows * 8 + ptid; c < 128 * 8; c += 256)
+  // rows of a query tile that hold no query are zeros; TMA brings the others
+  const auto clear_q = [&](int thread, int threads) {
+    for (int c = a.tile_rows * 8 + thread; c < 128 * 8; c += threads)
       for (int s = 0; s < 2 * QT; ++s) sts128(q_s + s * PANEL_BYTES + c * 16, 0, 0, 0, 0);
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) mbar_arrive(&bar_q);
+  };
 
-    // whether a key's mask lets it take part (its values are not looked at otherwise)
-    const auto taken = [&](int key) {
-      return !MASK || Elem<T>::to_f(static_cast<const T*>(p.mask)[b * p.mask_sb + mask_index(p, key)]) != -INFINITY;
-    };
+  if (!IMAGE && warp >= 8 && warp < MMA_WARP) {
+    // ================= operands =================
+    setmaxnreg_dec<Roles<IMAGE>::PRODUCER_REGS>();
+    const int pw = warp - 8, ptid = tid - 256;
+    bool ok = true;
+    clear_q(ptid, 256);
+
     Unit ku[2][2], vu[2][2];                  // requested: [tile of two][unit of the warp's two]
     const auto request_k = [&](int j, Unit (&x)[2]) {
       const int tile = k.t0 + j;
@@ -153,7 +244,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int key = tile * 128 + (pw + 8 * u) * 8 + (lane >> 2);
-          load_v_unit(p, bh, tile, pw + 8 * u, lane, key < p.t_vis && taken(key), x[u]);
+          load_v_unit(p, bh, tile, pw + 8 * u, lane, key < p.t_vis && takes_part<BF16, MASK>(p, b, key), x[u]);
         }
       }
     };
@@ -166,24 +257,6 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    const auto fp_tile = [&](const void* base, int tile, bool values, uint32_t dst) {
-      const T* src = static_cast<const T*>(base) + b * p.fp_sb + hk * p.fp_sh;
-      const int t_first = (tile - k.nv) * 128;
-#pragma unroll
-      for (int half = 0; half < 2; ++half) {
-        uint4 v[4];
-#pragma unroll
-        for (int it = 0; it < 4; ++it) {
-          const int t = t_first + (half * 4 + it) * 16 + (ptid >> 4);
-          v[it] = make_uint4(0, 0, 0, 0);
-          if (t < live && (!values || taken(p.t_vis + t))) v[it] = *reinterpret_cast<const uint4*>(src + (int64_t)t * 128 + (ptid & 15) * 8);
-          if (values) order_values(v[it]);
-        }
-#pragma unroll
-        for (int it = 0; it < 4; ++it)
-          sts128(chunk_at(dst, (half * 4 + it) * 16 + (ptid >> 4), ptid & 15), v[it].x, v[it].y, v[it].z, v[it].w);
-      }
-    };
     const auto produce_k = [&](int j, Unit (&x)[2]) {
       if (j >= k.n || !ok) return;
       const int tile = k.t0 + j, buf = j & 1;
@@ -194,7 +267,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
         store_k_unit<BF16>(hi, lo, x[0], pw, lane);
         store_k_unit<BF16>(hi, lo, x[1], pw + 8, lane);
       } else {
-        fp_tile(p.k_fp, tile, false, hi);
+        fill_fp_tile<BF16, MASK>(p, p.k_fp, b, hk, (tile - k.nv) * 128, live, false, hi, ptid);
       }
       publish(&bar_k[buf]);
       request_k(j + 2, x);                    // behind the fence, which would wait for what is under way
@@ -209,7 +282,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
         store_v_unit<BF16>(dst, x[0], pw, lane);
         store_v_unit<BF16>(dst, x[1], pw + 8, lane);
       } else {
-        fp_tile(p.v_fp, tile, true, dst);
+        fill_fp_tile<BF16, MASK>(p, p.v_fp, b, hk, (tile - k.nv) * 128, live, true, dst, ptid);
       }
       publish(&bar_v[buf]);
       request_v(j + 2, x);
@@ -229,7 +302,7 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
     if (!ok && lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
   } else if (warp >= MMA_WARP) {
     // ================= products =================
-    setmaxnreg_dec<CONTROL_REGS>();
+    setmaxnreg_dec<Roles<IMAGE>::CONTROL_REGS>();
     if (warp == MMA_WARP) {
     // The whole warp runs the loop and one elected lane issues.  Loop bounds and tile numbers come out of a shuffle, so that the compiler
     // knows them to be the warp's: operands that it holds per lane cost the issuing lane 104 cycles a product, of which the pipe takes 64.
@@ -346,10 +419,38 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
     }
     if (!ok && lead) atomicExch(a.status, CQ_ERR_TIMEOUT);
     __syncwarp();
+    } else if (IMAGE && warp == MMA_WARP + 1) {
+      // ================= operands from the images =================
+      clear_q(lane, 32);
+      if (lane == 0) {
+        const unsigned char* src = a.image + bh * image_bytes(k.nv, a.image_fp_tiles);
+        bool ok = true;
+        const auto load_k = [&](int j) {
+          if (j >= k.n || !ok) return;
+          const int tile = k.t0 + j, buf = j & 1;
+          if (j >= 2) ok = mbar_wait_bounded(&bar_kfree[buf], ((j >> 1) - 1) & 1, WAIT_TRIES);
+          if (!ok) return;
+          const uint32_t bytes = (tile < k.nv ? 2 : 1) * TILE_BYTES;
+          mbar_expect_tx(&bar_k[buf], bytes);
+          bulk_load_1d(smem + (QT + 2 * buf) * TILE_BYTES, src + (tile < k.nv ? (size_t)tile * 3 * TILE_BYTES : image_bytes(k.nv, tile - k.nv)), bytes, &bar_k[buf]);
+        };
+        load_k(0);
+        for (int j = 0; j < k.n && ok; ++j) {
+          load_k(j + 1);
+          if (ok && j > 0) ok = mbar_wait_bounded(&bar_vfree[0], (j - 1) & 1, WAIT_TRIES);
+          if (!ok) break;
+          const int tile = k.t0 + j;
+          mbar_expect_tx(&bar_v[0], TILE_BYTES);
+          bulk_load_1d(smem + (QT + 4) * TILE_BYTES, src + (tile < k.nv ? (size_t)(3 * tile + 2) * TILE_BYTES : image_bytes(k.nv, tile - k.nv) + TILE_BYTES),
+                       TILE_BYTES, &bar_v[0]);
+        }
+        if (!ok) atomicExch(a.status, CQ_ERR_TIMEOUT);
+      }
+      __syncwarp();
     }
   } else {
     // ================= softmax: thread = row =================
-    setmaxnreg_inc<SOFTMAX_REGS>();
+    setmaxnreg_inc<Roles<IMAGE>::SOFTMAX_REGS>();
     const int x = warp >> 2, quarter = warp & 3, r_in = quarter * 32 + lane;
     const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
     const uint32_t tS = tmem + (uint32_t)x * 128u + lane_off, tO = tmem + 256u + (uint32_t)x * 128u + lane_off;
@@ -400,17 +501,23 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
         }
       };
       float mx4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+      uint32_t s[IMAGE ? 4 : 2][32];          // with images the row's 128 scores, read once
+      const auto read = [&](int half) {
+        tmem_ld32_nowait(tS + half * 64, s[IMAGE ? half * 2 : 0]);
+        tmem_ld32_nowait(tS + half * 64 + 32, s[IMAGE ? half * 2 + 1 : 1]);
+      };
+      if (IMAGE) read(0);
+      if (IMAGE) read(1);
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        uint32_t s[2][32];
-        tmem_ld32_nowait(tS + half * 64, s[0]);
-        tmem_ld32_nowait(tS + half * 64 + 32, s[1]);
-        tmem_ld_wait();
+        if (!IMAGE) read(half);
+        if (!IMAGE || half == 0) tmem_ld_wait();
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
-          shown(half * 2 + cc, s[cc]);
+          uint32_t (&v)[32] = s[IMAGE ? half * 2 + cc : cc];
+          shown(half * 2 + cc, v);
 #pragma unroll
-          for (int c = 0; c < 32; c += 2) mx4[(c >> 1) & 3] = max3(mx4[(c >> 1) & 3], __uint_as_float(s[cc][c]), __uint_as_float(s[cc][c + 1]));
+          for (int c = 0; c < 32; c += 2) mx4[(c >> 1) & 3] = max3(mx4[(c >> 1) & 3], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
         }
       }
       const float m_true = fmaxf(m_ref, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
@@ -435,16 +542,18 @@ __global__ void __launch_bounds__(THREADS, 1) chunk_attn_kernel(const __grid_con
       float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
-        uint32_t w[32], s[2][32];
-        tmem_ld32_nowait(tS + half * 64, s[0]);
-        tmem_ld32_nowait(tS + half * 64 + 32, s[1]);
-        tmem_ld_wait();
+        uint32_t w[32];
+        if (!IMAGE) {
+          read(half);
+          tmem_ld_wait();
+        }
 #pragma unroll
         for (int cc = 0; cc < 2; ++cc) {
-          shown(half * 2 + cc, s[cc]);
+          uint32_t (&v)[32] = s[IMAGE ? half * 2 + cc : cc];
+          if (!IMAGE) shown(half * 2 + cc, v);
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
-            float e0 = __uint_as_float(s[cc][c]), e1 = __uint_as_float(s[cc][c + 1]);
+            float e0 = __uint_as_float(v[c]), e1 = __uint_as_float(v[c + 1]);
             if (MASK) {
               e0 = (e0 - m_use) * factor;
               e1 = (e1 - m_use) * factor;
@@ -561,9 +670,11 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(AttnParams a, int64_
   if (p.lse && lane == 0) p.lse[(b * p.hq + h) * p.q_len + i] = bad ? NAN : l > 0.f ? m + logf(l) : -INFINITY;
 }
 
+constexpr int IMAGE_BLOCKS = 3;
+
 // ---- host ---------------------------------------------------------------------------------------------------------
 struct Plan {
-  bool pair;
+  bool pair, image;
   int queries, row_blocks, grid_parts, parts;      // queries of a tile
 };
 // Split of the key tiles: as many CTAs as fill the SMs, in whole rounds where there are several; a CTA costs about three key tiles beside
@@ -584,28 +695,42 @@ static Plan make_plan(const cq_chunk_args* a) {
     const double c = (double)((items * s + sms - 1) / sms) * (per * (pl.pair ? 2 : 1) + 3 + (s > 1 && pl.pair ? 2 : 0));
     if (c < cost) { cost = c; best = s; }
   }
+  // Key tiles that several row blocks would unpack are unpacked once, if their images take a gigabyte at most
+  pl.image = pl.row_blocks >= IMAGE_BLOCKS && (size_t)a->batch * a->n_kv_heads * image_bytes((a->t_vis + 127) / 128, (a->t_fp + 127) / 128) <= (size_t)1 << 30;
   pl.grid_parts = best;
   pl.parts = pl.pair ? best : 2 * best;
   return pl;
 }
+// The status word's 256 bytes, the images, the partial results.
+static size_t images_of(const cq_chunk_args* a, const Plan& pl) {
+  return pl.image ? (size_t)a->batch * a->n_kv_heads * image_bytes((a->t_vis + 127) / 128, (a->t_fp + 127) / 128) : 0;
+}
 static size_t workspace_bytes(const cq_chunk_args* a, const Plan& pl) {
-  if (pl.parts == 1) return 256;
   const size_t rows = (size_t)a->batch * a->n_q_heads * a->q_len;
-  return 256 + rows * pl.parts * (128 * sizeof(float) + sizeof(float2));
+  return 256 + images_of(a, pl) + (pl.parts == 1 ? 0 : rows * pl.parts * (128 * sizeof(float) + sizeof(float2)));
 }
 
-template <bool BF16, bool MASK, bool PAIR>
+template <bool BF16, bool MASK, bool PAIR, bool IMAGE>
 static int launch_attn(const CUtensorMap& tm, const AttnParams& p, const Plan& pl, int batch, cudaStream_t st) {
   static bool configured[64] = {};
   int dev = 0;
   if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CQ_ERR_LAUNCH;
   if (!configured[dev]) {
-    if (cudaFuncSetAttribute(chunk_attn_kernel<BF16, MASK, PAIR>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess) return CQ_ERR_LAUNCH;
+    if (cudaFuncSetAttribute(chunk_attn_kernel<BF16, MASK, PAIR, IMAGE>, cudaFuncAttributeMaxDynamicSharedMemorySize, SMEM_BYTES) != cudaSuccess ||
+        cudaFuncSetAttribute(chunk_unpack_kernel<BF16, MASK>, cudaFuncAttributeMaxDynamicSharedMemorySize, 3 * TILE_BYTES + 1024) != cudaSuccess)
+      return CQ_ERR_LAUNCH;
     configured[dev] = true;
   }
   const dim3 grid(pl.row_blocks, batch * p.p.hkv, pl.grid_parts);
-  chunk_attn_kernel<BF16, MASK, PAIR><<<grid, THREADS, SMEM_BYTES, st>>>(tm, p);
-  if (const int rc = check_launch()) return rc;
+  if (IMAGE) {
+    const dim3 tiles((p.p.t_vis + 127) / 128 + p.image_fp_tiles, batch * p.p.hkv);
+    chunk_unpack_kernel<BF16, MASK><<<tiles, 256, 3 * TILE_BYTES + 1024, st>>>(p);
+    if (const int rc = check_launch()) return rc;
+    if (const int rc = launched(launch_pdl(chunk_attn_kernel<BF16, MASK, PAIR, IMAGE>, grid, dim3(Roles<IMAGE>::THREADS), SMEM_BYTES, st, tm, p))) return rc;
+  } else {
+    chunk_attn_kernel<BF16, MASK, PAIR, IMAGE><<<grid, Roles<IMAGE>::THREADS, SMEM_BYTES, st>>>(tm, p);
+    if (const int rc = check_launch()) return rc;
+  }
   if (pl.parts == 1) return CQ_OK;
   const int64_t rows = (int64_t)batch * p.p.hkv * p.p.rows;
   return launched(launch_pdl(chunk_combine_kernel<BF16>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p, rows));
@@ -649,10 +774,13 @@ extern "C" int cq_chunk_attn(const cq_chunk_args* a, void* workspace, size_t wor
   p.idesc_mn = chunk::idesc_of(bf16, 0, 1, 128, 128);
   const size_t rows = (size_t)a->batch * a->n_q_heads * a->q_len;
   p.status = static_cast<int*>(workspace);
-  p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256);
+  p.image = static_cast<unsigned char*>(workspace) + 256;
+  p.image_fp_tiles = (a->t_fp + 127) / 128;
+  p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256 + chunk::images_of(a, pl));
   p.part_ml = reinterpret_cast<float2*>(p.part_o + rows * pl.parts * 128);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-#define CQ_RUN(B, M) (pl.pair ? chunk::launch_attn<B, M, true>(tm, p, pl, a->batch, st) : chunk::launch_attn<B, M, false>(tm, p, pl, a->batch, st))
+#define CQ_RUN(B, M) (pl.image ? chunk::launch_attn<B, M, true, true>(tm, p, pl, a->batch, st) : \
+                      pl.pair ? chunk::launch_attn<B, M, true, false>(tm, p, pl, a->batch, st) : chunk::launch_attn<B, M, false, false>(tm, p, pl, a->batch, st))
   if (bf16) return a->mask ? CQ_RUN(true, true) : CQ_RUN(true, false);
   return a->mask ? CQ_RUN(false, true) : CQ_RUN(false, false);
 #undef CQ_RUN
