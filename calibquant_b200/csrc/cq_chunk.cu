@@ -27,12 +27,12 @@ using namespace ptx;
 using namespace tc;
 
 constexpr int PRODUCERS = 8;
-// Threads and registers.  Without images: 8 softmax warps, 8 producers, the issuer's warpgroup; 256 x 120 + 256 x 88 + 128 x 64 = the launch's
-// 640 x 96.  With images: 8 softmax warps, which hold a row's 128 scores at once, and the issuer's warpgroup; 256 x 200 + 128 x 96
+// Threads and registers.  Without images: 8 softmax warps, 8 producers, the issuer's warpgroup; 256 x 104 + 256 x 88 + 128 x 96 = the launch's
+// 640 x 96.  With images: 8 softmax warps, which hold a row's 128 scores at once, and the issuer's warpgroup; 256 x 184 + 128 x 128
 // = 63 488 of the launch's 384 x 168.
 template <bool IMAGE> struct Roles {
   static constexpr int MMA_WARP = IMAGE ? 8 : 16, THREADS = IMAGE ? 384 : 640;
-  static constexpr int SOFTMAX_REGS = IMAGE ? 200 : 120, CONTROL_REGS = IMAGE ? 96 : 64, PRODUCER_REGS = 88;
+  static constexpr int SOFTMAX_REGS = IMAGE ? 184 : 104, CONTROL_REGS = IMAGE ? 128 : 96, PRODUCER_REGS = 88;
 };
 constexpr int SMEM_BYTES = 7 * TILE_BYTES + 1024;
 constexpr uint32_t WAIT_TRIES = 1u << 22;
@@ -311,7 +311,7 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
     const Range k = {uniform(kr.nv), uniform(kr.t0), uniform(kr.n)};
     const uint32_t lead = elect_one();
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-    constexpr uint64_t tile16 = TILE_BYTES >> 4;
+    constexpr uint32_t tile16 = TILE_BYTES >> 4;
     const uint64_t qd = smem_desc(q_s, 16, 1024), kd = smem_desc(k_s, 16, 1024), kmd = smem_desc(k_s, PANEL_BYTES, 1024), vd = smem_desc(v_s, PANEL_BYTES, 1024);
     bool ok = true;
     const auto all = [](bool r) { return __all_sync(0xffffffffu, r) != 0; };
@@ -331,20 +331,20 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
     };
     const auto issue_s = [&](auto xc, auto bc, int j) {      // S_x = Q_x K^T of key tile j
       constexpr int x = decltype(xc)::value, buf = decltype(bc)::value;
-      constexpr uint64_t q0 = PAIR && x ? tile16 : 0, hi = 2 * buf * tile16, lo = hi + tile16;
+      constexpr uint32_t q0 = PAIR && x ? tile16 : 0, hi = 2 * buf * tile16, lo = hi + tile16;
       if (!lead) return;
       const uint32_t d = tm + (uint32_t)x * 128u;
       if (k.t0 + j < k.nv) {                                 // the small terms first: sums are cut off, not rounded
 #pragma unroll
         for (int ks = 0; ks < 16; ++ks) {
-          const uint64_t qo = (uint64_t)((((ks & 7) >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
-          umma(d, qd + (q0 + qo), kmd + ((ks < 8 ? lo : hi) + (uint64_t)((ks & 7) * 128)), a.idesc_mn, ks > 0);
+          const uint32_t qo = (uint32_t)((((ks & 7) >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
+          umma(d, desc_at(qd, q0 + qo), desc_at(kmd, (ks < 8 ? lo : hi) + (ks & 7) * 128), a.idesc_mn, ks > 0);
         }
       } else {
 #pragma unroll
         for (int ks = 0; ks < 8; ++ks) {
-          const uint64_t qo = (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
-          umma(d, qd + (q0 + qo), kd + (hi + qo), a.idesc_kmajor, ks > 0);
+          const uint32_t qo = (uint32_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
+          umma(d, desc_at(qd, q0 + qo), desc_at(kd, hi + qo), a.idesc_kmajor, ks > 0);
         }
       }
       umma_commit(&bar_s[x]);
@@ -360,7 +360,7 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
         if (lead) {
 #pragma unroll
           for (int ks = 4 * half; ks < 4 * half + 4; ++ks)
-            umma_ts(tm + 256u + (uint32_t)x * 128u, tm + (uint32_t)x * 128u + (uint32_t)ks * 8u, vd + (buf * tile16 + (uint64_t)(ks * 128)), a.idesc_mn,
+            umma_ts(tm + 256u + (uint32_t)x * 128u, tm + (uint32_t)x * 128u + (uint32_t)ks * 8u, desc_at(vd, buf * tile16 + ks * 128), a.idesc_mn,
                     (ks > 0 || count > 0) ? 1u : 0u);
         }
       }

@@ -130,7 +130,7 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
     const int nb = uniform(nb_lane), n_x = uniform(n_x_lane);
     const uint32_t lead = elect_one();
     const uint32_t tm = __shfl_sync(0xffffffffu, tmem, 0);
-    constexpr uint64_t tile16 = TILE_BYTES >> 4;
+    constexpr uint32_t tile16 = TILE_BYTES >> 4;
     const uint64_t kd = smem_desc(k_s, 16, 1024), md = smem_desc(k_s, PANEL_BYTES, 1024), qd = smem_desc(q_s, 16, 1024);
     const auto all = [](bool r) { return __all_sync(0xffffffffu, r) != 0; };
     // slot and tile as constants: with both as indices the issuing lane's address arithmetic held up the tensor pipe
@@ -141,15 +141,15 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
           // its small terms first: sums are cut off, not rounded
 #pragma unroll
           for (int ks = 0; ks < 16; ++ks) {
-            constexpr uint64_t lo = (2 * x + 1) * tile16, hi = 2 * x * tile16;
-            const uint64_t qo = (uint64_t)((((ks & 7) >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
-            umma(tm + (uint32_t)(x * 256 + s * 128), md + ((ks < 8 ? lo : hi) + (uint64_t)((ks & 7) * 128)), qd + (s * tile16 + qo), a.idesc_mn, ks > 0);
+            constexpr uint32_t lo = (2 * x + 1) * tile16, hi = 2 * x * tile16;
+            const uint32_t qo = (uint32_t)((((ks & 7) >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
+            umma(tm + (uint32_t)(x * 256 + s * 128), desc_at(md, (ks < 8 ? lo : hi) + (ks & 7) * 128), desc_at(qd, s * tile16 + qo), a.idesc_mn, ks > 0);
           }
         } else {
 #pragma unroll
           for (int ks = 0; ks < 8; ++ks) {
-            const uint64_t qo = (uint64_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
-            umma(tm + (uint32_t)(x * 256 + s * 128), kd + (2 * x * tile16 + qo), qd + (s * tile16 + qo), a.idesc_kmajor, ks > 0);
+            const uint32_t qo = (uint32_t)(((ks >> 2) * PANEL_BYTES + (ks & 3) * 32) >> 4);
+            umma(tm + (uint32_t)(x * 256 + s * 128), desc_at(kd, 2 * x * tile16 + qo), desc_at(qd, s * tile16 + qo), a.idesc_kmajor, ks > 0);
           }
         }
         umma_commit(&bar_d[x][s]);

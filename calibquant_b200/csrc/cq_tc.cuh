@@ -100,6 +100,14 @@ __device__ __forceinline__ uint64_t smem_desc(uint32_t addr, uint32_t lbo_bytes,
   return d;
 }
 
+// The same descriptor with its start address moved by `units` of 16 bytes.  The address field lies in the low word and cannot carry out of
+// it (shared memory ends below 256 KB): one 32-bit addition, and one register, per operand.
+__device__ __forceinline__ uint64_t desc_at(uint64_t desc, uint32_t units) {
+  uint64_t d;
+  asm("mov.b64 %0, {%1, %2};" : "=l"(d) : "r"((uint32_t)desc + units), "r"((uint32_t)(desc >> 32)));
+  return d;
+}
+
 // Instruction descriptor of kind::f16 with fp32 accumulators: A K-major, B K-major or MN-major, an M x N tile.
 inline uint32_t make_idesc(int is_bf16, int b_mn_major, int m, int n) {
   uint32_t d = 0;
