@@ -7,7 +7,7 @@
 // The keys of a CTA are a part of the request's key tiles, visual ones first (`parts` on the grid); partial results are merged by
 // combine_kernel.  Roles:
 //   warps 0-3 / 4-7  softmax of A / B: thread = row; running maximum and sum, probabilities back to tensor memory
-//   warps 8-15       operands: codes from global memory (requested two tiles ahead), unpacked into 16-bit tiles in shared memory: two
+//   warps 8-15       operands: codes from global memory (requested a tile ahead), unpacked into 16-bit tiles in shared memory: two
 //                    buffers of keys (two terms each) and one of values, two where there is one query tile; full-precision
 //                    rows into the same layout
 //   warp 16          issues the products
@@ -230,21 +230,21 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
     bool ok = true;
     clear_q(ptid, 256);
 
-    Unit ku[2][2], vu[2][2];                  // requested: [tile of two][unit of the warp's two]
-    const auto request_k = [&](int j, Unit (&x)[2]) {
+    Unit ku[2], vu[2];                        // requested: the warp's two units
+    const auto request_k = [&](int j) {
       const int tile = k.t0 + j;
       if (j < k.n && tile < k.nv) {
-        load_k_unit(p, bh, tile, pw, lane, x[0]);
-        load_k_unit(p, bh, tile, pw + 8, lane, x[1]);
+        load_k_unit(p, bh, tile, pw, lane, ku[0]);
+        load_k_unit(p, bh, tile, pw + 8, lane, ku[1]);
       }
     };
-    const auto request_v = [&](int j, Unit (&x)[2]) {
+    const auto request_v = [&](int j) {
       const int tile = k.t0 + j;
       if (j < k.n && tile < k.nv) {
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int key = tile * 128 + (pw + 8 * u) * 8 + (lane >> 2);
-          load_v_unit(p, bh, tile, pw + 8 * u, lane, key < p.t_vis && takes_part<BF16, MASK>(p, b, key), x[u]);
+          load_v_unit(p, bh, tile, pw + 8 * u, lane, key < p.t_vis && takes_part<BF16, MASK>(p, b, key), vu[u]);
         }
       }
     };
@@ -257,47 +257,39 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
       __syncwarp();
       if (lane == 0) mbar_arrive(bar);
     };
-    const auto produce_k = [&](int j, Unit (&x)[2]) {
-      if (j >= k.n || !ok) return;
-      const int tile = k.t0 + j, buf = j & 1;
-      const uint32_t hi = k_s + buf * 2 * TILE_BYTES, lo = hi + TILE_BYTES;
-      wait_free(&bar_kfree[buf], j >> 1);
-      if (!ok) return;
-      if (tile < k.nv) {
-        store_k_unit<BF16>(hi, lo, x[0], pw, lane);
-        store_k_unit<BF16>(hi, lo, x[1], pw + 8, lane);
-      } else {
-        fill_fp_tile<BF16, MASK>(p, p.k_fp, b, hk, (tile - k.nv) * 128, live, false, hi, ptid);
+    request_k(0);
+    request_v(0);
+    // Keys one tile ahead of values: scores come first.  What the next use needs is requested behind the fence, which would wait for
+    // it.  One copy of this code: with two tiles requested ahead and the loop written out twice instructions were missing
+    for (int j = -1; j < k.n && ok; ++j) {
+      if (j + 1 < k.n) {
+        const int tile = k.t0 + j + 1, buf = (j + 1) & 1;
+        const uint32_t hi = k_s + buf * 2 * TILE_BYTES, lo = hi + TILE_BYTES;
+        wait_free(&bar_kfree[buf], (j + 1) >> 1);
+        if (!ok) break;
+        if (tile < k.nv) {
+          store_k_unit<BF16>(hi, lo, ku[0], pw, lane);
+          store_k_unit<BF16>(hi, lo, ku[1], pw + 8, lane);
+        } else {
+          fill_fp_tile<BF16, MASK>(p, p.k_fp, b, hk, (tile - k.nv) * 128, live, false, hi, ptid);
+        }
+        publish(&bar_k[buf]);
+        request_k(j + 2);
       }
-      publish(&bar_k[buf]);
-      request_k(j + 2, x);                    // behind the fence, which would wait for what is under way
-    };
-    const auto produce_v = [&](int j, Unit (&x)[2]) {
-      if (j >= k.n || !ok) return;
-      const int tile = k.t0 + j, buf = PAIR ? 0 : j & 1;
-      const uint32_t dst = v_s + buf * TILE_BYTES;
-      wait_free(&bar_vfree[buf], PAIR ? j : j >> 1);
-      if (!ok) return;
-      if (tile < k.nv) {
-        store_v_unit<BF16>(dst, x[0], pw, lane);
-        store_v_unit<BF16>(dst, x[1], pw + 8, lane);
-      } else {
-        fill_fp_tile<BF16, MASK>(p, p.v_fp, b, hk, (tile - k.nv) * 128, live, true, dst, ptid);
+      if (j >= 0) {
+        const int tile = k.t0 + j, buf = PAIR ? 0 : j & 1;
+        const uint32_t dst = v_s + buf * TILE_BYTES;
+        wait_free(&bar_vfree[buf], PAIR ? j : j >> 1);
+        if (!ok) break;
+        if (tile < k.nv) {
+          store_v_unit<BF16>(dst, vu[0], pw, lane);
+          store_v_unit<BF16>(dst, vu[1], pw + 8, lane);
+        } else {
+          fill_fp_tile<BF16, MASK>(p, p.v_fp, b, hk, (tile - k.nv) * 128, live, true, dst, ptid);
+        }
+        publish(&bar_v[buf]);
+        request_v(j + 1);
       }
-      publish(&bar_v[buf]);
-      request_v(j + 2, x);
-    };
-    request_k(0, ku[0]);
-    request_k(1, ku[1]);
-    request_v(0, vu[0]);
-    request_v(1, vu[1]);
-    // keys one tile ahead of values: scores come first
-    produce_k(0, ku[0]);
-    for (int j = 0; j < k.n && ok; j += 2) {
-      produce_k(j + 1, ku[1]);
-      produce_v(j, vu[0]);
-      produce_k(j + 2, ku[0]);
-      produce_v(j + 1, vu[1]);
     }
     if (!ok && lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
   } else if (warp >= MMA_WARP) {
