@@ -18,6 +18,7 @@
 
 #include <type_traits>
 
+#include "cq_chunk_few.cuh"
 #include "cq_chunk_tc.cuh"
 
 namespace cq {
@@ -666,13 +667,20 @@ constexpr int IMAGE_BLOCKS = 3;
 
 // ---- host ---------------------------------------------------------------------------------------------------------
 struct Plan {
-  bool pair, image;
+  bool few, pair, image;      // few: cq_chunk_few.cu
   int queries, row_blocks, grid_parts, parts;      // queries of a tile
 };
 // Split of the key tiles: as many CTAs as fill the SMs, in whole rounds where there are several; a CTA costs about three key tiles beside
 // its own (its start, and its partial result).
 static Plan make_plan(const cq_chunk_args* a) {
   Plan pl;
+  pl.few = (int64_t)a->q_len * (a->n_q_heads / a->n_kv_heads) <= FEW_ROWS;
+  pl.pair = pl.image = false;
+  if (pl.few) {
+    pl.queries = pl.row_blocks = 0;
+    pl.grid_parts = pl.parts = few_parts((int64_t)a->batch * a->n_kv_heads, (a->t_vis + 255) / 256 + (a->t_fp + 255) / 256);
+    return pl;
+  }
   pl.queries = 128 / (a->n_q_heads / a->n_kv_heads);
   pl.pair = a->q_len > pl.queries;
   const int block = pl.queries * (pl.pair ? 2 : 1);
@@ -702,6 +710,13 @@ static size_t workspace_bytes(const cq_chunk_args* a, const Plan& pl) {
   return 256 + images_of(a, pl) + (pl.parts == 1 ? 0 : rows * pl.parts * (128 * sizeof(float) + sizeof(float2)));
 }
 
+template <bool BF16>
+static int launch_combine(const AttnParams& p, int batch, cudaStream_t st) {
+  if (p.parts == 1) return CQ_OK;
+  const int64_t rows = (int64_t)batch * p.p.hkv * p.p.rows;
+  return launched(launch_pdl(chunk_combine_kernel<BF16>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p, rows));
+}
+
 template <bool BF16, bool MASK, bool PAIR, bool IMAGE>
 static int launch_attn(const CUtensorMap& tm, const AttnParams& p, const Plan& pl, int batch, cudaStream_t st) {
   static bool configured[64] = {};
@@ -723,9 +738,7 @@ static int launch_attn(const CUtensorMap& tm, const AttnParams& p, const Plan& p
     chunk_attn_kernel<BF16, MASK, PAIR, IMAGE><<<grid, Roles<IMAGE>::THREADS, SMEM_BYTES, st>>>(tm, p);
     if (const int rc = check_launch()) return rc;
   }
-  if (pl.parts == 1) return CQ_OK;
-  const int64_t rows = (int64_t)batch * p.p.hkv * p.p.rows;
-  return launched(launch_pdl(chunk_combine_kernel<BF16>, dim3((unsigned)((rows + 7) / 8)), dim3(256), 0, st, p, rows));
+  return launch_combine<BF16>(p, batch, st);
 }
 
 static bool attn_valid(const cq_chunk_args* a) {
@@ -759,8 +772,6 @@ extern "C" int cq_chunk_attn(const cq_chunk_args* a, void* workspace, size_t wor
   p.parts = pl.parts;
   p.scale = 0.08838834764831845f;
   p.tile_queries = pl.queries; p.tile_rows = pl.queries * p.p.n_rep;
-  CUtensorMap tm;
-  if (!chunk::query_map(&tm, a, pl.queries)) return CQ_ERR_LAUNCH;
   const int bf16 = a->dtype == CQ_DTYPE_BF16;
   p.idesc_kmajor = chunk::idesc_of(bf16, 0, 0, 128, 128);
   p.idesc_mn = chunk::idesc_of(bf16, 0, 1, 128, 128);
@@ -771,6 +782,13 @@ extern "C" int cq_chunk_attn(const cq_chunk_args* a, void* workspace, size_t wor
   p.part_o = reinterpret_cast<float*>(static_cast<char*>(workspace) + 256 + chunk::images_of(a, pl));
   p.part_ml = reinterpret_cast<float2*>(p.part_o + rows * pl.parts * 128);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (pl.few) {
+    const chunk::FewParams f = {p.p, pl.parts, p.part_o, p.part_ml, nullptr, nullptr, nullptr, nullptr, 0};
+    if (const int rc = chunk::few_run(f, a->batch, bf16, false, st)) return rc;
+    return bf16 ? chunk::launch_combine<true>(p, a->batch, st) : chunk::launch_combine<false>(p, a->batch, st);
+  }
+  CUtensorMap tm;
+  if (!chunk::query_map(&tm, a, pl.queries)) return CQ_ERR_LAUNCH;
 #define CQ_RUN(B, M) (pl.image ? chunk::launch_attn<B, M, true, true>(tm, p, pl, a->batch, st) : \
                       pl.pair ? chunk::launch_attn<B, M, true, false>(tm, p, pl, a->batch, st) : chunk::launch_attn<B, M, false, false>(tm, p, pl, a->batch, st))
   if (bf16) return a->mask ? CQ_RUN(true, true) : CQ_RUN(true, false);

@@ -1,0 +1,498 @@
+// The chunk attention and the key weights for few rows (up to 16 of a KV head: single tokens, drafts): what counts is how fast codes are
+// unpacked, so they go from global memory to registers and from there, as operands, into the warp MMA (m16n8k16); no tile is built.
+//
+// A warp takes groups of 32 keys.  Keys are the M side, query rows the N side (NT blocks of eight):
+//   S^T = K Q^T       A = keys (16 keys x 16 channels, pairs along the channels).  scale * code is exact as the sum of two 16-bit products,
+//                     the scale's upper and lower bits by the code; the minima come in as a product of their own, one per group.
+//   O^T += V^T P^T    A = values (16 channels x 16 keys, pairs along the keys), scale * code + minimum rounded once; B = probabilities,
+//                     transposed from the layout of S^T by movmatrix.
+// Which key (channel) a lane's row of A is, is free to choose: lane (g, c) takes the codes of word g % 4 of its group, the lower or the
+// upper four by g / 4.  So it loads one word per channel (key), half of which it uses, and a byte permute of two words leaves the pairs of
+// four A registers: one operation per code.  Register j = 2 * block + half of a lane stands for key (channel) index_of(g, j).
+// Each warp has a softmax of its own (running maximum and sum); a CTA's eight warps are merged in shared memory, CTAs by
+// the combine launch.
+#include <math.h>
+
+#include <type_traits>
+
+#include "cq_chunk_few.cuh"
+#include "cq_ptx.cuh"
+
+namespace cq {
+namespace chunk {
+namespace few {
+
+using namespace ptx;
+
+constexpr int WARPS = 8, THREADS = WARPS * 32;
+constexpr float LOG2E = 1.4426950408889634f, SCALE = 0.08838834764831845f;
+
+__device__ __forceinline__ float ex2_approx(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+template <bool BF16>
+__device__ __forceinline__ float number(uint16_t bits) {
+  return BF16 ? __uint_as_float((uint32_t)bits << 16) : __half2float(__ushort_as_half(bits));
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  uint32_t r;
+  if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t fma2(uint32_t a, uint32_t b, uint32_t c) {
+  uint32_t r;
+  if (BF16) asm("fma.rn.bf16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  else asm("fma.rn.f16x2 %0, %1, %2, %3;" : "=r"(r) : "r"(a), "r"(b), "r"(c));
+  return r;
+}
+template <bool BF16>
+__device__ __forceinline__ uint32_t sub2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  if (BF16) asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  else asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+template <bool BF16>
+__device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
+  if (BF16) mma_bf16(d, a0, a1, a2, a3, b0, b1);
+  else mma_f16(d, a0, a1, a2, a3, b0, b1);
+}
+// codes j of two words (their lower or upper halves side by side in z) as a pair of numbers
+template <bool BF16>
+__device__ __forceinline__ uint32_t code_pair(uint32_t z, int j) {
+  return sub2<BF16>(((z >> (4 * j)) & 0x000f000fu) | (BF16 ? 0x43004300u : 0x64006400u), BF16 ? 0x43004300u : 0x64006400u);
+}
+// Place within a group of 32 of row g (0..7) of register j = 2 * block + half
+__device__ __forceinline__ int index_of(int g, int j) { return (g & 3) * 8 + (g >> 2) * 4 + j; }
+
+// Scales of a group's keys for two neighbouring channels: upper and lower bits, each exact times a code.
+struct Pair { uint32_t hi, lo; };
+
+template <bool BF16, bool MASK, int NT, bool WEIGHTS>
+__global__ void __launch_bounds__(THREADS, 1) few_kernel(const __grid_constant__ FewParams a) {
+  using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
+  const Params& p = a.p;
+  constexpr int ROWS = 8 * NT;
+  // scales and minima of the keys of the tile at hand and the next: [buffer][group][channel pair]
+  __shared__ __align__(16) Pair scale_s[2][8][64];
+  __shared__ uint32_t mn_s[2][8][68];      // a row apart by four banks
+  extern __shared__ float merge_s[];       // [warp][row][128], then maxima and sums [warp][row]
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
+  const int hk = blockIdx.x % p.hkv, b = blockIdx.x / p.hkv, part = blockIdx.y;
+  const int64_t bh = blockIdx.x;
+  pdl_launch_dependents();
+  const int live = live_tokens(p), groups = p.t_vis >> 5, nv = (groups + 7) >> 3;
+  // tiles of eight groups: visual ones, then full-precision ones (of what is to be written, for weights)
+  const int64_t fp_keys = WEIGHTS ? a.capacity : live;
+  const int tiles = nv + (int)((fp_keys + 255) >> 8), per = (tiles + (int)gridDim.y - 1) / (int)gridDim.y;
+  const int t0 = min(tiles, part * per), t1 = min(tiles, t0 + per);
+  const uint32_t half_sel = g >> 2 ? 0x7632 : 0x5410;
+
+  // ---- the queries, as the B operand: channels 2c, 2c+1 (+8) of row g of block nt
+  uint32_t q[NT][8][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    const int r = nt * 8 + g, i = r / p.n_rep;
+    const T* src = static_cast<const T*>(p.q) + b * p.q_sb + i * p.q_st + (int64_t)(hk * p.n_rep + r - i * p.n_rep) * p.q_sh + 2 * c;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) q[nt][ks][e] = r < p.rows ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + e * 8) : 0u;
+  }
+  // rows 2c, 2c+1 of each block: full-precision tokens that they see, log-sum-exp (weights)
+  int limit[NT][2];
+  float lse[NT][2];
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int r = nt * 8 + 2 * c + e, i = r / p.n_rep;
+      limit[nt][e] = live - p.q_len + i + 1;
+      lse[nt][e] = INFINITY;
+      if (WEIGHTS && r < p.rows) {
+        const float v = p.lse[((int64_t)b * p.hq + hk * p.n_rep + r - i * p.n_rep) * p.q_len + i];
+        lse[nt][e] = v == -INFINITY ? INFINITY : v;      // such a row adds nothing
+      }
+    }
+
+  // scales and minima of visual tile t: thread = channel pair and two groups
+  const auto stage = [&](int t) {
+    if (t >= t1 || t >= nv) return;
+    const int pair = tid & 63;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const int grp = (tid >> 6) * 2 + e;
+      uint32_t s2 = 0, m2 = 0;
+      if (t * 8 + grp < groups) {
+        const int64_t at = (bh * 128 + 2 * pair) * groups + t * 8 + grp;
+        const uint16_t* s = static_cast<const uint16_t*>(p.k_scale);
+        const uint16_t* m = static_cast<const uint16_t*>(p.k_mn);
+        s2 = s[at] | (uint32_t)s[at + groups] << 16;
+        m2 = m[at] | (uint32_t)m[at + groups] << 16;
+      }
+      const uint32_t hi = s2 & 0xfff0fff0u;      // four (bf16) or seven (fp16) significant bits; with a code's four they fit the type
+      scale_s[t & 1][grp][pair] = {hi, sub2<BF16>(s2, hi)};
+      mn_s[t & 1][grp][pair] = m2;
+    }
+  };
+
+  uint32_t kw[8][4];      // codes of channels 2c, 2c+1, 2c+8, 2c+9 of each 16
+  const auto load_k = [&](int t) {
+    const int grp = t * 8 + warp;
+    if (t >= t1 || grp >= groups) return;
+    const uint32_t* src = p.k_code + (bh * 128 + 2 * c) * (p.t_vis >> 3) + grp * 4 + (g & 3);
+    const int64_t row = p.t_vis >> 3;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) kw[ks][e] = src[(ks * 16 + (e >> 1) * 8 + (e & 1)) * row];
+  };
+
+  float m_ref[NT][2], l_run[NT][2], o[8][NT][4];      // rows 2c, 2c+1; o: channel block, as the A rows are ordered
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) { m_ref[nt][e] = -INFINITY; l_run[nt][e] = 0.f; }
+#pragma unroll
+  for (int i = 0; i < 8; ++i)
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
+
+  stage(t0);
+  if (t0 < nv) load_k(t0);
+  for (int t = t0; t < t1; ++t) {
+    const bool vis = t < nv;
+    const int buf = t & 1;
+    __syncthreads();
+    stage(t + 1);
+    // this warp's 32 keys: first one in cache order, how many there are
+    const int key0 = vis ? (t * 8 + warp) * 32 : p.t_vis + ((t - nv) * 8 + warp) * 32;
+    const int there = vis ? min(32, p.t_vis - key0) : min(32, live - (key0 - p.t_vis));
+    if (there <= 0 && !(WEIGHTS && !vis && key0 - p.t_vis < a.capacity)) continue;
+
+    float mask[2][2];
+    bool dead = false;
+    if (MASK) {
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int k = index_of(g, j);
+        mask[j >> 1][j & 1] = k < there ? Elem<T>::to_f(static_cast<const T*>(p.mask)[b * p.mask_sb + mask_index(p, key0 + k)]) : -INFINITY;
+      }
+      dead = __any_sync(0xffffffffu, mask[0][0] == -INFINITY || mask[0][1] == -INFINITY || mask[1][0] == -INFINITY || mask[1][1] == -INFINITY);
+    }
+
+    // ---- scores: s[block][nt]: key index_of(g, 2 * block + (e >> 1)), row 2c + (e & 1)
+    float s[2][NT][4], small[2][NT][4];
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[mb][nt][e] = small[mb][nt][e] = 0.f;
+    uint32_t vw[2][2][2][4];                    // codes of the values: [k step][half][key 2c or 2c+1][channel group]
+    uint2 vs[2][2][2], vm[2][2][2];             // their scales and minima, all four groups
+    if (vis) {
+      if (!WEIGHTS) {
+#pragma unroll
+        for (int kt = 0; kt < 2; ++kt)
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int64_t tok = bh * p.t_vis + key0 + index_of(2 * c + e, 2 * kt + h);
+#pragma unroll
+              for (int grp = 0; grp < 4; ++grp) vw[kt][h][e][grp] = p.v_code[tok * 16 + grp * 4 + (g & 3)];
+              vs[kt][h][e] = reinterpret_cast<const uint2*>(p.v_scale)[tok];
+              vm[kt][h][e] = reinterpret_cast<const uint2*>(p.v_mn)[tok];
+            }
+      }
+      float minima[NT][4];
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) minima[nt][e] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        const Pair sa = scale_s[buf][warp][ks * 8 + c], sb = scale_s[buf][warp][ks * 8 + c + 4];
+        const uint32_t za = prmt(kw[ks][0], kw[ks][1], half_sel), zb = prmt(kw[ks][2], kw[ks][3], half_sel);
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb) {
+          const uint32_t c0 = code_pair<BF16>(za, 2 * mb), c1 = code_pair<BF16>(za, 2 * mb + 1), c2 = code_pair<BF16>(zb, 2 * mb), c3 = code_pair<BF16>(zb, 2 * mb + 1);
+          constexpr uint32_t zero = 0x80008000u;      // -0: what is added to a product and leaves its sign
+          const uint32_t h0 = fma2<BF16>(c0, sa.hi, zero), h1 = fma2<BF16>(c1, sa.hi, zero), h2 = fma2<BF16>(c2, sb.hi, zero), h3 = fma2<BF16>(c3, sb.hi, zero);
+          const uint32_t l0 = fma2<BF16>(c0, sa.lo, zero), l1 = fma2<BF16>(c1, sa.lo, zero), l2 = fma2<BF16>(c2, sb.lo, zero), l3 = fma2<BF16>(c3, sb.lo, zero);
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) {
+            mma<BF16>(s[mb][nt], h0, h1, h2, h3, q[nt][ks][0], q[nt][ks][1]);
+            mma<BF16>(small[mb][nt], l0, l1, l2, l3, q[nt][ks][0], q[nt][ks][1]);
+          }
+        }
+        // minima of the tile's eight groups as rows g
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+          mma<BF16>(minima[nt], mn_s[buf][g][ks * 8 + c], 0u, mn_s[buf][g][ks * 8 + c + 4], 0u, q[nt][ks][0], q[nt][ks][1]);
+      }
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float own = __shfl_sync(0xffffffffu, minima[nt][e], warp * 4 + c);
+#pragma unroll
+          for (int mb = 0; mb < 2; ++mb) {
+            s[mb][nt][e] += small[mb][nt][e] + own;
+            s[mb][nt][e + 2] += small[mb][nt][e + 2] + own;
+          }
+        }
+      load_k(t + 1);
+    } else if (there > 0) {
+      const T* src = static_cast<const T*>(p.k_fp) + b * p.fp_sb + hk * p.fp_sh + (int64_t)(key0 - p.t_vis) * 128 + 2 * c;
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) {
+        uint32_t f[4][2];                       // [j][channels 2c.. or 2c+8..]
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+#pragma unroll
+          for (int e = 0; e < 2; ++e)
+            f[j][e] = index_of(g, j) < there ? *reinterpret_cast<const uint32_t*>(src + (int64_t)index_of(g, j) * 128 + ks * 16 + e * 8) : 0u;
+#pragma unroll
+        for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma<BF16>(s[mb][nt], f[2 * mb][0], f[2 * mb + 1][0], f[2 * mb][1], f[2 * mb + 1][1], q[nt][ks][0], q[nt][ks][1]);
+      }
+    }
+    // natural units, masks
+#pragma unroll
+    for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int k = index_of(g, 2 * mb + (e >> 1));
+          float x = s[mb][nt][e] * SCALE;
+          if (MASK) x = mask[mb][e >> 1] == -INFINITY ? -INFINITY : x + mask[mb][e >> 1];
+          if (k >= there || (!vis && key0 - p.t_vis + k >= limit[nt][e & 1])) x = -INFINITY;
+          s[mb][nt][e] = x;
+        }
+
+    if constexpr (WEIGHTS) {
+      float w[4] = {};                          // key index_of(g, j), over this lane's rows, then the other lanes'
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) w[j] += ex2_approx((s[j >> 1][nt][(j & 1) * 2 + e] - lse[nt][e]) * LOG2E);
+        w[j] += __shfl_xor_sync(0xffffffffu, w[j], 1);
+        w[j] += __shfl_xor_sync(0xffffffffu, w[j], 2);
+      }
+      if (c == 0) {
+        const int64_t first = vis ? bh * p.t_vis + key0 : bh * a.capacity + key0 - p.t_vis;
+        const float* in = vis ? a.vis_in : a.fp_in;
+        float* out = vis ? a.vis : a.fp;
+        const int end = vis ? there : (int)min((int64_t)32, a.capacity - (key0 - p.t_vis));
+        const int k = index_of(g, 0);
+#pragma unroll
+        for (int j = 0; j < 4; ++j)
+          if (k + j < end) out[first + k + j] = (in ? in[first + k + j] : 0.f) + w[j];
+      }
+      continue;
+    }
+
+    // ---- softmax of the warp's keys so far
+    bool grow_any = false;
+    float top[NT][2];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        float x = fmaxf(fmaxf(s[0][nt][e], s[0][nt][e + 2]), fmaxf(s[1][nt][e], s[1][nt][e + 2]));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 4));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 8));
+        x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 16));
+        top[nt][e] = fmaxf(x, m_ref[nt][e]);
+        grow_any |= top[nt][e] - m_ref[nt][e] > 5.5f;      // a row keeps its reference until the true maximum is e^5.5 above it
+      }
+    if (__any_sync(0xffffffffu, grow_any)) {
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float alpha = top[nt][e] == -INFINITY ? 1.f : ex2_approx((m_ref[nt][e] - top[nt][e]) * LOG2E);
+          m_ref[nt][e] = top[nt][e];
+          l_run[nt][e] *= alpha;
+#pragma unroll
+          for (int i = 0; i < 8; ++i) { o[i][nt][e] *= alpha; o[i][nt][e + 2] *= alpha; }
+        }
+    }
+    uint32_t pb[2][NT][2];                      // probabilities, B operand: [k step][nt][half]
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+      const float m0 = m_ref[nt][0] == -INFINITY ? 0.f : m_ref[nt][0], m1 = m_ref[nt][1] == -INFINITY ? 0.f : m_ref[nt][1];
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          const float e0 = ex2_approx((s[mb][nt][2 * h] - m0) * LOG2E), e1 = ex2_approx((s[mb][nt][2 * h + 1] - m1) * LOG2E);
+          l_run[nt][0] += e0;
+          l_run[nt][1] += e1;
+          pb[mb][nt][h] = movmatrix_trans(pack16<BF16>(e0, e1));
+        }
+    }
+
+    // ---- values
+    if (vis) {
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        if (MASK && dead) {      // a key that takes no part: zeros, whatever its values are
+#pragma unroll
+          for (int h = 0; h < 2; ++h)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const int k = index_of(2 * c + e, 2 * kt + h);
+              if (Elem<T>::to_f(static_cast<const T*>(p.mask)[b * p.mask_sb + mask_index(p, key0 + k)]) == -INFINITY) vs[kt][h][e] = vm[kt][h][e] = make_uint2(0, 0);
+            }
+        }
+#pragma unroll
+        for (int grp = 0; grp < 4; ++grp) {
+          uint32_t s2[2], m2[2], z[2];
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const uint32_t sel = grp & 1 ? 0x7632 : 0x5410;
+            s2[h] = grp < 2 ? prmt(vs[kt][h][0].x, vs[kt][h][1].x, sel) : prmt(vs[kt][h][0].y, vs[kt][h][1].y, sel);
+            m2[h] = grp < 2 ? prmt(vm[kt][h][0].x, vm[kt][h][1].x, sel) : prmt(vm[kt][h][0].y, vm[kt][h][1].y, sel);
+            z[h] = prmt(vw[kt][h][0][grp], vw[kt][h][1][grp], half_sel);
+          }
+#pragma unroll
+          for (int mb = 0; mb < 2; ++mb) {
+            const uint32_t a0 = fma2<BF16>(code_pair<BF16>(z[0], 2 * mb), s2[0], m2[0]), a1 = fma2<BF16>(code_pair<BF16>(z[0], 2 * mb + 1), s2[0], m2[0]);
+            const uint32_t a2 = fma2<BF16>(code_pair<BF16>(z[1], 2 * mb), s2[1], m2[1]), a3 = fma2<BF16>(code_pair<BF16>(z[1], 2 * mb + 1), s2[1], m2[1]);
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) mma<BF16>(o[grp * 2 + mb][nt], a0, a1, a2, a3, pb[kt][nt][0], pb[kt][nt][1]);
+          }
+        }
+      }
+    } else {
+      // rows of full-precision values, transposed block by block: a lane loads the channel pairs of rows 2c and 2c+1 of A
+      const T* src = static_cast<const T*>(p.v_fp) + b * p.fp_sb + hk * p.fp_sh + (int64_t)(key0 - p.t_vis) * 128;
+#pragma unroll
+      for (int kt = 0; kt < 2; ++kt) {
+        bool use[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h) use[h] = index_of(g, 2 * kt + h) < there && !(MASK && mask[kt][h] == -INFINITY);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          uint32_t av[2][2];                    // [half of the keys][channel half]
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            const T* row = src + (int64_t)index_of(g, 2 * kt + h) * 128 + (i >> 1) * 32 + 2 * (i & 1);
+            const uint32_t w0 = use[h] ? *reinterpret_cast<const uint32_t*>(row + index_of(2 * c, 0)) : 0u;
+            const uint32_t w1 = use[h] ? *reinterpret_cast<const uint32_t*>(row + index_of(2 * c + 1, 0)) : 0u;
+            av[h][0] = movmatrix_trans(prmt(w0, w1, 0x5410));
+            av[h][1] = movmatrix_trans(prmt(w0, w1, 0x7632));
+          }
+#pragma unroll
+          for (int nt = 0; nt < NT; ++nt) mma<BF16>(o[i][nt], av[0][0], av[0][1], av[1][0], av[1][1], pb[kt][nt][0], pb[kt][nt][1]);
+        }
+      }
+    }
+  }
+  if constexpr (WEIGHTS) return;
+
+  // ---- the warps' results
+  float* ml_s = merge_s + WARPS * ROWS * 128;
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      float l = l_run[nt][e];
+      l += __shfl_xor_sync(0xffffffffu, l, 4);
+      l += __shfl_xor_sync(0xffffffffu, l, 8);
+      l += __shfl_xor_sync(0xffffffffu, l, 16);
+      const int r = nt * 8 + 2 * c + e;
+      if (g == 0) {
+        ml_s[(warp * ROWS + r) * 2] = m_ref[nt][e];
+        ml_s[(warp * ROWS + r) * 2 + 1] = l;
+      }
+#pragma unroll
+      for (int i = 0; i < 8; ++i)
+#pragma unroll
+        for (int h = 0; h < 2; ++h) merge_s[(warp * ROWS + r) * 128 + (i >> 1) * 32 + index_of(g, 2 * (i & 1) + h)] = o[i][nt][e + 2 * h];
+    }
+  __syncthreads();
+  for (int r = warp; r < min(ROWS, p.rows); r += WARPS) {
+    float m = -INFINITY, l = 0.f, x[4] = {};
+    for (int w = 0; w < WARPS; ++w) m = fmaxf(m, ml_s[(w * ROWS + r) * 2]);
+    for (int w = 0; w < WARPS; ++w) {
+      const float mw = ml_s[(w * ROWS + r) * 2];
+      if (mw == -INFINITY) continue;
+      const float f = ex2_approx((mw - m) * LOG2E);
+      const float4 v = *reinterpret_cast<const float4*>(merge_s + (w * ROWS + r) * 128 + lane * 4);
+      l = fmaf(ml_s[(w * ROWS + r) * 2 + 1], f, l);
+      x[0] = fmaf(v.x, f, x[0]); x[1] = fmaf(v.y, f, x[1]); x[2] = fmaf(v.z, f, x[2]); x[3] = fmaf(v.w, f, x[3]);
+    }
+    const int i = r / p.n_rep;
+    const int64_t h = hk * p.n_rep + r - i * p.n_rep;
+    if (gridDim.y == 1) {
+      const float inv = l > 0.f ? 1.f / l : 0.f;
+      T* dst = static_cast<T*>(p.out) + b * p.o_sb + i * p.o_st + h * p.o_sh + lane * 4;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<BF16>(x[0] * inv, x[1] * inv), pack16<BF16>(x[2] * inv, x[3] * inv));
+      if (p.lse && lane == 0) p.lse[(b * (int64_t)p.hq + h) * p.q_len + i] = l > 0.f ? m + logf(l) : -INFINITY;
+    } else {
+      const int64_t at = (bh * p.rows + r) * a.parts + part;
+      *reinterpret_cast<float4*>(a.part_o + at * 128 + lane * 4) = make_float4(x[0], x[1], x[2], x[3]);
+      if (lane == 0) a.part_ml[at] = make_float2(m, l);
+    }
+  }
+}
+
+template <bool BF16, bool MASK, int NT, bool WEIGHTS>
+static int run(const FewParams& p, int batch, cudaStream_t st) {
+  constexpr int smem = WEIGHTS ? 0 : (WARPS * 8 * NT * 130) * (int)sizeof(float);
+  if (smem > 24 * 1024) {
+    static bool configured[64] = {};
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return CQ_ERR_LAUNCH;
+    if (!configured[dev]) {
+      if (cudaFuncSetAttribute(few_kernel<BF16, MASK, NT, WEIGHTS>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess) return CQ_ERR_LAUNCH;
+      configured[dev] = true;
+    }
+  }
+  few_kernel<BF16, MASK, NT, WEIGHTS><<<dim3((unsigned)(batch * p.p.hkv), p.parts), THREADS, smem, st>>>(p);
+  return check_launch();
+}
+
+}  // namespace few
+
+// Tiles of 256 keys; CTAs for every SM once or more, in whole rounds; a CTA costs about a tile beside its own.
+int few_parts(int64_t heads, int64_t tiles) {
+  const int sms = sm_count();
+  int best = 1;
+  double cost = 1e300;
+  for (int s = 1; s <= 64 && s <= tiles; ++s) {
+    const int64_t per = (tiles + s - 1) / s;
+    if ((tiles + per - 1) / per != s) continue;
+    const double c = (double)((heads * s + sms - 1) / sms) * (per + 1.0) + (s > 1 ? 1.0 : 0.0);
+    if (c < cost) { cost = c; best = s; }
+  }
+  return best;
+}
+
+int few_run(const FewParams& p, int batch, bool bf16, bool weights, cudaStream_t st) {
+  using few::run;
+#define CQ_NT(B, M, W) (p.p.rows <= 8 ? run<B, M, 1, W>(p, batch, st) : run<B, M, 2, W>(p, batch, st))
+#define CQ_M(B, W) (p.p.mask ? CQ_NT(B, true, W) : CQ_NT(B, false, W))
+  if (weights) return bf16 ? CQ_M(true, true) : CQ_M(false, true);
+  return bf16 ? CQ_M(true, false) : CQ_M(false, false);
+#undef CQ_M
+#undef CQ_NT
+}
+
+}  // namespace chunk
+}  // namespace cq

@@ -1,0 +1,25 @@
+// Few rows (cq_chunk_few.cu): what the entry points of the chunk attention and of the key weights call.
+#pragma once
+
+#include "cq_chunk.cuh"
+
+namespace cq {
+namespace chunk {
+
+constexpr int FEW_ROWS = 16;
+
+struct FewParams {
+  Params p;
+  int parts;                                   // CTAs per KV head
+  float* part_o;                               // attention, parts > 1: [batch][KV head][row][part][128] and maximum, sum
+  float2* part_ml;
+  const float *vis_in, *fp_in;                 // weights
+  float *vis, *fp;
+  int64_t capacity;
+};
+
+int few_parts(int64_t heads, int64_t tiles);
+int few_run(const FewParams& p, int batch, bool bf16, bool weights, cudaStream_t st);
+
+}  // namespace chunk
+}  // namespace cq

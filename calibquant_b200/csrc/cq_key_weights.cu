@@ -15,6 +15,7 @@
 
 #include <type_traits>
 
+#include "cq_chunk_few.cuh"
 #include "cq_chunk_tc.cuh"
 
 namespace cq {
@@ -368,9 +369,16 @@ extern "C" int cq_key_weights(const cq_chunk_args* a, const float* w_vis_in, con
   if (!chunk::valid(a) || !a->lse || (a->t_vis && !w_vis) || !w_fp || w_capacity < a->t_fp) return CQ_ERR_BAD_ARG;
   if (!weights_supported(a, w_capacity)) return CQ_ERR_UNSUPPORTED;
   const Plan pl = make_plan(a, w_capacity);
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (!workspace || !aligned16(workspace) || workspace_bytes < bytes_of(a, w_capacity, pl)) return CQ_ERR_WORKSPACE;
   if (a->batch == 0) return CQ_OK;
   const int bf16 = a->dtype == CQ_DTYPE_BF16;
+  if ((int64_t)a->q_len * (a->n_q_heads / a->n_kv_heads) <= chunk::FEW_ROWS) {
+    const int64_t heads = (int64_t)a->batch * a->n_kv_heads;
+    const chunk::FewParams f = {chunk::make_params(a), chunk::few_parts(heads, (a->t_vis + 255) / 256 + (w_capacity + 255) / 256), nullptr, nullptr,
+                                w_vis_in, w_fp_in, w_vis, w_fp, w_capacity};
+    return chunk::few_run(f, a->batch, bf16, true, st);
+  }
   WeightParams p = {};
   p.p = chunk::make_params(a);
   p.vis_in = w_vis_in; p.fp_in = w_fp_in; p.vis = w_vis; p.fp = w_fp;
@@ -383,7 +391,6 @@ extern "C" int cq_key_weights(const cq_chunk_args* a, const float* w_vis_in, con
   p.idesc_kmajor = chunk::idesc_of(bf16, 0, 0, 128, pl.nb);
   p.idesc_mn = chunk::idesc_of(bf16, 1, 0, 128, pl.nb);
   p.status = static_cast<int*>(workspace);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
 #define CQ_RUN(B, M) (pl.nb == 32 ? run<B, M, 32>(tm, p, pl, st) : run<B, M, 128>(tm, p, pl, st))
   if (bf16) return a->mask ? CQ_RUN(true, true) : CQ_RUN(true, false);
   return a->mask ? CQ_RUN(false, true) : CQ_RUN(false, false);
