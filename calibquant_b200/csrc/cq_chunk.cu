@@ -674,11 +674,12 @@ struct Plan {
 // its own (its start, and its partial result).
 static Plan make_plan(const cq_chunk_args* a) {
   Plan pl;
-  pl.few = (int64_t)a->q_len * (a->n_q_heads / a->n_kv_heads) <= FEW_ROWS;
+  const int64_t rows = (int64_t)a->q_len * (a->n_q_heads / a->n_kv_heads);
+  pl.few = rows <= FEW_ROWS;
   pl.pair = pl.image = false;
   if (pl.few) {
     pl.queries = pl.row_blocks = 0;
-    pl.grid_parts = pl.parts = few_parts((int64_t)a->batch * a->n_kv_heads, (a->t_vis + 255) / 256 + (a->t_fp + 255) / 256);
+    pl.grid_parts = pl.parts = few_parts((int64_t)a->batch * a->n_kv_heads, (a->t_vis + 255) / 256 + (a->t_fp + 255) / 256, rows > 8);
     return pl;
   }
   pl.queries = 128 / (a->n_q_heads / a->n_kv_heads);

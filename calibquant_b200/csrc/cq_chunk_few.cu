@@ -9,8 +9,8 @@
 // Which key (channel) a lane's row of A is, is free to choose: lane (g, c) takes the codes of word g % 4 of its group, the lower or the
 // upper four by g / 4.  So it loads one word per channel (key), half of which it uses, and a byte permute of two words leaves the pairs of
 // four A registers: one operation per code.  Register j = 2 * block + half of a lane stands for key (channel) index_of(g, j).
-// Each warp has a softmax of its own (running maximum and sum); a CTA's eight warps are merged in shared memory, CTAs by
-// the combine launch.
+// Each warp has a softmax of its own (running maximum and sum) and its own two buffers in shared memory, which cp.async fills a group
+// ahead; warps do not wait for one another.  A CTA's eight warps are merged in shared memory at the end, CTAs by the combine launch.
 #include <math.h>
 
 #include <type_traits>
@@ -70,24 +70,40 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t z, int j) {
 // Place within a group of 32 of row g (0..7) of register j = 2 * block + half
 __device__ __forceinline__ int index_of(int g, int j) { return (g & 3) * 8 + (g >> 2) * 4 + j; }
 
-// Scales of a group's keys for two neighbouring channels: upper and lower bits, each exact times a code.
+// Scales of a group's keys for two neighbouring channels (upper and lower bits, each exact times a code) and their minima.
 struct Pair { uint32_t hi, lo; };
+// A group as a warp holds it: codes [channel][4 words] and [key][16 words], scales and minima of the values [key][4].
+struct __align__(16) Stage {
+  uint32_t k[128][4];
+  uint32_t v[32][16];
+  uint2 vs[32], vm[32];
+};
+struct __align__(16) KeyStage {
+  uint32_t k[128][4];
+};
+template <bool WEIGHTS> using StageOf = typename std::conditional<WEIGHTS, KeyStage, Stage>::type;
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
 
 template <bool BF16, bool MASK, int NT, bool WEIGHTS>
-__global__ void __launch_bounds__(THREADS, 1) few_kernel(const __grid_constant__ FewParams a) {
+__global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kernel(const __grid_constant__ FewParams a) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   const Params& p = a.p;
   constexpr int ROWS = 8 * NT;
-  // scales and minima of the keys of the tile at hand and the next: [buffer][group][channel pair]
-  __shared__ __align__(16) Pair scale_s[2][8][64];
-  __shared__ uint32_t mn_s[2][8][68];      // a row apart by four banks
-  extern __shared__ float merge_s[];       // [warp][row][128], then maxima and sums [warp][row]
+  __shared__ __align__(16) Pair scale_s[WARPS][64];
+  __shared__ uint32_t mn_s[WARPS][64];
+  extern __shared__ __align__(16) unsigned char dyn_s[];      // stages [warp][2]; at the end the warps' results [warp][row][128], [warp][row][2]
+  float* merge_s = reinterpret_cast<float*>(dyn_s);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int hk = blockIdx.x % p.hkv, b = blockIdx.x / p.hkv, part = blockIdx.y;
   const int64_t bh = blockIdx.x;
   pdl_launch_dependents();
   const int live = live_tokens(p), groups = p.t_vis >> 5, nv = (groups + 7) >> 3;
-  // tiles of eight groups: visual ones, then full-precision ones (of what is to be written, for weights)
+  // groups of 32 keys, eight to a tile: visual ones, then full-precision ones (of what is to be written, for weights)
   const int64_t fp_keys = WEIGHTS ? a.capacity : live;
   const int tiles = nv + (int)((fp_keys + 255) >> 8), per = (tiles + (int)gridDim.y - 1) / (int)gridDim.y;
   const int t0 = min(tiles, part * per), t1 = min(tiles, t0 + per);
@@ -120,37 +136,34 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const __grid_constant__
       }
     }
 
-  // scales and minima of visual tile t: thread = channel pair and two groups
-  const auto stage = [&](int t) {
-    if (t >= t1 || t >= nv) return;
-    const int pair = tid & 63;
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const int grp = (tid >> 6) * 2 + e;
-      uint32_t s2 = 0, m2 = 0;
-      if (t * 8 + grp < groups) {
-        const int64_t at = (bh * 128 + 2 * pair) * groups + t * 8 + grp;
-        const uint16_t* s = static_cast<const uint16_t*>(p.k_scale);
-        const uint16_t* m = static_cast<const uint16_t*>(p.k_mn);
-        s2 = s[at] | (uint32_t)s[at + groups] << 16;
-        m2 = m[at] | (uint32_t)m[at + groups] << 16;
-      }
-      const uint32_t hi = s2 & 0xfff0fff0u;      // four (bf16) or seven (fp16) significant bits; with a code's four they fit the type
-      scale_s[t & 1][grp][pair] = {hi, sub2<BF16>(s2, hi)};
-      mn_s[t & 1][grp][pair] = m2;
-    }
-  };
-
-  uint32_t kw[8][4];      // codes of channels 2c, 2c+1, 2c+8, 2c+9 of each 16
-  const auto load_k = [&](int t) {
+  using St = StageOf<WEIGHTS>;
+  St* stages = reinterpret_cast<St*>(dyn_s) + warp * 2;
+  uint32_t ks2[2], km2[2];                      // scales and minima of the next group: channels 4 lane .. 4 lane + 3
+  const auto request = [&](int t) {             // this warp's group of tile t
     const int grp = t * 8 + warp;
-    if (t >= t1 || grp >= groups) return;
-    const uint32_t* src = p.k_code + (bh * 128 + 2 * c) * (p.t_vis >> 3) + grp * 4 + (g & 3);
-    const int64_t row = p.t_vis >> 3;
+    if (t < t1 && grp < groups) {
+      St& st = stages[t & 1];
+      const uint4* k = reinterpret_cast<const uint4*>(p.k_code) + bh * 128 * groups + grp;
 #pragma unroll
-    for (int ks = 0; ks < 8; ++ks)
+      for (int e = 0; e < 4; ++e) cp_async16(smem_u32(&st.k[e * 32 + lane][0]), k + (int64_t)(e * 32 + lane) * groups);
+      if constexpr (!WEIGHTS) {
+        const int64_t tok = bh * p.t_vis + grp * 32;
+        const uint4* v = reinterpret_cast<const uint4*>(p.v_code) + tok * 4;
 #pragma unroll
-      for (int e = 0; e < 4; ++e) kw[ks][e] = src[(ks * 16 + (e >> 1) * 8 + (e & 1)) * row];
+        for (int e = 0; e < 4; ++e) cp_async16(smem_u32(&st.v[0][0]) + (e * 32 + lane) * 16, v + e * 32 + lane);
+        const char* sm = static_cast<const char*>(lane < 16 ? p.v_scale : p.v_mn) + tok * 8 + (lane & 15) * 16;
+        cp_async16(smem_u32(lane < 16 ? &st.vs[0] : &st.vm[0]) + (lane & 15) * 16, sm);
+      }
+      const int64_t at = (bh * 128 + 4 * lane) * groups + grp;
+      const uint16_t* s = static_cast<const uint16_t*>(p.k_scale) + at;
+      const uint16_t* m = static_cast<const uint16_t*>(p.k_mn) + at;
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        ks2[e] = s[2 * e * groups] | (uint32_t)s[(2 * e + 1) * groups] << 16;
+        km2[e] = m[2 * e * groups] | (uint32_t)m[(2 * e + 1) * groups] << 16;
+      }
+    }
+    cp_async_commit();
   };
 
   float m_ref[NT][2], l_run[NT][2], o[8][NT][4];      // rows 2c, 2c+1; o: channel block, as the A rows are ordered
@@ -165,17 +178,29 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const __grid_constant__
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
 
-  stage(t0);
-  if (t0 < nv) load_k(t0);
+  request(t0);
   for (int t = t0; t < t1; ++t) {
     const bool vis = t < nv;
-    const int buf = t & 1;
-    __syncthreads();
-    stage(t + 1);
     // this warp's 32 keys: first one in cache order, how many there are
     const int key0 = vis ? (t * 8 + warp) * 32 : p.t_vis + ((t - nv) * 8 + warp) * 32;
     const int there = vis ? min(32, p.t_vis - key0) : min(32, live - (key0 - p.t_vis));
-    if (there <= 0 && !(WEIGHTS && !vis && key0 - p.t_vis < a.capacity)) continue;
+    if (there <= 0 && !(WEIGHTS && !vis && key0 - p.t_vis < a.capacity)) {
+      request(t + 1);
+      continue;
+    }
+    const St& st = stages[t & 1];
+    __syncwarp();                               // the group before has been read by all lanes
+    if (vis) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const uint32_t hi = ks2[e] & 0xfff0fff0u;      // four (bf16) or seven (fp16) significant bits; with a code's four they fit the type
+        scale_s[warp][2 * lane + e] = {hi, sub2<BF16>(ks2[e], hi)};
+        mn_s[warp][2 * lane + e] = km2[e];
+      }
+    }
+    request(t + 1);
+    cp_async_wait<1>();
+    __syncwarp();
 
     float mask[2][2];
     bool dead = false;
@@ -196,23 +221,7 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const __grid_constant__
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[mb][nt][e] = small[mb][nt][e] = 0.f;
-    uint32_t vw[2][2][2][4];                    // codes of the values: [k step][half][key 2c or 2c+1][channel group]
-    uint2 vs[2][2][2], vm[2][2][2];             // their scales and minima, all four groups
     if (vis) {
-      if (!WEIGHTS) {
-#pragma unroll
-        for (int kt = 0; kt < 2; ++kt)
-#pragma unroll
-          for (int h = 0; h < 2; ++h)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int64_t tok = bh * p.t_vis + key0 + index_of(2 * c + e, 2 * kt + h);
-#pragma unroll
-              for (int grp = 0; grp < 4; ++grp) vw[kt][h][e][grp] = p.v_code[tok * 16 + grp * 4 + (g & 3)];
-              vs[kt][h][e] = reinterpret_cast<const uint2*>(p.v_scale)[tok];
-              vm[kt][h][e] = reinterpret_cast<const uint2*>(p.v_mn)[tok];
-            }
-      }
       float minima[NT][4];
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -220,8 +229,9 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const __grid_constant__
         for (int e = 0; e < 4; ++e) minima[nt][e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) {
-        const Pair sa = scale_s[buf][warp][ks * 8 + c], sb = scale_s[buf][warp][ks * 8 + c + 4];
-        const uint32_t za = prmt(kw[ks][0], kw[ks][1], half_sel), zb = prmt(kw[ks][2], kw[ks][3], half_sel);
+        const Pair sa = scale_s[warp][ks * 8 + c], sb = scale_s[warp][ks * 8 + c + 4];
+        const uint32_t (*kw)[4] = &st.k[ks * 16 + 2 * c];
+        const uint32_t za = prmt(kw[0][g & 3], kw[1][g & 3], half_sel), zb = prmt(kw[8][g & 3], kw[9][g & 3], half_sel);
 #pragma unroll
         for (int mb = 0; mb < 2; ++mb) {
           const uint32_t c0 = code_pair<BF16>(za, 2 * mb), c1 = code_pair<BF16>(za, 2 * mb + 1), c2 = code_pair<BF16>(zb, 2 * mb), c3 = code_pair<BF16>(zb, 2 * mb + 1);
@@ -234,23 +244,22 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const __grid_constant__
             mma<BF16>(small[mb][nt], l0, l1, l2, l3, q[nt][ks][0], q[nt][ks][1]);
           }
         }
-        // minima of the tile's eight groups as rows g
+        // the minima in every row
+        const uint32_t m0 = mn_s[warp][ks * 8 + c], m1 = mn_s[warp][ks * 8 + c + 4];
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt)
-          mma<BF16>(minima[nt], mn_s[buf][g][ks * 8 + c], 0u, mn_s[buf][g][ks * 8 + c + 4], 0u, q[nt][ks][0], q[nt][ks][1]);
+        for (int nt = 0; nt < NT; ++nt) mma<BF16>(minima[nt], m0, 0u, m1, 0u, q[nt][ks][0], q[nt][ks][1]);
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float own = __shfl_sync(0xffffffffu, minima[nt][e], warp * 4 + c);
+          const float own = minima[nt][e];
 #pragma unroll
           for (int mb = 0; mb < 2; ++mb) {
             s[mb][nt][e] += small[mb][nt][e] + own;
             s[mb][nt][e + 2] += small[mb][nt][e + 2] + own;
           }
         }
-      load_k(t + 1);
     } else if (there > 0) {
       const T* src = static_cast<const T*>(p.k_fp) + b * p.fp_sb + hk * p.fp_sh + (int64_t)(key0 - p.t_vis) * 128 + 2 * c;
 #pragma unroll
@@ -348,26 +357,31 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const __grid_constant__
 
     // ---- values
     if (vis) {
+     if constexpr (!WEIGHTS) {
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
-        if (MASK && dead) {      // a key that takes no part: zeros, whatever its values are
+        uint2 vs[2][2], vm[2][2];               // scales and minima of keys 2c, 2c+1 of both halves, all four groups of channels
+        int tok[2][2];
 #pragma unroll
-          for (int h = 0; h < 2; ++h)
+        for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              const int k = index_of(2 * c + e, 2 * kt + h);
-              if (Elem<T>::to_f(static_cast<const T*>(p.mask)[b * p.mask_sb + mask_index(p, key0 + k)]) == -INFINITY) vs[kt][h][e] = vm[kt][h][e] = make_uint2(0, 0);
-            }
-        }
+          for (int e = 0; e < 2; ++e) {
+            tok[h][e] = index_of(2 * c + e, 2 * kt + h);
+            vs[h][e] = st.vs[tok[h][e]];
+            vm[h][e] = st.vm[tok[h][e]];
+            // a key that takes no part: zeros, whatever its values are
+            if (MASK && dead && Elem<T>::to_f(static_cast<const T*>(p.mask)[b * p.mask_sb + mask_index(p, key0 + tok[h][e])]) == -INFINITY)
+              vs[h][e] = vm[h][e] = make_uint2(0, 0);
+          }
 #pragma unroll
         for (int grp = 0; grp < 4; ++grp) {
           uint32_t s2[2], m2[2], z[2];
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
             const uint32_t sel = grp & 1 ? 0x7632 : 0x5410;
-            s2[h] = grp < 2 ? prmt(vs[kt][h][0].x, vs[kt][h][1].x, sel) : prmt(vs[kt][h][0].y, vs[kt][h][1].y, sel);
-            m2[h] = grp < 2 ? prmt(vm[kt][h][0].x, vm[kt][h][1].x, sel) : prmt(vm[kt][h][0].y, vm[kt][h][1].y, sel);
-            z[h] = prmt(vw[kt][h][0][grp], vw[kt][h][1][grp], half_sel);
+            s2[h] = grp < 2 ? prmt(vs[h][0].x, vs[h][1].x, sel) : prmt(vs[h][0].y, vs[h][1].y, sel);
+            m2[h] = grp < 2 ? prmt(vm[h][0].x, vm[h][1].x, sel) : prmt(vm[h][0].y, vm[h][1].y, sel);
+            z[h] = prmt(st.v[tok[h][0]][grp * 4 + (g & 3)], st.v[tok[h][1]][grp * 4 + (g & 3)], half_sel);
           }
 #pragma unroll
           for (int mb = 0; mb < 2; ++mb) {
@@ -378,6 +392,7 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const __grid_constant__
           }
         }
       }
+     }
     } else {
       // rows of full-precision values, transposed block by block: a lane loads the channel pairs of rows 2c and 2c+1 of A
       const T* src = static_cast<const T*>(p.v_fp) + b * p.fp_sb + hk * p.fp_sh + (int64_t)(key0 - p.t_vis) * 128;
@@ -403,9 +418,14 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const __grid_constant__
       }
     }
   }
-  if constexpr (WEIGHTS) return;
+  if constexpr (WEIGHTS) {
+    cp_async_wait<0>();
+    return;
+  }
 
-  // ---- the warps' results
+  // ---- the warps' results, over the stages
+  cp_async_wait<0>();
+  __syncthreads();
   float* ml_s = merge_s + WARPS * ROWS * 128;
 #pragma unroll
   for (int nt = 0; nt < NT; ++nt)
@@ -454,7 +474,8 @@ __global__ void __launch_bounds__(THREADS, 1) few_kernel(const __grid_constant__
 
 template <bool BF16, bool MASK, int NT, bool WEIGHTS>
 static int run(const FewParams& p, int batch, cudaStream_t st) {
-  constexpr int smem = WEIGHTS ? 0 : (WARPS * 8 * NT * 130) * (int)sizeof(float);
+  constexpr int stages = WARPS * 2 * (int)sizeof(StageOf<WEIGHTS>), results = WEIGHTS ? 0 : WARPS * 8 * NT * 130 * (int)sizeof(float);
+  constexpr int smem = stages > results ? stages : results;
   if (smem > 24 * 1024) {
     static bool configured[64] = {};
     int dev = 0;
@@ -470,9 +491,9 @@ static int run(const FewParams& p, int batch, cudaStream_t st) {
 
 }  // namespace few
 
-// Tiles of 256 keys; CTAs for every SM once or more, in whole rounds; a CTA costs about a tile beside its own.
-int few_parts(int64_t heads, int64_t tiles) {
-  const int sms = sm_count();
+// Tiles of 256 keys; two CTAs an SM (one with more than eight rows, attention), in whole rounds; a CTA costs about a tile beside its own.
+int few_parts(int64_t heads, int64_t tiles, bool one) {
+  const int sms = sm_count() * (one ? 1 : 2);
   int best = 1;
   double cost = 1e300;
   for (int s = 1; s <= 64 && s <= tiles; ++s) {

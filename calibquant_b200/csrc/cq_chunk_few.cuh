@@ -18,7 +18,7 @@ struct FewParams {
   int64_t capacity;
 };
 
-int few_parts(int64_t heads, int64_t tiles);
+int few_parts(int64_t heads, int64_t tiles, bool one);
 int few_run(const FewParams& p, int batch, bool bf16, bool weights, cudaStream_t st);
 
 }  // namespace chunk
