@@ -679,7 +679,10 @@ static Plan make_plan(const cq_chunk_args* a) {
   pl.pair = pl.image = false;
   if (pl.few) {
     pl.queries = pl.row_blocks = 0;
-    pl.grid_parts = pl.parts = few_parts((int64_t)a->batch * a->n_kv_heads, (a->t_vis + 255) / 256 + (a->t_fp + 255) / 256, rows > 8);
+    FewParams f = {};
+    f.p.t_vis = a->t_vis;
+    few_plan(f, (int64_t)a->batch * a->n_kv_heads, a->t_fp, false);
+    pl.grid_parts = pl.parts = f.parts;
     return pl;
   }
   pl.queries = 128 / (a->n_q_heads / a->n_kv_heads);
@@ -784,7 +787,9 @@ extern "C" int cq_chunk_attn(const cq_chunk_args* a, void* workspace, size_t wor
   p.part_ml = reinterpret_cast<float2*>(p.part_o + rows * pl.parts * 128);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (pl.few) {
-    const chunk::FewParams f = {p.p, pl.parts, p.part_o, p.part_ml, nullptr, nullptr, nullptr, nullptr, 0};
+    chunk::FewParams f = {};
+    f.p = p.p; f.part_o = p.part_o; f.part_ml = p.part_ml; f.status = p.status;
+    chunk::few_plan(f, (int64_t)a->batch * a->n_kv_heads, a->t_fp, false);
     if (const int rc = chunk::few_run(f, a->batch, bf16, false, st)) return rc;
     return bf16 ? chunk::launch_combine<true>(p, a->batch, st) : chunk::launch_combine<false>(p, a->batch, st);
   }

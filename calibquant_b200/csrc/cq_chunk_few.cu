@@ -1,22 +1,24 @@
 // The chunk attention and the key weights for few rows (up to 16 of a KV head: single tokens, drafts): what counts is how fast codes are
 // unpacked, so they go from global memory to registers and from there, as operands, into the warp MMA (m16n8k16); no tile is built.
 //
-// A warp takes groups of 32 keys.  Keys are the M side, query rows the N side (NT blocks of eight):
-//   S^T = K Q^T       A = keys (16 keys x 16 channels, pairs along the channels).  scale * code is exact as the sum of two 16-bit products,
-//                     the scale's upper and lower bits by the code; the minima come in as a product of their own, one per group.
+// A warp takes runs of up to eight groups of 32 keys.  Keys are the M side, query rows the N side (NT blocks of eight):
+//   S^T = K Q^T       A = codes (16 keys x 16 channels, pairs along the channels), exact as they are; B = query * scale, which changes with
+//                     the group and is exact as the sum of two 16-bit numbers (the product rounded, and what an fma finds
+//                     missing); the minima come in as a product of their own, one per run.  fp16 queries are scaled by a power of two per
+//                     row, so that the products stay in range.
 //   O^T += V^T P^T    A = values (16 channels x 16 keys, pairs along the keys), scale * code + minimum rounded once; B = probabilities,
 //                     transposed from the layout of S^T by movmatrix.
 // Which key (channel) a lane's row of A is, is free to choose: lane (g, c) takes the codes of word g % 4 of its group, the lower or the
 // upper four by g / 4.  So it loads one word per channel (key), half of which it uses, and a byte permute of two words leaves the pairs of
 // four A registers: one operation per code.  Register j = 2 * block + half of a lane stands for key (channel) index_of(g, j).
-// Each warp has a softmax of its own (running maximum and sum) and its own two buffers in shared memory, which cp.async fills a group
-// ahead; warps do not wait for one another.  A CTA's eight warps are merged in shared memory at the end, CTAs by the combine launch.
+// Each warp has a softmax of its own (running maximum and sum) and its own two buffers in shared memory, which TMA fills two groups
+// at a time while the two before are worked on; warps do not wait for one another.  A CTA's eight warps are merged in shared memory at the end, CTAs by the combine launch.
 #include <math.h>
 
 #include <type_traits>
 
 #include "cq_chunk_few.cuh"
-#include "cq_ptx.cuh"
+#include "cq_chunk_tc.cuh"
 
 namespace cq {
 namespace chunk {
@@ -31,10 +33,6 @@ __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
-}
-template <bool BF16>
-__device__ __forceinline__ float number(uint16_t bits) {
-  return BF16 ? __uint_as_float((uint32_t)bits << 16) : __half2float(__ushort_as_half(bits));
 }
 template <bool BF16>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
@@ -70,43 +68,44 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t z, int j) {
 // Place within a group of 32 of row g (0..7) of register j = 2 * block + half
 __device__ __forceinline__ int index_of(int g, int j) { return (g & 3) * 8 + (g >> 2) * 4 + j; }
 
-// Scales of a group's keys for two neighbouring channels (upper and lower bits, each exact times a code) and their minima.
-struct Pair { uint32_t hi, lo; };
-// A group as a warp holds it: codes [channel][4 words] and [key][16 words], scales and minima of the values [key][4].
-struct __align__(16) Stage {
-  uint32_t k[128][4];
-  uint32_t v[32][16];
-  uint2 vs[32], vm[32];
+// Two groups as a warp holds them: codes [channel][8 words] (32-byte swizzle) and [key][16 words] (64-byte swizzle), scales and minima of the
+// values [key][4].
+struct __align__(1024) Stage {
+  uint32_t k[128][8];
+  uint32_t v[64][16];
+  uint2 vs[64], vm[64];
 };
-struct __align__(16) KeyStage {
-  uint32_t k[128][4];
+struct __align__(1024) KeyStage {
+  uint32_t k[128][8];
 };
+// Scales and minima of the keys of a run of groups: [group][channel pair]
+struct __align__(16) Scales {
+  uint32_t s[8][64], m[8][64];
+};
+// words [row][quad * 4 ..] under the swizzles
+__device__ __forceinline__ int quad32(int row, int quad) { return (quad ^ ((row >> 2) & 1)) * 4; }
+__device__ __forceinline__ int quad64(int row, int quad) { return (quad ^ ((row >> 1) & 3)) * 4; }
+constexpr uint32_t WAIT_TRIES = 1u << 22;
 template <bool WEIGHTS> using StageOf = typename std::conditional<WEIGHTS, KeyStage, Stage>::type;
 
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
-template <int N> __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory"); }
-
 template <bool BF16, bool MASK, int NT, bool WEIGHTS>
-__global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kernel(const __grid_constant__ FewParams a) {
+__global__ void __launch_bounds__(THREADS, WEIGHTS ? 2 : 1) few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FewParams a) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   const Params& p = a.p;
   constexpr int ROWS = 8 * NT;
-  __shared__ __align__(16) Pair scale_s[WARPS][64];
-  __shared__ uint32_t mn_s[WARPS][64];
-  extern __shared__ __align__(16) unsigned char dyn_s[];      // stages [warp][2]; at the end the warps' results [warp][row][128], [warp][row][2]
+  extern __shared__ unsigned char smem_raw[];
+  unsigned char* dyn_s = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);      // stages [warp][2], scales [warp]; at the end
+                                                                                           // results [warp][row][128], [warp][row][2]
+  __shared__ __align__(8) uint64_t bar[WARPS][2];
   float* merge_s = reinterpret_cast<float*>(dyn_s);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int hk = blockIdx.x % p.hkv, b = blockIdx.x / p.hkv, part = blockIdx.y;
   const int64_t bh = blockIdx.x;
   pdl_launch_dependents();
-  const int live = live_tokens(p), groups = p.t_vis >> 5, nv = (groups + 7) >> 3;
-  // groups of 32 keys, eight to a tile: visual ones, then full-precision ones (of what is to be written, for weights)
-  const int64_t fp_keys = WEIGHTS ? a.capacity : live;
-  const int tiles = nv + (int)((fp_keys + 255) >> 8), per = (tiles + (int)gridDim.y - 1) / (int)gridDim.y;
-  const int t0 = min(tiles, part * per), t1 = min(tiles, t0 + per);
+  const int live = live_tokens(p), groups = p.t_vis >> 5;
+  // Runs of a.run groups, then full-precision groups (of what is to be written, for weights); all warps of the KV head take them in turn
+  const int runs = (groups + a.run - 1) / a.run;
+  const int units = runs + (int)(((WEIGHTS ? a.capacity : (int64_t)live) + 31) >> 5);
   const uint32_t half_sel = g >> 2 ? 0x7632 : 0x5410;
 
   // ---- the queries, as the B operand: channels 2c, 2c+1 (+8) of row g of block nt
@@ -119,6 +118,35 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
     for (int ks = 0; ks < 8; ++ks)
 #pragma unroll
       for (int e = 0; e < 2; ++e) q[nt][ks][e] = r < p.rows ? *reinterpret_cast<const uint32_t*>(src + ks * 16 + e * 8) : 0u;
+  }
+  float unit[NT][2];      // of the scores of rows 2c, 2c + 1: 1 / sqrt(128), times what fp16 queries were divided by
+#pragma unroll
+  for (int nt = 0; nt < NT; ++nt) {
+    unit[nt][0] = unit[nt][1] = SCALE;
+    if (!BF16) {
+      float top = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float2 v = __half22float2(*reinterpret_cast<const __half2*>(&q[nt][ks][e]));
+          top = fmaxf(top, fmaxf(fabsf(v.x), fabsf(v.y)));
+        }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      const int exponent = top > 0.f && top < INFINITY ? ilogbf(top) : 0;      // -24 .. 15
+      const __half down = __float2half_rn(exp2f((float)-(exponent / 2))), down2 = __float2half_rn(exp2f((float)-(exponent - exponent / 2)));
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          __half2 v = *reinterpret_cast<const __half2*>(&q[nt][ks][e]);
+          v = __hmul2(__hmul2(v, __half2half2(down)), __half2half2(down2));
+          q[nt][ks][e] = *reinterpret_cast<const uint32_t*>(&v);
+        }
+#pragma unroll
+      for (int e = 0; e < 2; ++e) unit[nt][e] = SCALE * exp2f((float)__shfl_sync(0xffffffffu, exponent, (2 * c + e) * 4));
+    }
   }
   // rows 2c, 2c+1 of each block: full-precision tokens that they see, log-sum-exp (weights)
   int limit[NT][2];
@@ -138,32 +166,64 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
 
   using St = StageOf<WEIGHTS>;
   St* stages = reinterpret_cast<St*>(dyn_s) + warp * 2;
-  uint32_t ks2[2], km2[2];                      // scales and minima of the next group: channels 4 lane .. 4 lane + 3
-  const auto request = [&](int t) {             // this warp's group of tile t
-    const int grp = t * 8 + warp;
-    if (t < t1 && grp < groups) {
-      St& st = stages[t & 1];
-      const uint4* k = reinterpret_cast<const uint4*>(p.k_code) + bh * 128 * groups + grp;
-#pragma unroll
-      for (int e = 0; e < 4; ++e) cp_async16(smem_u32(&st.k[e * 32 + lane][0]), k + (int64_t)(e * 32 + lane) * groups);
+  Scales& sc = reinterpret_cast<Scales*>(dyn_s + WARPS * 2 * sizeof(St))[warp];
+  if (lane == 0) {
+    mbar_init(&bar[warp][0], 1);
+    mbar_init(&bar[warp][1], 1);
+    mbar_fence_init();
+  }
+  __syncwarp();
+  bool ok = true;
+  uint32_t asked = 0, taken = 0;                // pairs of groups so far
+  const auto request = [&](int grp, int n) {    // the n (1 or 2) groups from grp on
+    if (lane == 0) {
+      St& st = stages[asked & 1];
+      uint64_t* full = &bar[warp][asked & 1];
+      mbar_expect_tx(full, sizeof(st.k) + (WEIGHTS ? 0 : 4096 + n * 512));
+      tma_load_2d(st.k, &tm_k, grp * 4, (int)(bh * 128), full);
       if constexpr (!WEIGHTS) {
         const int64_t tok = bh * p.t_vis + grp * 32;
-        const uint4* v = reinterpret_cast<const uint4*>(p.v_code) + tok * 4;
-#pragma unroll
-        for (int e = 0; e < 4; ++e) cp_async16(smem_u32(&st.v[0][0]) + (e * 32 + lane) * 16, v + e * 32 + lane);
-        const char* sm = static_cast<const char*>(lane < 16 ? p.v_scale : p.v_mn) + tok * 8 + (lane & 15) * 16;
-        cp_async16(smem_u32(lane < 16 ? &st.vs[0] : &st.vm[0]) + (lane & 15) * 16, sm);
-      }
-      const int64_t at = (bh * 128 + 4 * lane) * groups + grp;
-      const uint16_t* s = static_cast<const uint16_t*>(p.k_scale) + at;
-      const uint16_t* m = static_cast<const uint16_t*>(p.k_mn) + at;
-#pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        ks2[e] = s[2 * e * groups] | (uint32_t)s[(2 * e + 1) * groups] << 16;
-        km2[e] = m[2 * e * groups] | (uint32_t)m[(2 * e + 1) * groups] << 16;
+        tma_load_3d(st.v, &tm_v, 0, grp * 32, (int)bh, full);
+        bulk_load_1d(st.vs, static_cast<const char*>(p.v_scale) + tok * 8, n * 256, full);
+        bulk_load_1d(st.vm, static_cast<const char*>(p.v_mn) + tok * 8, n * 256, full);
       }
     }
-    cp_async_commit();
+    ++asked;
+  };
+  // Scales and minima of the keys of n groups from grp on, for channels 2 lane, 2 lane + 1 (+64): as wide as a run and the pitch of
+  // a channel allow, since every load of a warp touches 32 rows
+  const auto fetch_scales = [&](int grp, int n) {
+    uint32_t x[2][2][2][4];                     // [scale, minimum][lower, upper channels][channel][two groups a word]
+#pragma unroll
+    for (int kind = 0; kind < 2; ++kind)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const uint16_t* src = static_cast<const uint16_t*>(kind ? p.k_mn : p.k_scale) + (bh * 128 + h * 64 + 2 * lane + e) * groups + grp;
+          uint32_t (&w)[4] = x[kind][h][e];
+          if (a.wide == 8) {
+            const uint4 v = *reinterpret_cast<const uint4*>(src);
+            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
+          } else if (a.wide == 4) {
+            const uint2 v = *reinterpret_cast<const uint2*>(src), z = n > 4 ? *reinterpret_cast<const uint2*>(src + 4) : make_uint2(0, 0);
+            w[0] = v.x; w[1] = v.y; w[2] = z.x; w[3] = z.y;
+          } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              w[i] = 2 * i < n ? src[2 * i] : 0u;
+              if (2 * i + 1 < n) w[i] |= (uint32_t)src[2 * i + 1] << 16;
+            }
+          }
+        }
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const uint32_t sel = i & 1 ? 0x7632 : 0x5410;
+        sc.s[i][h * 32 + lane] = prmt(x[0][h][0][i >> 1], x[0][h][1][i >> 1], sel);
+        sc.m[i][h * 32 + lane] = prmt(x[1][h][0][i >> 1], x[1][h][1][i >> 1], sel);
+      }
   };
 
   float m_ref[NT][2], l_run[NT][2], o[8][NT][4];      // rows 2c, 2c+1; o: channel block, as the A rows are ordered
@@ -178,30 +238,38 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
 
-  request(t0);
-  for (int t = t0; t < t1; ++t) {
-    const bool vis = t < nv;
-    // this warp's 32 keys: first one in cache order, how many there are
-    const int key0 = vis ? (t * 8 + warp) * 32 : p.t_vis + ((t - nv) * 8 + warp) * 32;
-    const int there = vis ? min(32, p.t_vis - key0) : min(32, live - (key0 - p.t_vis));
-    if (there <= 0 && !(WEIGHTS && !vis && key0 - p.t_vis < a.capacity)) {
-      request(t + 1);
-      continue;
-    }
-    const St& st = stages[t & 1];
-    __syncwarp();                               // the group before has been read by all lanes
-    if (vis) {
+  for (int u = part * WARPS + warp; u < units; u += WARPS * (int)gridDim.y) {
+   const bool vis = u < runs;
+   const int grp0 = u * a.run, n = vis ? min(a.run, groups - grp0) : 1;      // the unit's groups
+   float minima[NT][4];                         // of group g, rows 2c, 2c + 1
+   __syncwarp();                                // what the unit before left has been read by all lanes
+   if (vis) {
+     request(grp0, min(2, n));
+     fetch_scales(grp0, n);
+     __syncwarp();
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const uint32_t hi = ks2[e] & 0xfff0fff0u;      // four (bf16) or seven (fp16) significant bits; with a code's four they fit the type
-        scale_s[warp][2 * lane + e] = {hi, sub2<BF16>(ks2[e], hi)};
-        mn_s[warp][2 * lane + e] = km2[e];
-      }
+     for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+       for (int e = 0; e < 4; ++e) minima[nt][e] = 0.f;
+#pragma unroll
+     for (int ks = 0; ks < 8; ++ks) {
+       const uint32_t m0 = sc.m[g][ks * 8 + c], m1 = sc.m[g][ks * 8 + c + 4];
+#pragma unroll
+       for (int nt = 0; nt < NT; ++nt) mma<BF16>(minima[nt], m0, 0u, m1, 0u, q[nt][ks][0], q[nt][ks][1]);
+     }
+   }
+   for (int i = 0; i < n; ++i) {
+    // this group's 32 keys: first one in cache order, how many there are
+    const int key0 = vis ? (grp0 + i) * 32 : p.t_vis + (u - runs) * 32;
+    const int there = vis ? 32 : min(32, live - (key0 - p.t_vis));
+    if (vis && !(i & 1)) {
+      __syncwarp();                             // the other stage has been read by all lanes
+      if (i + 2 < n) request(grp0 + i + 2, min(2, n - i - 2));
+      if (ok) ok = mbar_wait_bounded(&bar[warp][taken & 1], (taken >> 1) & 1, WAIT_TRIES);
+      ++taken;
     }
-    request(t + 1);
-    cp_async_wait<1>();
-    __syncwarp();
-
+    const St& st = stages[(taken - 1) & 1];
+    const int in = i & 1;                       // which of the stage's two groups
     float mask[2][2];
     bool dead = false;
     if (MASK) {
@@ -222,38 +290,35 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[mb][nt][e] = small[mb][nt][e] = 0.f;
     if (vis) {
-      float minima[NT][4];
-#pragma unroll
-      for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) minima[nt][e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) {
-        const Pair sa = scale_s[warp][ks * 8 + c], sb = scale_s[warp][ks * 8 + c + 4];
-        const uint32_t (*kw)[4] = &st.k[ks * 16 + 2 * c];
-        const uint32_t za = prmt(kw[0][g & 3], kw[1][g & 3], half_sel), zb = prmt(kw[8][g & 3], kw[9][g & 3], half_sel);
+        const uint32_t s2[2] = {sc.s[i][ks * 8 + c], sc.s[i][ks * 8 + c + 4]};
+        const int row = ks * 16 + 2 * c, quad = quad32(row, in) + (g & 3), quad8 = quad32(row + 8, in) + (g & 3);      // rows 2c, 2c + 1 have one swizzle
+        const uint32_t za = prmt(st.k[row][quad], st.k[row + 1][quad], half_sel), zb = prmt(st.k[row + 8][quad8], st.k[row + 9][quad8], half_sel);
+        uint32_t hi[NT][2], lo[NT][2];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            constexpr uint32_t zero = 0x80008000u;      // -0: what is added to a product and leaves its sign
+            hi[nt][e] = fma2<BF16>(q[nt][ks][e], s2[e], zero);
+            lo[nt][e] = fma2<BF16>(q[nt][ks][e], s2[e], hi[nt][e] ^ 0x80008000u);
+          }
 #pragma unroll
         for (int mb = 0; mb < 2; ++mb) {
           const uint32_t c0 = code_pair<BF16>(za, 2 * mb), c1 = code_pair<BF16>(za, 2 * mb + 1), c2 = code_pair<BF16>(zb, 2 * mb), c3 = code_pair<BF16>(zb, 2 * mb + 1);
-          constexpr uint32_t zero = 0x80008000u;      // -0: what is added to a product and leaves its sign
-          const uint32_t h0 = fma2<BF16>(c0, sa.hi, zero), h1 = fma2<BF16>(c1, sa.hi, zero), h2 = fma2<BF16>(c2, sb.hi, zero), h3 = fma2<BF16>(c3, sb.hi, zero);
-          const uint32_t l0 = fma2<BF16>(c0, sa.lo, zero), l1 = fma2<BF16>(c1, sa.lo, zero), l2 = fma2<BF16>(c2, sb.lo, zero), l3 = fma2<BF16>(c3, sb.lo, zero);
 #pragma unroll
           for (int nt = 0; nt < NT; ++nt) {
-            mma<BF16>(s[mb][nt], h0, h1, h2, h3, q[nt][ks][0], q[nt][ks][1]);
-            mma<BF16>(small[mb][nt], l0, l1, l2, l3, q[nt][ks][0], q[nt][ks][1]);
+            mma<BF16>(s[mb][nt], c0, c1, c2, c3, hi[nt][0], hi[nt][1]);
+            mma<BF16>(small[mb][nt], c0, c1, c2, c3, lo[nt][0], lo[nt][1]);
           }
         }
-        // the minima in every row
-        const uint32_t m0 = mn_s[warp][ks * 8 + c], m1 = mn_s[warp][ks * 8 + c + 4];
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) mma<BF16>(minima[nt], m0, 0u, m1, 0u, q[nt][ks][0], q[nt][ks][1]);
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float own = minima[nt][e];
+          const float own = __shfl_sync(0xffffffffu, minima[nt][e], i * 4 + c);
 #pragma unroll
           for (int mb = 0; mb < 2; ++mb) {
             s[mb][nt][e] += small[mb][nt][e] + own;
@@ -284,7 +349,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int k = index_of(g, 2 * mb + (e >> 1));
-          float x = s[mb][nt][e] * SCALE;
+          float x = s[mb][nt][e] * unit[nt][e & 1];
           if (MASK) x = mask[mb][e >> 1] == -INFINITY ? -INFINITY : x + mask[mb][e >> 1];
           if (k >= there || (!vis && key0 - p.t_vis + k >= limit[nt][e & 1])) x = -INFINITY;
           s[mb][nt][e] = x;
@@ -367,8 +432,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             tok[h][e] = index_of(2 * c + e, 2 * kt + h);
-            vs[h][e] = st.vs[tok[h][e]];
-            vm[h][e] = st.vm[tok[h][e]];
+            vs[h][e] = st.vs[in * 32 + tok[h][e]];
+            vm[h][e] = st.vm[in * 32 + tok[h][e]];
             // a key that takes no part: zeros, whatever its values are
             if (MASK && dead && Elem<T>::to_f(static_cast<const T*>(p.mask)[b * p.mask_sb + mask_index(p, key0 + tok[h][e])]) == -INFINITY)
               vs[h][e] = vm[h][e] = make_uint2(0, 0);
@@ -381,7 +446,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
             const uint32_t sel = grp & 1 ? 0x7632 : 0x5410;
             s2[h] = grp < 2 ? prmt(vs[h][0].x, vs[h][1].x, sel) : prmt(vs[h][0].y, vs[h][1].y, sel);
             m2[h] = grp < 2 ? prmt(vm[h][0].x, vm[h][1].x, sel) : prmt(vm[h][0].y, vm[h][1].y, sel);
-            z[h] = prmt(st.v[tok[h][0]][grp * 4 + (g & 3)], st.v[tok[h][1]][grp * 4 + (g & 3)], half_sel);
+            z[h] = prmt(st.v[in * 32 + tok[h][0]][quad64(tok[h][0], grp) + (g & 3)], st.v[in * 32 + tok[h][1]][quad64(tok[h][1], grp) + (g & 3)], half_sel);
           }
 #pragma unroll
           for (int mb = 0; mb < 2; ++mb) {
@@ -402,29 +467,27 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
 #pragma unroll
         for (int h = 0; h < 2; ++h) use[h] = index_of(g, 2 * kt + h) < there && !(MASK && mask[kt][h] == -INFINITY);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
+        for (int j = 0; j < 8; ++j) {
           uint32_t av[2][2];                    // [half of the keys][channel half]
 #pragma unroll
           for (int h = 0; h < 2; ++h) {
-            const T* row = src + (int64_t)index_of(g, 2 * kt + h) * 128 + (i >> 1) * 32 + 2 * (i & 1);
+            const T* row = src + (int64_t)index_of(g, 2 * kt + h) * 128 + (j >> 1) * 32 + 2 * (j & 1);
             const uint32_t w0 = use[h] ? *reinterpret_cast<const uint32_t*>(row + index_of(2 * c, 0)) : 0u;
             const uint32_t w1 = use[h] ? *reinterpret_cast<const uint32_t*>(row + index_of(2 * c + 1, 0)) : 0u;
             av[h][0] = movmatrix_trans(prmt(w0, w1, 0x5410));
             av[h][1] = movmatrix_trans(prmt(w0, w1, 0x7632));
           }
 #pragma unroll
-          for (int nt = 0; nt < NT; ++nt) mma<BF16>(o[i][nt], av[0][0], av[0][1], av[1][0], av[1][1], pb[kt][nt][0], pb[kt][nt][1]);
+          for (int nt = 0; nt < NT; ++nt) mma<BF16>(o[j][nt], av[0][0], av[0][1], av[1][0], av[1][1], pb[kt][nt][0], pb[kt][nt][1]);
         }
       }
     }
+   }
   }
-  if constexpr (WEIGHTS) {
-    cp_async_wait<0>();
-    return;
-  }
+  if (!__all_sync(0xffffffffu, ok) && lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
+  if constexpr (WEIGHTS) return;
 
-  // ---- the warps' results, over the stages
-  cp_async_wait<0>();
+  // ---- the warps' results, over scales and stages
   __syncthreads();
   float* ml_s = merge_s + WARPS * ROWS * 128;
 #pragma unroll
@@ -472,9 +535,27 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
   }
 }
 
+// Packed codes as a map of 32-bit words: `words` of a row, `rows` rows, `heads` of those (0: a map of two dimensions); a box of box_words x box_rows
+static bool code_map(CUtensorMap* m, const void* base, int64_t words, int64_t rows, int64_t heads, int box_words, int box_rows, CUtensorMapSwizzle swizzle) {
+  if (!base || words == 0 || rows == 0) {      // no packed keys: a map that nothing uses
+    *m = CUtensorMap{};
+    return true;
+  }
+  const EncodeTiled encode = encode_tiled();
+  if (!encode) return false;
+  const cuuint64_t dims[3] = {(cuuint64_t)words, (cuuint64_t)rows, (cuuint64_t)heads}, strides[2] = {(cuuint64_t)words * 4, (cuuint64_t)(words * rows) * 4};
+  const cuuint32_t box[3] = {(cuuint32_t)box_words, (cuuint32_t)box_rows, 1}, one[3] = {1, 1, 1};
+  return encode(m, CU_TENSOR_MAP_DATA_TYPE_INT32, heads ? 3 : 2, const_cast<void*>(base), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
+                CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
 template <bool BF16, bool MASK, int NT, bool WEIGHTS>
 static int run(const FewParams& p, int batch, cudaStream_t st) {
-  constexpr int stages = WARPS * 2 * (int)sizeof(StageOf<WEIGHTS>), results = WEIGHTS ? 0 : WARPS * 8 * NT * 130 * (int)sizeof(float);
+  CUtensorMap tk, tv;
+  if (!code_map(&tk, p.p.k_code, p.p.t_vis / 8, 128 * (int64_t)batch * p.p.hkv, 0, 8, 128, CU_TENSOR_MAP_SWIZZLE_32B) ||
+      !code_map(&tv, p.p.v_code, 16, p.p.t_vis, (int64_t)batch * p.p.hkv, 16, 64, CU_TENSOR_MAP_SWIZZLE_64B))
+    return CQ_ERR_LAUNCH;
+  constexpr int stages = 1024 + WARPS * (int)(sizeof(Scales) + 2 * sizeof(StageOf<WEIGHTS>)), results = WEIGHTS ? 0 : 1024 + WARPS * 8 * NT * 130 * (int)sizeof(float);
   constexpr int smem = stages > results ? stages : results;
   if (smem > 24 * 1024) {
     static bool configured[64] = {};
@@ -485,24 +566,26 @@ static int run(const FewParams& p, int batch, cudaStream_t st) {
       configured[dev] = true;
     }
   }
-  few_kernel<BF16, MASK, NT, WEIGHTS><<<dim3((unsigned)(batch * p.p.hkv), p.parts), THREADS, smem, st>>>(p);
+  few_kernel<BF16, MASK, NT, WEIGHTS><<<dim3((unsigned)(batch * p.p.hkv), p.parts), THREADS, smem, st>>>(tk, tv, p);
   return check_launch();
 }
 
 }  // namespace few
 
-// Tiles of 256 keys; two CTAs an SM (one with more than eight rows, attention), in whole rounds; a CTA costs about a tile beside its own.
-int few_parts(int64_t heads, int64_t tiles, bool one) {
-  const int sms = sm_count() * (one ? 1 : 2);
-  int best = 1;
+// CTAs per KV head: two an SM for weights, one for the attention, in whole rounds; a warp's time in groups, and about three more for
+// a CTA.  Then runs as long as a warp's share allows: eight groups, whose scales are loads of 16 bytes; four; or single groups.
+void few_plan(FewParams& f, int64_t heads, int64_t fp_keys, bool weights) {
+  const int64_t slots = (int64_t)sm_count() * (weights ? 2 : 1), groups = f.p.t_vis / 32, all = groups + (fp_keys + 31) / 32;
   double cost = 1e300;
-  for (int s = 1; s <= 64 && s <= tiles; ++s) {
-    const int64_t per = (tiles + s - 1) / s;
-    if ((tiles + per - 1) / per != s) continue;
-    const double c = (double)((heads * s + sms - 1) / sms) * (per + 1.0) + (s > 1 ? 1.0 : 0.0);
-    if (c < cost) { cost = c; best = s; }
+  f.parts = 1;
+  for (int s = 1; s <= 64 && s <= (all + few::WARPS - 1) / few::WARPS; ++s) {
+    const int64_t share = (all + (int64_t)s * few::WARPS - 1) / ((int64_t)s * few::WARPS);
+    const double c = (double)((heads * s + slots - 1) / slots) * (share + 3.0) + (s > 1 ? 3.0 : 0.0);
+    if (c < cost) { cost = c; f.parts = s; }
   }
-  return best;
+  const int64_t share = (groups + (int64_t)f.parts * few::WARPS - 1) / ((int64_t)f.parts * few::WARPS);
+  f.run = share > 4 ? 8 : share > 2 ? 4 : 1;
+  f.wide = f.run == 8 && groups % 8 == 0 ? 8 : f.run >= 4 && groups % 4 == 0 ? 4 : 1;
 }
 
 int few_run(const FewParams& p, int batch, bool bf16, bool weights, cudaStream_t st) {

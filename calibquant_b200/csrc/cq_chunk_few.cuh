@@ -10,15 +10,16 @@ constexpr int FEW_ROWS = 16;
 
 struct FewParams {
   Params p;
-  int parts;                                   // CTAs per KV head
+  int parts, run, wide;                        // CTAs per KV head, groups of a run, groups whose scales one load brings
   float* part_o;                               // attention, parts > 1: [batch][KV head][row][part][128] and maximum, sum
   float2* part_ml;
   const float *vis_in, *fp_in;                 // weights
   float *vis, *fp;
   int64_t capacity;
+  int* status;
 };
 
-int few_parts(int64_t heads, int64_t tiles, bool one);
+void few_plan(FewParams& f, int64_t heads, int64_t fp_keys, bool weights);      // fills parts, run and wide; p.t_vis is set
 int few_run(const FewParams& p, int batch, bool bf16, bool weights, cudaStream_t st);
 
 }  // namespace chunk

@@ -168,17 +168,29 @@ __device__ __forceinline__ void tma_load_4d(uint32_t dst, const void* tmap, int 
       : "memory");
 }
 
-// Queries [B,L,Hq,128] as a map (channel, head, query, batch row) whose box is 64 channels of the heads of a KV head for
-// `queries` queries: rows of 128 bytes in query-major order, the panel layout above.
-inline bool query_map(CUtensorMap* m, const cq_chunk_args* a, int queries) {
-  typedef CUresult (*Encode)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
-                             const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-  static const Encode encode = []() -> Encode {
+__device__ __forceinline__ void tma_load_3d(void* dst, const void* tmap, int c0, int c1, int c2, uint64_t* bar) {
+  asm volatile(
+      "cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
+      ::"r"(ptx::smem_u32(dst)), "l"(tmap), "r"(c0), "r"(c1), "r"(c2), "r"(ptx::smem_u32(bar))
+      : "memory");
+}
+
+typedef CUresult (*EncodeTiled)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*, const cuuint32_t*,
+                                const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+inline EncodeTiled encode_tiled() {
+  static const EncodeTiled fn = []() -> EncodeTiled {
     void* p = nullptr;
     cudaDriverEntryPointQueryResult q;
     if (cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &p, cudaEnableDefault, &q) != cudaSuccess || q != cudaDriverEntryPointSuccess) return nullptr;
-    return reinterpret_cast<Encode>(p);
+    return reinterpret_cast<EncodeTiled>(p);
   }();
+  return fn;
+}
+
+// Queries [B,L,Hq,128] as a map (channel, head, query, batch row) whose box is 64 channels of the heads of a KV head for
+// `queries` queries: rows of 128 bytes in query-major order, the panel layout above.
+inline bool query_map(CUtensorMap* m, const cq_chunk_args* a, int queries) {
+  const EncodeTiled encode = encode_tiled();
   if (!encode) return false;
   const cuuint64_t dims[4] = {128, (cuuint64_t)a->n_q_heads, (cuuint64_t)a->q_len, (cuuint64_t)a->batch};
   const int64_t step[3] = {a->q_strides[2], a->q_strides[1], a->q_strides[0]};

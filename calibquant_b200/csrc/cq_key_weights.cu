@@ -374,9 +374,11 @@ extern "C" int cq_key_weights(const cq_chunk_args* a, const float* w_vis_in, con
   if (a->batch == 0) return CQ_OK;
   const int bf16 = a->dtype == CQ_DTYPE_BF16;
   if ((int64_t)a->q_len * (a->n_q_heads / a->n_kv_heads) <= chunk::FEW_ROWS) {
-    const int64_t heads = (int64_t)a->batch * a->n_kv_heads;
-    const chunk::FewParams f = {chunk::make_params(a), chunk::few_parts(heads, (a->t_vis + 255) / 256 + (w_capacity + 255) / 256, false), nullptr, nullptr,
-                                w_vis_in, w_fp_in, w_vis, w_fp, w_capacity};
+    chunk::FewParams f = {};
+    f.p = chunk::make_params(a);
+    f.vis_in = w_vis_in; f.fp_in = w_fp_in; f.vis = w_vis; f.fp = w_fp; f.capacity = w_capacity;
+    f.status = static_cast<int*>(workspace);
+    chunk::few_plan(f, (int64_t)a->batch * a->n_kv_heads, w_capacity, true);
     return chunk::few_run(f, a->batch, bf16, true, st);
   }
   WeightParams p = {};
