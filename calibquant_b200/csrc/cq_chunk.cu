@@ -679,10 +679,7 @@ static Plan make_plan(const cq_chunk_args* a) {
   pl.pair = pl.image = false;
   if (pl.few) {
     pl.queries = pl.row_blocks = 0;
-    FewParams f = {};
-    f.p.t_vis = a->t_vis;
-    few_plan(f, (int64_t)a->batch * a->n_kv_heads, a->t_fp, false);
-    pl.grid_parts = pl.parts = f.parts;
+    pl.grid_parts = pl.parts = few_parts((int64_t)a->batch * a->n_kv_heads, a->t_vis, a->t_fp, rows > 8);
     return pl;
   }
   pl.queries = 128 / (a->n_q_heads / a->n_kv_heads);
@@ -788,8 +785,7 @@ extern "C" int cq_chunk_attn(const cq_chunk_args* a, void* workspace, size_t wor
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (pl.few) {
     chunk::FewParams f = {};
-    f.p = p.p; f.part_o = p.part_o; f.part_ml = p.part_ml; f.status = p.status;
-    chunk::few_plan(f, (int64_t)a->batch * a->n_kv_heads, a->t_fp, false);
+    f.p = p.p; f.part_o = p.part_o; f.part_ml = p.part_ml; f.status = p.status; f.parts = pl.parts;
     if (const int rc = chunk::few_run(f, a->batch, bf16, false, st)) return rc;
     return bf16 ? chunk::launch_combine<true>(p, a->batch, st) : chunk::launch_combine<false>(p, a->batch, st);
   }

@@ -1,18 +1,19 @@
 // The chunk attention and the key weights for few rows (up to 16 of a KV head: single tokens, drafts): what counts is how fast codes are
 // unpacked, so they go from global memory to registers and from there, as operands, into the warp MMA (m16n8k16); no tile is built.
 //
-// A warp takes runs of up to eight groups of 32 keys.  Keys are the M side, query rows the N side (NT blocks of eight):
+// A CTA goes over tiles of eight groups of 32 keys, a group for each of its eight warps.  Keys are the M side, query rows the N side (NT blocks of eight):
 //   S^T = K Q^T       A = codes (16 keys x 16 channels, pairs along the channels), exact as they are; B = query * scale, which changes with
 //                     the group and is exact as the sum of two 16-bit numbers (the product rounded, and what an fma finds
-//                     missing); the minima come in as a product of their own, one per run.  fp16 queries are scaled by a power of two per
+//                     missing); the minima come in as a product of their own.  fp16 queries are scaled by a power of two per
 //                     row, so that the products stay in range.
 //   O^T += V^T P^T    A = values (16 channels x 16 keys, pairs along the keys), scale * code + minimum rounded once; B = probabilities,
 //                     transposed from the layout of S^T by movmatrix.
 // Which key (channel) a lane's row of A is, is free to choose: lane (g, c) takes the codes of word g % 4 of its group, the lower or the
 // upper four by g / 4.  So it loads one word per channel (key), half of which it uses, and a byte permute of two words leaves the pairs of
 // four A registers: one operation per code.  Register j = 2 * block + half of a lane stands for key (channel) index_of(g, j).
-// Each warp has a softmax of its own (running maximum and sum) and its own two buffers in shared memory, which TMA fills two groups
-// at a time while the two before are worked on; warps do not wait for one another.  A CTA's eight warps are merged in shared memory at the end, CTAs by the combine launch.
+// Each warp has a softmax of its own (running maximum and sum), merged in shared memory at the end; CTAs are merged by the combine launch.
+// TMA brings the codes of the next tile in while one is worked on, whole 128-byte rows (with the 16 or 32 bytes of one or two groups a
+// request, the requests were the bound).
 #include <math.h>
 
 #include <type_traits>
@@ -68,44 +69,44 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t z, int j) {
 // Place within a group of 32 of row g (0..7) of register j = 2 * block + half
 __device__ __forceinline__ int index_of(int g, int j) { return (g & 3) * 8 + (g >> 2) * 4 + j; }
 
-// Two groups as a warp holds them: codes [channel][8 words] (32-byte swizzle) and [key][16 words] (64-byte swizzle), scales and minima of the
-// values [key][4].
+// A tile: codes [channel][32 words] and [two keys][32 words] (128-byte swizzle), scales and minima of the values [key][4].
 struct __align__(1024) Stage {
-  uint32_t k[128][8];
-  uint32_t v[64][16];
-  uint2 vs[64], vm[64];
+  uint32_t k[128][32];
+  uint32_t v[128][32];
+  uint2 vs[256], vm[256];
 };
 struct __align__(1024) KeyStage {
-  uint32_t k[128][8];
+  uint32_t k[128][32];
 };
-// Scales and minima of the keys of a run of groups: [group][channel pair]
+template <bool WEIGHTS> using StageOf = typename std::conditional<WEIGHTS, KeyStage, Stage>::type;
+// Scales and minima of a tile's keys: [scale, minimum][group][channel]
 struct __align__(16) Scales {
-  uint32_t s[8][64], m[8][64];
+  uint16_t x[2][8][128];
 };
-// words [row][quad * 4 ..] under the swizzles
-__device__ __forceinline__ int quad32(int row, int quad) { return (quad ^ ((row >> 2) & 1)) * 4; }
-__device__ __forceinline__ int quad64(int row, int quad) { return (quad ^ ((row >> 1) & 3)) * 4; }
+// words of 16 bytes `part` of a key, two keys a row, under the swizzle
+__device__ __forceinline__ int quad(int key, int part) { return (((key & 1) * 4 + part) ^ ((key >> 1) & 7)) * 4; }
 constexpr uint32_t WAIT_TRIES = 1u << 22;
 template <bool WEIGHTS> using StageOf = typename std::conditional<WEIGHTS, KeyStage, Stage>::type;
 
 template <bool BF16, bool MASK, int NT, bool WEIGHTS>
-__global__ void __launch_bounds__(THREADS, WEIGHTS ? 2 : 1) few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FewParams a) {
+__global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kernel(const __grid_constant__ CUtensorMap tm_k, const __grid_constant__ CUtensorMap tm_v, const __grid_constant__ FewParams a) {
   using T = typename std::conditional<BF16, __nv_bfloat16, __half>::type;
   const Params& p = a.p;
   constexpr int ROWS = 8 * NT;
   extern __shared__ unsigned char smem_raw[];
-  unsigned char* dyn_s = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);      // stages [warp][2], scales [warp]; at the end
-                                                                                           // results [warp][row][128], [warp][row][2]
-  __shared__ __align__(8) uint64_t bar[WARPS][2];
+  unsigned char* dyn_s = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);      // stages [2], scales [2]; at the end results
+                                                                                           // [warp][row][128], [warp][row][2]
+  __shared__ __align__(8) uint64_t bar[2];
   float* merge_s = reinterpret_cast<float*>(dyn_s);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, g = lane >> 2, c = lane & 3;
   const int hk = blockIdx.x % p.hkv, b = blockIdx.x / p.hkv, part = blockIdx.y;
   const int64_t bh = blockIdx.x;
   pdl_launch_dependents();
   const int live = live_tokens(p), groups = p.t_vis >> 5;
-  // Runs of a.run groups, then full-precision groups (of what is to be written, for weights); all warps of the KV head take them in turn
-  const int runs = (groups + a.run - 1) / a.run;
-  const int units = runs + (int)(((WEIGHTS ? a.capacity : (int64_t)live) + 31) >> 5);
+  const int nv = (groups + 7) >> 3;
+  // tiles: visual ones, then full-precision ones (of what is to be written, for weights)
+  const int tiles = nv + (int)(((WEIGHTS ? a.capacity : (int64_t)live) + 255) >> 8), per = (tiles + (int)gridDim.y - 1) / (int)gridDim.y;
+  const int t0 = min(tiles, part * per), t1 = min(tiles, t0 + per);
   const uint32_t half_sel = g >> 2 ? 0x7632 : 0x5410;
 
   // ---- the queries, as the B operand: channels 2c, 2c+1 (+8) of row g of block nt
@@ -165,65 +166,49 @@ __global__ void __launch_bounds__(THREADS, WEIGHTS ? 2 : 1) few_kernel(const __g
     }
 
   using St = StageOf<WEIGHTS>;
-  St* stages = reinterpret_cast<St*>(dyn_s) + warp * 2;
-  Scales& sc = reinterpret_cast<Scales*>(dyn_s + WARPS * 2 * sizeof(St))[warp];
-  if (lane == 0) {
-    mbar_init(&bar[warp][0], 1);
-    mbar_init(&bar[warp][1], 1);
+  St* stages = reinterpret_cast<St*>(dyn_s);
+  Scales* scales = reinterpret_cast<Scales*>(dyn_s + 2 * sizeof(St));
+  if (tid == 0) {
+    mbar_init(&bar[0], 1);
+    mbar_init(&bar[1], 1);
     mbar_fence_init();
   }
-  __syncwarp();
-  bool ok = true;
-  uint32_t asked = 0, taken = 0;                // pairs of groups so far
-  const auto request = [&](int grp, int n) {    // the n (1 or 2) groups from grp on
-    if (lane == 0) {
-      St& st = stages[asked & 1];
-      uint64_t* full = &bar[warp][asked & 1];
-      mbar_expect_tx(full, sizeof(st.k) + (WEIGHTS ? 0 : 4096 + n * 512));
-      tma_load_2d(st.k, &tm_k, grp * 4, (int)(bh * 128), full);
-      if constexpr (!WEIGHTS) {
-        const int64_t tok = bh * p.t_vis + grp * 32;
-        tma_load_3d(st.v, &tm_v, 0, grp * 32, (int)bh, full);
-        bulk_load_1d(st.vs, static_cast<const char*>(p.v_scale) + tok * 8, n * 256, full);
-        bulk_load_1d(st.vm, static_cast<const char*>(p.v_mn) + tok * 8, n * 256, full);
+  const auto request = [&](int t) {             // codes of visual tile t; one thread
+    if (t >= t1 || t >= nv) return;
+    St& st = stages[(t - t0) & 1];
+    uint64_t* full = &bar[(t - t0) & 1];
+    const int keys = min(256, p.t_vis - t * 256);
+    mbar_expect_tx(full, sizeof(st.k) + (WEIGHTS ? 0 : 16384 + 16 * keys));
+    tma_load_2d(st.k, &tm_k, t * 32, (int)(bh * 128), full);
+    if constexpr (!WEIGHTS) {
+      const int64_t tok = bh * p.t_vis + t * 256;
+      tma_load_3d(st.v, &tm_v, 0, t * 128, (int)bh, full);
+      bulk_load_1d(st.vs, static_cast<const char*>(p.v_scale) + tok * 8, 8 * keys, full);
+      bulk_load_1d(st.vm, static_cast<const char*>(p.v_mn) + tok * 8, 8 * keys, full);
+    }
+  };
+  // Scales (threads 0-127) or minima (128-255) of a channel of visual tile t: one load where the pitch of a channel allows it
+  uint32_t sc[4];
+  const auto fetch_scales = [&](int t) {
+    if (t >= t1 || t >= nv) return;
+    const uint16_t* src = static_cast<const uint16_t*>(tid < 128 ? p.k_scale : p.k_mn) + (bh * 128 + (tid & 127)) * groups + t * 8;
+    if (groups % 8 == 0) {
+      const uint4 v = *reinterpret_cast<const uint4*>(src);
+      sc[0] = v.x; sc[1] = v.y; sc[2] = v.z; sc[3] = v.w;
+    } else {
+      const int n = groups - t * 8;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        sc[i] = 2 * i < n ? src[2 * i] : 0u;
+        if (2 * i + 1 < n) sc[i] |= (uint32_t)src[2 * i + 1] << 16;
       }
     }
-    ++asked;
   };
-  // Scales and minima of the keys of n groups from grp on, for channels 2 lane, 2 lane + 1 (+64): as wide as a run and the pitch of
-  // a channel allow, since every load of a warp touches 32 rows
-  const auto fetch_scales = [&](int grp, int n) {
-    uint32_t x[2][2][2][4];                     // [scale, minimum][lower, upper channels][channel][two groups a word]
+  const auto put_scales = [&](int t) {
+    if (t >= t1 || t >= nv) return;
+    uint16_t* dst = &scales[(t - t0) & 1].x[tid >> 7][0][tid & 127];
 #pragma unroll
-    for (int kind = 0; kind < 2; ++kind)
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const uint16_t* src = static_cast<const uint16_t*>(kind ? p.k_mn : p.k_scale) + (bh * 128 + h * 64 + 2 * lane + e) * groups + grp;
-          uint32_t (&w)[4] = x[kind][h][e];
-          if (a.wide == 8) {
-            const uint4 v = *reinterpret_cast<const uint4*>(src);
-            w[0] = v.x; w[1] = v.y; w[2] = v.z; w[3] = v.w;
-          } else if (a.wide == 4) {
-            const uint2 v = *reinterpret_cast<const uint2*>(src), z = n > 4 ? *reinterpret_cast<const uint2*>(src + 4) : make_uint2(0, 0);
-            w[0] = v.x; w[1] = v.y; w[2] = z.x; w[3] = z.y;
-          } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              w[i] = 2 * i < n ? src[2 * i] : 0u;
-              if (2 * i + 1 < n) w[i] |= (uint32_t)src[2 * i + 1] << 16;
-            }
-          }
-        }
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const uint32_t sel = i & 1 ? 0x7632 : 0x5410;
-        sc.s[i][h * 32 + lane] = prmt(x[0][h][0][i >> 1], x[0][h][1][i >> 1], sel);
-        sc.m[i][h * 32 + lane] = prmt(x[1][h][0][i >> 1], x[1][h][1][i >> 1], sel);
-      }
+    for (int i = 0; i < 8; ++i) dst[i * 128] = (uint16_t)(sc[i >> 1] >> (16 * (i & 1)));
   };
 
   float m_ref[NT][2], l_run[NT][2], o[8][NT][4];      // rows 2c, 2c+1; o: channel block, as the A rows are ordered
@@ -238,38 +223,26 @@ __global__ void __launch_bounds__(THREADS, WEIGHTS ? 2 : 1) few_kernel(const __g
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[i][nt][e] = 0.f;
 
-  for (int u = part * WARPS + warp; u < units; u += WARPS * (int)gridDim.y) {
-   const bool vis = u < runs;
-   const int grp0 = u * a.run, n = vis ? min(a.run, groups - grp0) : 1;      // the unit's groups
-   float minima[NT][4];                         // of group g, rows 2c, 2c + 1
-   __syncwarp();                                // what the unit before left has been read by all lanes
-   if (vis) {
-     request(grp0, min(2, n));
-     fetch_scales(grp0, n);
-     __syncwarp();
-#pragma unroll
-     for (int nt = 0; nt < NT; ++nt)
-#pragma unroll
-       for (int e = 0; e < 4; ++e) minima[nt][e] = 0.f;
-#pragma unroll
-     for (int ks = 0; ks < 8; ++ks) {
-       const uint32_t m0 = sc.m[g][ks * 8 + c], m1 = sc.m[g][ks * 8 + c + 4];
-#pragma unroll
-       for (int nt = 0; nt < NT; ++nt) mma<BF16>(minima[nt], m0, 0u, m1, 0u, q[nt][ks][0], q[nt][ks][1]);
-     }
-   }
-   for (int i = 0; i < n; ++i) {
-    // this group's 32 keys: first one in cache order, how many there are
-    const int key0 = vis ? (grp0 + i) * 32 : p.t_vis + (u - runs) * 32;
-    const int there = vis ? 32 : min(32, live - (key0 - p.t_vis));
-    if (vis && !(i & 1)) {
-      __syncwarp();                             // the other stage has been read by all lanes
-      if (i + 2 < n) request(grp0 + i + 2, min(2, n - i - 2));
-      if (ok) ok = mbar_wait_bounded(&bar[warp][taken & 1], (taken >> 1) & 1, WAIT_TRIES);
-      ++taken;
-    }
-    const St& st = stages[(taken - 1) & 1];
-    const int in = i & 1;                       // which of the stage's two groups
+  __syncthreads();
+  bool ok = true;
+  if (tid == 0) request(t0);
+  fetch_scales(t0);
+  put_scales(t0);
+  fetch_scales(t0 + 1);
+  for (int t = t0; t < t1; ++t) {
+    __syncthreads();                            // the tile before has been read, this one's scales are there
+    if (tid == 0) request(t + 1);
+    put_scales(t + 1);
+    fetch_scales(t + 2);
+    const bool vis = t < nv;
+    // this warp's 32 keys: first one in cache order, how many there are
+    const int key0 = vis ? (t * 8 + warp) * 32 : p.t_vis + ((t - nv) * 8 + warp) * 32;
+    const int there = vis ? min(32, p.t_vis - key0) : min(32, live - (key0 - p.t_vis));
+    const St& st = stages[(t - t0) & 1];
+    const uint32_t (*sc_s)[64] = reinterpret_cast<const uint32_t (*)[64]>(scales[(t - t0) & 1].x);      // [scale or minimum, group][channel pair]
+    if (vis && ok) ok = mbar_wait_bounded(&bar[(t - t0) & 1], ((t - t0) >> 1) & 1, WAIT_TRIES);
+    if (there <= 0 && !(WEIGHTS && !vis && key0 - p.t_vis < a.capacity)) continue;
+
     float mask[2][2];
     bool dead = false;
     if (MASK) {
@@ -290,11 +263,16 @@ __global__ void __launch_bounds__(THREADS, WEIGHTS ? 2 : 1) few_kernel(const __g
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[mb][nt][e] = small[mb][nt][e] = 0.f;
     if (vis) {
+      float minima[NT][4];                      // the same in every row
+#pragma unroll
+      for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) minima[nt][e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) {
-        const uint32_t s2[2] = {sc.s[i][ks * 8 + c], sc.s[i][ks * 8 + c + 4]};
-        const int row = ks * 16 + 2 * c, quad = quad32(row, in) + (g & 3), quad8 = quad32(row + 8, in) + (g & 3);      // rows 2c, 2c + 1 have one swizzle
-        const uint32_t za = prmt(st.k[row][quad], st.k[row + 1][quad], half_sel), zb = prmt(st.k[row + 8][quad8], st.k[row + 9][quad8], half_sel);
+        const uint32_t s2[2] = {sc_s[warp][ks * 8 + c], sc_s[warp][ks * 8 + c + 4]};
+        const int row = ks * 16 + 2 * c, quad = (warp ^ (2 * c)) * 4 + (g & 3), quad1 = quad ^ 4;
+        const uint32_t za = prmt(st.k[row][quad], st.k[row + 1][quad1], half_sel), zb = prmt(st.k[row + 8][quad], st.k[row + 9][quad1], half_sel);
         uint32_t hi[NT][2], lo[NT][2];
 #pragma unroll
         for (int nt = 0; nt < NT; ++nt)
@@ -313,12 +291,15 @@ __global__ void __launch_bounds__(THREADS, WEIGHTS ? 2 : 1) few_kernel(const __g
             mma<BF16>(small[mb][nt], c0, c1, c2, c3, lo[nt][0], lo[nt][1]);
           }
         }
+        const uint32_t m0 = sc_s[8 + warp][ks * 8 + c], m1 = sc_s[8 + warp][ks * 8 + c + 4];
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) mma<BF16>(minima[nt], m0, 0u, m1, 0u, q[nt][ks][0], q[nt][ks][1]);
       }
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float own = __shfl_sync(0xffffffffu, minima[nt][e], i * 4 + c);
+          const float own = minima[nt][e];
 #pragma unroll
           for (int mb = 0; mb < 2; ++mb) {
             s[mb][nt][e] += small[mb][nt][e] + own;
@@ -432,8 +413,8 @@ __global__ void __launch_bounds__(THREADS, WEIGHTS ? 2 : 1) few_kernel(const __g
 #pragma unroll
           for (int e = 0; e < 2; ++e) {
             tok[h][e] = index_of(2 * c + e, 2 * kt + h);
-            vs[h][e] = st.vs[in * 32 + tok[h][e]];
-            vm[h][e] = st.vm[in * 32 + tok[h][e]];
+            vs[h][e] = st.vs[warp * 32 + tok[h][e]];
+            vm[h][e] = st.vm[warp * 32 + tok[h][e]];
             // a key that takes no part: zeros, whatever its values are
             if (MASK && dead && Elem<T>::to_f(static_cast<const T*>(p.mask)[b * p.mask_sb + mask_index(p, key0 + tok[h][e])]) == -INFINITY)
               vs[h][e] = vm[h][e] = make_uint2(0, 0);
@@ -446,7 +427,7 @@ __global__ void __launch_bounds__(THREADS, WEIGHTS ? 2 : 1) few_kernel(const __g
             const uint32_t sel = grp & 1 ? 0x7632 : 0x5410;
             s2[h] = grp < 2 ? prmt(vs[h][0].x, vs[h][1].x, sel) : prmt(vs[h][0].y, vs[h][1].y, sel);
             m2[h] = grp < 2 ? prmt(vm[h][0].x, vm[h][1].x, sel) : prmt(vm[h][0].y, vm[h][1].y, sel);
-            z[h] = prmt(st.v[in * 32 + tok[h][0]][quad64(tok[h][0], grp) + (g & 3)], st.v[in * 32 + tok[h][1]][quad64(tok[h][1], grp) + (g & 3)], half_sel);
+            z[h] = prmt(st.v[warp * 16 + (tok[h][0] >> 1)][quad(tok[h][0], grp) + (g & 3)], st.v[warp * 16 + (tok[h][1] >> 1)][quad(tok[h][1], grp) + (g & 3)], half_sel);
           }
 #pragma unroll
           for (int mb = 0; mb < 2; ++mb) {
@@ -482,7 +463,6 @@ __global__ void __launch_bounds__(THREADS, WEIGHTS ? 2 : 1) few_kernel(const __g
         }
       }
     }
-   }
   }
   if (!__all_sync(0xffffffffu, ok) && lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
   if constexpr (WEIGHTS) return;
@@ -552,10 +532,10 @@ static bool code_map(CUtensorMap* m, const void* base, int64_t words, int64_t ro
 template <bool BF16, bool MASK, int NT, bool WEIGHTS>
 static int run(const FewParams& p, int batch, cudaStream_t st) {
   CUtensorMap tk, tv;
-  if (!code_map(&tk, p.p.k_code, p.p.t_vis / 8, 128 * (int64_t)batch * p.p.hkv, 0, 8, 128, CU_TENSOR_MAP_SWIZZLE_32B) ||
-      !code_map(&tv, p.p.v_code, 16, p.p.t_vis, (int64_t)batch * p.p.hkv, 16, 64, CU_TENSOR_MAP_SWIZZLE_64B))
+  if (!code_map(&tk, p.p.k_code, p.p.t_vis / 8, 128 * (int64_t)batch * p.p.hkv, 0, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
+      !code_map(&tv, p.p.v_code, 32, p.p.t_vis / 2, (int64_t)batch * p.p.hkv, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B))
     return CQ_ERR_LAUNCH;
-  constexpr int stages = 1024 + WARPS * (int)(sizeof(Scales) + 2 * sizeof(StageOf<WEIGHTS>)), results = WEIGHTS ? 0 : 1024 + WARPS * 8 * NT * 130 * (int)sizeof(float);
+  constexpr int stages = 1024 + 2 * (int)(sizeof(Scales) + sizeof(StageOf<WEIGHTS>)), results = WEIGHTS ? 0 : 1024 + WARPS * 8 * NT * 130 * (int)sizeof(float);
   constexpr int smem = stages > results ? stages : results;
   if (smem > 24 * 1024) {
     static bool configured[64] = {};
@@ -572,20 +552,18 @@ static int run(const FewParams& p, int batch, cudaStream_t st) {
 
 }  // namespace few
 
-// CTAs per KV head: two an SM for weights, one for the attention, in whole rounds; a warp's time in groups, and about three more for
-// a CTA.  Then runs as long as a warp's share allows: eight groups, whose scales are loads of 16 bytes; four; or single groups.
-void few_plan(FewParams& f, int64_t heads, int64_t fp_keys, bool weights) {
-  const int64_t slots = (int64_t)sm_count() * (weights ? 2 : 1), groups = f.p.t_vis / 32, all = groups + (fp_keys + 31) / 32;
+// CTAs per KV head: two an SM (one for the attention of more than eight rows), in whole rounds; a CTA costs about a tile of 256 keys beside its own.
+int few_parts(int64_t heads, int64_t t_vis, int64_t fp_keys, bool one) {
+  const int64_t slots = (int64_t)sm_count() * (one ? 1 : 2), tiles = (t_vis + 255) / 256 + (fp_keys + 255) / 256;
   double cost = 1e300;
-  f.parts = 1;
-  for (int s = 1; s <= 64 && s <= (all + few::WARPS - 1) / few::WARPS; ++s) {
-    const int64_t share = (all + (int64_t)s * few::WARPS - 1) / ((int64_t)s * few::WARPS);
-    const double c = (double)((heads * s + slots - 1) / slots) * (share + 3.0) + (s > 1 ? 3.0 : 0.0);
-    if (c < cost) { cost = c; f.parts = s; }
+  int best = 1;
+  for (int s = 1; s <= 64 && s <= tiles; ++s) {
+    const int64_t per = (tiles + s - 1) / s;
+    if ((tiles + per - 1) / per != s) continue;      // leaves a part empty
+    const double c = (double)((heads * s + slots - 1) / slots) * (per + 1.0) + (s > 1 ? 1.0 : 0.0);
+    if (c < cost) { cost = c; best = s; }
   }
-  const int64_t share = (groups + (int64_t)f.parts * few::WARPS - 1) / ((int64_t)f.parts * few::WARPS);
-  f.run = share > 4 ? 8 : share > 2 ? 4 : 1;
-  f.wide = f.run == 8 && groups % 8 == 0 ? 8 : f.run >= 4 && groups % 4 == 0 ? 4 : 1;
+  return best;
 }
 
 int few_run(const FewParams& p, int batch, bool bf16, bool weights, cudaStream_t st) {

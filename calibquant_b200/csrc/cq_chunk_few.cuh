@@ -10,7 +10,7 @@ constexpr int FEW_ROWS = 16;
 
 struct FewParams {
   Params p;
-  int parts, run, wide;                        // CTAs per KV head, groups of a run, groups whose scales one load brings
+  int parts;                                   // CTAs per KV head
   float* part_o;                               // attention, parts > 1: [batch][KV head][row][part][128] and maximum, sum
   float2* part_ml;
   const float *vis_in, *fp_in;                 // weights
@@ -19,7 +19,7 @@ struct FewParams {
   int* status;
 };
 
-void few_plan(FewParams& f, int64_t heads, int64_t fp_keys, bool weights);      // fills parts, run and wide; p.t_vis is set
+int few_parts(int64_t heads, int64_t t_vis, int64_t fp_keys, bool one);
 int few_run(const FewParams& p, int batch, bool bf16, bool weights, cudaStream_t st);
 
 }  // namespace chunk

@@ -378,7 +378,7 @@ extern "C" int cq_key_weights(const cq_chunk_args* a, const float* w_vis_in, con
     f.p = chunk::make_params(a);
     f.vis_in = w_vis_in; f.fp_in = w_fp_in; f.vis = w_vis; f.fp = w_fp; f.capacity = w_capacity;
     f.status = static_cast<int*>(workspace);
-    chunk::few_plan(f, (int64_t)a->batch * a->n_kv_heads, w_capacity, true);
+    f.parts = chunk::few_parts((int64_t)a->batch * a->n_kv_heads, a->t_vis, w_capacity, false);
     return chunk::few_run(f, a->batch, bf16, true, st);
   }
   WeightParams p = {};
