@@ -83,8 +83,6 @@ template <bool WEIGHTS> using StageOf = typename std::conditional<WEIGHTS, KeySt
 struct __align__(16) Scales {
   uint16_t x[2][8][128];
 };
-// words of 16 bytes `part` of a key, two keys a row, under the swizzle
-__device__ __forceinline__ int quad(int key, int part) { return (((key & 1) * 4 + part) ^ ((key >> 1) & 7)) * 4; }
 constexpr uint32_t WAIT_TRIES = 1u << 22;
 template <bool WEIGHTS> using StageOf = typename std::conditional<WEIGHTS, KeyStage, Stage>::type;
 
@@ -108,6 +106,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
   const int tiles = nv + (int)(((WEIGHTS ? a.capacity : (int64_t)live) + 255) >> 8), per = (tiles + (int)gridDim.y - 1) / (int)gridDim.y;
   const int t0 = min(tiles, part * per), t1 = min(tiles, t0 + per);
   const uint32_t half_sel = g >> 2 ? 0x7632 : 0x5410;
+  const int v_row = index_of(2 * c, 0) >> 1, v_base = (warp * 16 + v_row) * 32 + (v_row & 7) * 4 + (g & 3);
 
   // ---- the queries, as the B operand: channels 2c, 2c+1 (+8) of row g of block nt
   uint32_t q[NT][8][2];
@@ -322,19 +321,27 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
           for (int nt = 0; nt < NT; ++nt) mma<BF16>(s[mb][nt], f[2 * mb][0], f[2 * mb + 1][0], f[2 * mb][1], f[2 * mb + 1][1], q[nt][ks][0], q[nt][ks][1]);
       }
     }
-    // natural units, masks
+    // natural units, masks; a visual group is whole
 #pragma unroll
     for (int mb = 0; mb < 2; ++mb)
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const int k = index_of(g, 2 * mb + (e >> 1));
-          float x = s[mb][nt][e] * unit[nt][e & 1];
-          if (MASK) x = mask[mb][e >> 1] == -INFINITY ? -INFINITY : x + mask[mb][e >> 1];
-          if (k >= there || (!vis && key0 - p.t_vis + k >= limit[nt][e & 1])) x = -INFINITY;
-          s[mb][nt][e] = x;
+          s[mb][nt][e] *= unit[nt][e & 1];
+          if (MASK) s[mb][nt][e] = mask[mb][e >> 1] == -INFINITY ? -INFINITY : s[mb][nt][e] + mask[mb][e >> 1];
         }
+    if (!vis) {
+#pragma unroll
+      for (int mb = 0; mb < 2; ++mb)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const int k = index_of(g, 2 * mb + (e >> 1));
+            if (k >= there || key0 - p.t_vis + k >= limit[nt][e & 1]) s[mb][nt][e] = -INFINITY;
+          }
+    }
 
     if constexpr (WEIGHTS) {
       float w[4] = {};                          // key index_of(g, j), over this lane's rows, then the other lanes'
@@ -404,6 +411,11 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
     // ---- values
     if (vis) {
      if constexpr (!WEIGHTS) {
+      // Where the words of key index_of(2c, 0) are, for each of the eight values that the swizzle's exclusive or may take: those of key
+      // index_of(2c + e, 2 kt + h) and channel group grp are 4 e + kt rows on, under (h ^ e) * 4 + (grp ^ kt)
+      const uint32_t* at[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) at[i] = &st.v[0][0] + (v_base ^ (i * 4));
 #pragma unroll
       for (int kt = 0; kt < 2; ++kt) {
         uint2 vs[2][2], vm[2][2];               // scales and minima of keys 2c, 2c+1 of both halves, all four groups of channels
@@ -427,7 +439,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
             const uint32_t sel = grp & 1 ? 0x7632 : 0x5410;
             s2[h] = grp < 2 ? prmt(vs[h][0].x, vs[h][1].x, sel) : prmt(vs[h][0].y, vs[h][1].y, sel);
             m2[h] = grp < 2 ? prmt(vm[h][0].x, vm[h][1].x, sel) : prmt(vm[h][0].y, vm[h][1].y, sel);
-            z[h] = prmt(st.v[warp * 16 + (tok[h][0] >> 1)][quad(tok[h][0], grp) + (g & 3)], st.v[warp * 16 + (tok[h][1] >> 1)][quad(tok[h][1], grp) + (g & 3)], half_sel);
+            z[h] = prmt(at[h * 4 + (grp ^ kt)][kt * 32], at[(h ^ 1) * 4 + (grp ^ kt)][kt * 32 + 128], half_sel);
           }
 #pragma unroll
           for (int mb = 0; mb < 2; ++mb) {
