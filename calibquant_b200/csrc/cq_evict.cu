@@ -2,9 +2,9 @@
 // the `keep` with the largest weight stay, in their order, and move to a smaller cache unchanged.
 //
 // Selection: the weights become integers whose order is the weights' order (the bits of the number, all of them flipped for a negative one, the
-// sign bit for any other; -0 as +0, NaN above infinity), and the value of the keep-th largest is found eight bits at a time from a histogram of
-// the units that agree with it so far.  A unit stays if it is above that value, or equal to it and among the first of the equal
-// ones that fill the rest.  A group's weight is the sum of its 32 weights in 64 bits, so that the order of the additions decides
+// sign bit for any other; -0 as +0, NaN above infinity).  Up to a thread's number of units are ranked by counting those above; of more, the
+// value of the keep-th largest is found eight bits at a time from a histogram of the units that agree with it so far, until all that
+// agree stay.  A unit stays if it is above that value, or equal to it and among the first of the equal ones that fill the rest.  A group's weight is the sum of its 32 weights in 64 bits, so that the order of the additions decides
 // no border.  Only counts are added atomically: the result depends on nothing but the weights.
 // One launch: every CTA of a (batch row, KV head) finds the selection itself and moves its share of the cache.
 #include "cq_common.cuh"
@@ -55,10 +55,25 @@ __device__ __forceinline__ int2 block_prefix(int x, int* total, int (*scan)[2], 
   return make_int2(before + inc - x, all);
 }
 
-// list[0 .. keep-1] = the units with the keep largest keys of key[0 .. n-1], ascending; all threads.  `list` may be the memory of `key`
-// only if it lies behind it.
+// list[0 .. keep-1] = the units with the keep largest keys of key[0 .. n-1], ascending; all threads.
 template <typename Key>
 __device__ __forceinline__ void select(const Key* key, int n, int keep, int* list, Shared& s) {
+  if (n <= THREADS) {
+    const int i = threadIdx.x;
+    bool stays = false;
+    if (i < n) {
+      const Key own = key[i];
+      int above = 0;
+#pragma unroll 8
+      for (int j = 0; j < n; ++j) above += key[j] > own || (key[j] == own && j < i);
+      stays = above < keep;
+    }
+    int total;
+    const int at = block_prefix(stays, &total, s.scan, 0).x;
+    if (stays) list[at] = i;
+    __syncthreads();
+    return;
+  }
   Key prefix = 0, mask = 0;
   int rest = keep;                               // how many of the units that agree with the prefix stay
   for (int shift = 8 * (int)sizeof(Key) - 8; shift >= 0; shift -= 8) {
@@ -90,31 +105,39 @@ __device__ __forceinline__ void select(const Key* key, int n, int keep, int* lis
     prefix |= (Key)s.digit << shift;
     mask |= (Key)(BINS - 1) << shift;
     rest -= s.above;
+    const bool whole = s.hist[s.digit] == rest;      // all that agree so far stay
     __syncthreads();
+    if (whole) break;
   }
   // each thread a run of consecutive units, so that the places are ascending
   const int run = (n + THREADS - 1) / THREADS, i0 = min(n, (int)threadIdx.x * run), i1 = min(n, i0 + run);
   int above = 0, equal = 0;
   for (int i = i0; i < i1; ++i) {
-    above += key[i] > prefix;
-    equal += key[i] == prefix;
+    above += (key[i] & mask) > prefix;
+    equal += (key[i] & mask) == prefix;
   }
   int total;
   int ties = block_prefix(equal, &total, s.scan, 0).x;
   int place = block_prefix(above, &total, s.scan, 1).x + min(ties, rest);
   for (int i = i0; i < i1; ++i) {
-    if (key[i] > prefix) list[place++] = i;
-    else if (key[i] == prefix && ties++ < rest) list[place++] = i;
+    const Key k = key[i] & mask;
+    if (k > prefix) list[place++] = i;
+    else if (k == prefix && ties++ < rest) list[place++] = i;
   }
   __syncthreads();
 }
 
+template <int WORDS> struct Codes;      // of a channel and group
+template <> struct Codes<1> { using T = uint32_t; };
+template <> struct Codes<2> { using T = uint2; };
+template <> struct Codes<4> { using T = uint4; };
+
 struct Groups {
-  const uint32_t* k_code; const uint16_t *k_scale, *k_mn;
-  const uint4* v_code; const uint2 *v_scale, *v_mn;
+  const void* k_code; const uint16_t *k_scale, *k_mn;
+  const uint4* v_code; const uint4 *v_scale, *v_mn;
   const float4* weights;
-  uint32_t* k_code_out; uint16_t *k_scale_out, *k_mn_out;
-  uint4* v_code_out; uint2 *v_scale_out, *v_mn_out;
+  void* k_code_out; uint16_t *k_scale_out, *k_mn_out;
+  uint4* v_code_out; uint4 *v_scale_out, *v_mn_out;
   float4* w_out;
   int64_t* kept;
   int groups, keep;
@@ -123,40 +146,71 @@ struct Groups {
 // WORDS (= bits) 32-bit words of codes per channel and group
 template <int WORDS>
 __global__ void __launch_bounds__(THREADS) groups_kernel(Groups p) {
+  using C = typename Codes<WORDS>::T;
   extern __shared__ uint64_t key[];
   __shared__ Shared s;
   int* list = reinterpret_cast<int*>(key + p.groups);
   const int64_t bh = blockIdx.y;
-  const float4* w = p.weights + bh * p.groups * 8;
-  for (int g = threadIdx.x; g < p.groups; g += THREADS) {
+  const int keep = p.keep, groups = p.groups, lane = threadIdx.x & 31;
+  const float4* w = p.weights + bh * groups * 8;
+  for (int g = threadIdx.x; g < groups; g += THREADS) {
+    float4 v[8];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) v[i] = w[(int64_t)g * 8 + i];
     double sum = 0.0;
-    for (int i = 0; i < 8; ++i) {
-      const float4 v = w[(int64_t)g * 8 + i];
-      sum += v.x; sum += v.y; sum += v.z; sum += v.w;
-    }
+#pragma unroll
+    for (int i = 0; i < 8; ++i) { sum += v[i].x; sum += v[i].y; sum += v[i].z; sum += v[i].w; }
     key[g] = ordered(sum);
   }
   __syncthreads();
-  select(key, p.groups, p.keep, list, s);
-  const int64_t tid = (int64_t)blockIdx.x * THREADS + threadIdx.x, all = (int64_t)gridDim.x * THREADS, keep = p.keep;
-  // keys: a row of words, scales and minima per channel
-  for (int64_t i = tid; i < 128 * keep; i += all) {
-    const int64_t row = bh * 128 + i / keep;
-    const int j = (int)(i % keep), g = list[j];
-    for (int c = 0; c < WORDS; ++c) p.k_code_out[(row * keep + j) * WORDS + c] = p.k_code[(row * p.groups + g) * WORDS + c];
-    p.k_scale_out[row * keep + j] = p.k_scale[row * p.groups + g];
-    p.k_mn_out[row * keep + j] = p.k_mn[row * p.groups + g];
+  select(key, groups, keep, list, s);
+  // A warp takes a channel of the keys (32 groups at a time, side by side in the result) or the values and weights of a group
+  const int warps = (int)gridDim.x * (THREADS / 32);
+  for (int item = (int)blockIdx.x * (THREADS / 32) + ((int)threadIdx.x >> 5); item < 128 + keep; item += warps) {
+    if (item < 128) {
+      const int64_t from = (bh * 128 + item) * groups, to = (bh * 128 + item) * keep;
+      const C* src = static_cast<const C*>(p.k_code) + from;
+      C* dst = static_cast<C*>(p.k_code_out) + to;
+      for (int j0 = 0; j0 < keep; j0 += 128) {
+        C c[4];
+        uint16_t sc[4], mn[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int j = j0 + u * 32 + lane;
+          if (j < keep) {
+            const int g = list[j];
+            c[u] = src[g];
+            sc[u] = p.k_scale[from + g];
+            mn[u] = p.k_mn[from + g];
+          }
+        }
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+          const int j = j0 + u * 32 + lane;
+          if (j < keep) {
+            dst[j] = c[u];
+            p.k_scale_out[to + j] = sc[u];
+            p.k_mn_out[to + j] = mn[u];
+          }
+        }
+      }
+    } else {
+      const int j = item - 128, g = list[j];
+      const int64_t from = bh * groups + g, to = bh * keep + j;
+      uint4 c[WORDS];
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) c[i] = p.v_code[from * 32 * WORDS + i * 32 + lane];      // 32 tokens of WORDS 16-byte pieces
+      const uint4 sm = lane < 16 ? p.v_scale[from * 16 + lane] : p.v_mn[from * 16 + lane - 16];
+      float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (lane < 8) x = w[(int64_t)g * 8 + lane];
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) p.v_code_out[to * 32 * WORDS + i * 32 + lane] = c[i];
+      if (lane < 16) p.v_scale_out[to * 16 + lane] = sm;
+      else p.v_mn_out[to * 16 + lane - 16] = sm;
+      if (lane < 8) p.w_out[to * 8 + lane] = x;
+      if (lane == 0) p.kept[to] = g;
+    }
   }
-  // values and weights: what belongs to a group lies together
-  for (int64_t i = tid; i < keep * 32 * WORDS; i += all)
-    p.v_code_out[bh * keep * 32 * WORDS + i] = p.v_code[(bh * p.groups + list[i / (32 * WORDS)]) * 32 * WORDS + i % (32 * WORDS)];
-  for (int64_t i = tid; i < keep * 32; i += all) {
-    const int64_t from = (bh * p.groups + list[i / 32]) * 32 + i % 32, to = bh * keep * 32 + i;
-    p.v_scale_out[to] = p.v_scale[from];
-    p.v_mn_out[to] = p.v_mn[from];
-  }
-  for (int64_t i = tid; i < keep * 8; i += all) p.w_out[bh * keep * 8 + i] = w[(int64_t)list[i / 8] * 8 + i % 8];
-  for (int64_t i = tid; i < keep; i += all) p.kept[bh * keep + i] = list[i];
 }
 
 struct Tokens {
@@ -181,19 +235,35 @@ __global__ void __launch_bounds__(THREADS) tokens_kernel(Tokens p) {
   for (int t = threadIdx.x; t < n; t += THREADS) key32[t] = ordered(w[p.t_sys + t]);
   __syncthreads();
   if (m > 0) select(key32, n, m, list, s);
-  const int64_t base = (bh / p.heads) * p.sb + (bh % p.heads) * p.sh;
-  const int64_t tid = (int64_t)blockIdx.x * THREADS + threadIdx.x, all = (int64_t)gridDim.x * THREADS, keep = p.keep;
-  const auto source = [&](int64_t j) -> int64_t {
-    return j < p.t_sys ? j : j < p.t_sys + m ? p.t_sys + list[j - p.t_sys] : p.t_fp - (keep - j);
-  };
-  for (int64_t i = tid; i < keep * 16; i += all) {
-    const int64_t from = base + source(i / 16) * 16 + i % 16, to = bh * keep * 16 + i;
-    p.k_out[to] = p.k[from];
-    p.v_out[to] = p.v[from];
-  }
-  for (int64_t j = tid; j < keep; j += all) {
-    p.w_out[bh * keep + j] = w[source(j)];
-    p.kept[bh * keep + j] = source(j);
+  const uint4 *k = p.k + (bh / p.heads) * p.sb + (bh % p.heads) * p.sh, *v = p.v + (bh / p.heads) * p.sb + (bh % p.heads) * p.sh;
+  const int64_t out = bh * p.keep;
+  const auto source = [&](int j) { return j < p.t_sys ? j : j < p.t_sys + m ? p.t_sys + list[j - p.t_sys] : p.t_fp - (p.keep - j); };
+  // half a warp takes a token's row, four of them at a time
+  const int half = ((int)blockIdx.x * THREADS + (int)threadIdx.x) >> 4, halves = (int)gridDim.x * (THREADS / 16), c = threadIdx.x & 15;
+  for (int j0 = half; j0 < p.keep; j0 += 4 * halves) {
+    uint4 kx[4], vx[4];
+    int t[4];
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = j0 + u * halves;
+      if (j < p.keep) {
+        t[u] = source(j);
+        kx[u] = k[(int64_t)t[u] * 16 + c];
+        vx[u] = v[(int64_t)t[u] * 16 + c];
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < 4; ++u) {
+      const int j = j0 + u * halves;
+      if (j < p.keep) {
+        p.k_out[(out + j) * 16 + c] = kx[u];
+        p.v_out[(out + j) * 16 + c] = vx[u];
+        if (c == 0) {
+          p.w_out[out + j] = w[t[u]];
+          p.kept[out + j] = t[u];
+        }
+      }
+    }
   }
 }
 
@@ -233,11 +303,10 @@ extern "C" int cq_evict_groups(const int32_t* k_code, const void* k_scale, const
       (int64_t)batch * heads > 65535)
     return CQ_ERR_UNSUPPORTED;
   if (batch == 0) return CQ_OK;
-  evict::Groups p = {reinterpret_cast<const uint32_t*>(k_code), static_cast<const uint16_t*>(k_scale), static_cast<const uint16_t*>(k_mn),
-                     reinterpret_cast<const uint4*>(v_code), static_cast<const uint2*>(v_scale), static_cast<const uint2*>(v_mn),
-                     reinterpret_cast<const float4*>(weights), reinterpret_cast<uint32_t*>(k_code_out), static_cast<uint16_t*>(k_scale_out),
-                     static_cast<uint16_t*>(k_mn_out), reinterpret_cast<uint4*>(v_code_out), static_cast<uint2*>(v_scale_out),
-                     static_cast<uint2*>(v_mn_out), reinterpret_cast<float4*>(w_out), kept, groups, keep};
+  evict::Groups p = {k_code, static_cast<const uint16_t*>(k_scale), static_cast<const uint16_t*>(k_mn), reinterpret_cast<const uint4*>(v_code),
+                     static_cast<const uint4*>(v_scale), static_cast<const uint4*>(v_mn), reinterpret_cast<const float4*>(weights), k_code_out,
+                     static_cast<uint16_t*>(k_scale_out), static_cast<uint16_t*>(k_mn_out), reinterpret_cast<uint4*>(v_code_out),
+                     static_cast<uint4*>(v_scale_out), static_cast<uint4*>(v_mn_out), reinterpret_cast<float4*>(w_out), kept, groups, keep};
   const int64_t rows = (int64_t)batch * heads;
   const dim3 grid(evict::slices(rows, (int64_t)keep * 32 * (32 * bits + 32)), (unsigned)rows);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
