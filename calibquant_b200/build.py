@@ -73,7 +73,7 @@ def _bind_command():
            os.path.join(cuda, "include"), sysconfig.get_paths()["include"]]
     return ["g++", "-O2", "-std=c++17", "-shared", "-fPIC", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
             *[f"-I{i}" for i in inc], BIND_SRC, "-o", NATIVE_PATH, f"-L{os.path.join(root, 'lib')}", "-lc10", "-lc10_cuda",
-            "-ltorch_cpu", "-ltorch_python", f"-L{PKG_DIR}", "-l:libcalibquant_b200.so", "-Wl,-rpath,$ORIGIN"]
+            "-ltorch_cpu", "-ltorch_cuda", "-ltorch_python", f"-L{PKG_DIR}", "-l:libcalibquant_b200.so", "-Wl,-rpath,$ORIGIN"]
 
 
 def build_library(force: bool = False, verbose: bool = False, extra=()) -> str:

@@ -6,6 +6,7 @@
 // through c10.  No arithmetic lives here: every function checks its arguments, allocates its results and calls one
 // entry point of libcalibquant_b200.so on torch's current stream.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <c10/cuda/CUDAException.h>
@@ -139,6 +140,8 @@ struct Call {            // device and stream of one call
 
 Tensor empty(at::IntArrayRef size, const Tensor& like) { return at::empty(size, like.options()); }
 Tensor empty(at::IntArrayRef size, const Tensor& like, at::ScalarType dt) { return at::empty(size, like.options().dtype(dt)); }
+// The same from the device's allocator without the dispatcher, for calls with many results
+Tensor fresh(at::IntArrayRef size, const Tensor& like, at::ScalarType dt) { return at::detail::empty_cuda(size, dt, like.device(), c10::nullopt); }
 
 PyObject* wrap(Tensor t) { return THPVariable_Wrap(std::move(t)); }
 PyObject* wrap2(Tensor a, Tensor b) {
@@ -884,14 +887,14 @@ PyObject* py_chunk_attention(PyObject*, PyObject* const* a, Py_ssize_t n) {
     want_size(out, c.q.sizes(), c.q.scalar_type(), c.q, "out");
     if (!rows_ok(out)) raise(PyExc_ValueError, "out must have contiguous channels, strides that are multiples of 8 and a 16-byte aligned start");
   } else {
-    out = empty(c.q.sizes(), c.q);
+    out = fresh(c.q.sizes(), c.q, c.q.scalar_type());
   }
   d.out = out.data_ptr();
   for (int i = 0; i < 3; ++i) d.out_strides[i] = out.stride(i);
   const bool want_lse = truth(a[12]);
   Tensor lse;
   if (want_lse) {
-    lse = empty({d.batch, d.n_q_heads, d.q_len}, c.q, at::kFloat);
+    lse = fresh({d.batch, d.n_q_heads, d.q_len}, c.q, at::kFloat);
     d.lse = lse.data_ptr<float>();
   }
   if (out.numel()) {
@@ -946,8 +949,8 @@ PyObject* py_key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (!t.is_contiguous()) raise(PyExc_ValueError, "out must be contiguous");
     if (given && out[1].size(2) != in[1].size(2)) raise(PyExc_ValueError, "weights and out must have the same shapes");
   } else {
-    out[0] = empty({d.batch, d.n_kv_heads, d.t_vis}, c.q, at::kFloat);
-    out[1] = empty({d.batch, d.n_kv_heads, given ? in[1].size(2) : d.t_fp}, c.q, at::kFloat);
+    out[0] = fresh({d.batch, d.n_kv_heads, d.t_vis}, c.q, at::kFloat);
+    out[1] = fresh({d.batch, d.n_kv_heads, given ? in[1].size(2) : d.t_fp}, c.q, at::kFloat);
   }
   if (d.batch > 0) {
     const size_t nbytes = cq_key_weights_workspace_bytes(&d, out[1].size(2));
@@ -991,13 +994,13 @@ PyObject* py_evict_groups(PyObject*, PyObject* const* a, Py_ssize_t n) {
   want_pack(vp, B, H, 32 * G, bits, false, like, "v_pack");
   want_size(tensor(a[2]), {B, H, 32 * G}, at::kFloat, like, "weights");
   const Tensor w = packed_rows(tensor(a[2]));
-  ko[0] = empty({B, H, D, keep * bits}, like, at::kInt);
-  vo[0] = empty({B, H, 32 * keep, 4 * bits}, like, at::kInt);
+  ko[0] = fresh({B, H, D, keep * bits}, like, at::kInt);
+  vo[0] = fresh({B, H, 32 * keep, 4 * bits}, like, at::kInt);
   for (int i : {1, 2}) {
-    ko[i] = empty({B, H, D, keep}, like);
-    vo[i] = empty({B, H, 32 * keep, 4}, like);
+    ko[i] = fresh({B, H, D, keep}, like, like.scalar_type());
+    vo[i] = fresh({B, H, 32 * keep, 4}, like, like.scalar_type());
   }
-  const Tensor wo = empty({B, H, 32 * keep}, like, at::kFloat), kept = empty({B, H, keep}, like, at::kLong);
+  const Tensor wo = fresh({B, H, 32 * keep}, like, at::kFloat), kept = fresh({B, H, keep}, like, at::kLong);
   if (B * H)
     launch([&] { return cq_evict_groups((const int32_t*)kp[0].data_ptr(), kp[1].data_ptr(), kp[2].data_ptr(), (const int32_t*)vp[0].data_ptr(), vp[1].data_ptr(),
                            vp[2].data_ptr(), w.data_ptr<float>(), (int)B, (int)H, (int)D, (int)(32 * G), (int)keep, (int)bits, (int)group,
@@ -1030,8 +1033,8 @@ PyObject* py_evict_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
   want_size(w, {B, H, w.size(2)}, at::kFloat, c.k_fp, "weights");
   if (w.size(2) < t_fp) raise(PyExc_ValueError, "the weights must cover t_fp tokens");
   w = contiguous(w);
-  const Tensor ko = empty({B, H, keep, D}, c.k_fp), vo = empty({B, H, keep, D}, c.k_fp);
-  const Tensor wo = empty({B, H, keep}, c.k_fp, at::kFloat), kept = empty({B, H, keep}, c.k_fp, at::kLong);
+  const Tensor ko = fresh({B, H, keep, D}, c.k_fp, c.k_fp.scalar_type()), vo = fresh({B, H, keep, D}, c.k_fp, c.k_fp.scalar_type());
+  const Tensor wo = fresh({B, H, keep}, c.k_fp, at::kFloat), kept = fresh({B, H, keep}, c.k_fp, at::kLong);
   if (B * H)
     launch([&] { return cq_evict_tokens(c.k_fp.data_ptr(), c.v_fp.data_ptr(), c.k_fp.stride(0), c.k_fp.stride(1), w.data_ptr<float>(), w.size(2), (int)B, (int)H,
                            (int)D, (int)t_fp, (int)keep, (int)sys, (int)recent, ko.data_ptr(), vo.data_ptr(), wo.data_ptr<float>(),

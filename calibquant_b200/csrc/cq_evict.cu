@@ -267,10 +267,11 @@ __global__ void __launch_bounds__(THREADS) tokens_kernel(Tokens p) {
   }
 }
 
-// CTAs per (batch row, KV head): four per SM in all, at least 16 KB to move for each
+// CTAs per (batch row, KV head): as many as PER_SM an SM hold at once, at least 16 KB to move for each
+constexpr int PER_SM = 2;
 static int slices(int64_t rows, int64_t bytes) {
-  const int64_t fill = (4 * sm_count() + rows - 1) / rows, work = (bytes + 16383) / 16384;
-  return (int)(fill < work ? (fill > 0 ? fill : 1) : (work > 0 ? work : 1));
+  const int64_t fill = PER_SM * sm_count() / rows, work = (bytes + 16383) / 16384, n = fill < work ? fill : work;
+  return (int)(n > 0 ? n : 1);
 }
 
 template <typename... K, typename... A>
