@@ -101,9 +101,8 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
   const int64_t bh = blockIdx.x;
   pdl_launch_dependents();
   const int live = live_tokens(p), groups = p.t_vis >> 5;
-  const int nv = (groups + 7) >> 3;
-  // tiles: visual ones, then full-precision ones (of what is to be written, for weights)
-  const int tiles = nv + (int)(((WEIGHTS ? a.capacity : (int64_t)live) + 255) >> 8), per = (tiles + (int)gridDim.y - 1) / (int)gridDim.y;
+  // tiles: full-precision ones first (of what is to be written, for weights), under which the codes of the first visual one come in
+  const int nf = (int)(((WEIGHTS ? a.capacity : (int64_t)live) + 255) >> 8), tiles = nf + ((groups + 7) >> 3), per = (tiles + (int)gridDim.y - 1) / (int)gridDim.y;
   const int t0 = min(tiles, part * per), t1 = min(tiles, t0 + per);
   const uint32_t half_sel = g >> 2 ? 0x7632 : 0x5410;
   const int v_row = index_of(2 * c, 0) >> 1, v_base = (warp * 16 + v_row) * 32 + (v_row & 7) * 4 + (g & 3);
@@ -172,30 +171,31 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
     mbar_init(&bar[1], 1);
     mbar_fence_init();
   }
-  const auto request = [&](int t) {             // codes of visual tile t; one thread
-    if (t >= t1 || t >= nv) return;
+  const auto request = [&](int t) {             // codes of tile t; one thread
+    if (t >= t1 || t < nf) return;
+    const int first = (t - nf) * 256;
     St& st = stages[(t - t0) & 1];
     uint64_t* full = &bar[(t - t0) & 1];
-    const int keys = min(256, p.t_vis - t * 256);
+    const int keys = min(256, p.t_vis - first);
     mbar_expect_tx(full, sizeof(st.k) + (WEIGHTS ? 0 : 16384 + 16 * keys));
-    tma_load_2d(st.k, &tm_k, t * 32, (int)(bh * 128), full);
+    tma_load_2d(st.k, &tm_k, first / 8, (int)(bh * 128), full);
     if constexpr (!WEIGHTS) {
-      const int64_t tok = bh * p.t_vis + t * 256;
-      tma_load_3d(st.v, &tm_v, 0, t * 128, (int)bh, full);
+      const int64_t tok = bh * p.t_vis + first;
+      tma_load_3d(st.v, &tm_v, 0, first / 2, (int)bh, full);
       bulk_load_1d(st.vs, static_cast<const char*>(p.v_scale) + tok * 8, 8 * keys, full);
       bulk_load_1d(st.vm, static_cast<const char*>(p.v_mn) + tok * 8, 8 * keys, full);
     }
   };
-  // Scales (threads 0-127) or minima (128-255) of a channel of visual tile t: one load where the pitch of a channel allows it
+  // Scales (threads 0-127) or minima (128-255) of a channel of tile t: one load where the pitch of a channel allows it
   uint32_t sc[4];
   const auto fetch_scales = [&](int t) {
-    if (t >= t1 || t >= nv) return;
-    const uint16_t* src = static_cast<const uint16_t*>(tid < 128 ? p.k_scale : p.k_mn) + (bh * 128 + (tid & 127)) * groups + t * 8;
+    if (t >= t1 || t < nf) return;
+    const uint16_t* src = static_cast<const uint16_t*>(tid < 128 ? p.k_scale : p.k_mn) + (bh * 128 + (tid & 127)) * groups + (t - nf) * 8;
     if (groups % 8 == 0) {
       const uint4 v = *reinterpret_cast<const uint4*>(src);
       sc[0] = v.x; sc[1] = v.y; sc[2] = v.z; sc[3] = v.w;
     } else {
-      const int n = groups - t * 8;
+      const int n = groups - (t - nf) * 8;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
         sc[i] = 2 * i < n ? src[2 * i] : 0u;
@@ -204,7 +204,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
     }
   };
   const auto put_scales = [&](int t) {
-    if (t >= t1 || t >= nv) return;
+    if (t >= t1 || t < nf) return;
     uint16_t* dst = &scales[(t - t0) & 1].x[tid >> 7][0][tid & 127];
 #pragma unroll
     for (int i = 0; i < 8; ++i) dst[i * 128] = (uint16_t)(sc[i >> 1] >> (16 * (i & 1)));
@@ -233,13 +233,16 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
     if (tid == 0) request(t + 1);
     put_scales(t + 1);
     fetch_scales(t + 2);
-    const bool vis = t < nv;
+    const bool vis = t >= nf;
     // this warp's 32 keys: first one in cache order, how many there are
-    const int key0 = vis ? (t * 8 + warp) * 32 : p.t_vis + ((t - nv) * 8 + warp) * 32;
+    const int key0 = vis ? ((t - nf) * 8 + warp) * 32 : p.t_vis + (t * 8 + warp) * 32;
     const int there = vis ? min(32, p.t_vis - key0) : min(32, live - (key0 - p.t_vis));
     const St& st = stages[(t - t0) & 1];
     const uint32_t (*sc_s)[64] = reinterpret_cast<const uint32_t (*)[64]>(scales[(t - t0) & 1].x);      // [scale or minimum, group][channel pair]
-    if (vis && ok) ok = mbar_wait_bounded(&bar[(t - t0) & 1], ((t - t0) >> 1) & 1, WAIT_TRIES);
+    if (vis && ok) {
+      const int use = (t - max(t0, nf)) >> 1;    // visual tiles that came through this stage before
+      ok = mbar_wait_bounded(&bar[(t - t0) & 1], use & 1, WAIT_TRIES);
+    }
     if (there <= 0 && !(WEIGHTS && !vis && key0 - p.t_vis < a.capacity)) continue;
 
     float mask[2][2];
