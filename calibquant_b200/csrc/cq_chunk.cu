@@ -73,7 +73,13 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   return r;
 }
-__device__ __forceinline__ void tile_barrier(int id) { asm volatile("bar.sync %0, 128;" ::"r"(id) : "memory"); }
+// barrier among the four softmax warps of a tile that also tells whether any thread passed `flag`
+__device__ __forceinline__ bool tile_any(int id, bool flag) {
+  uint32_t out;
+  asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 q, %1, 0;\n\tbar.red.or.pred p, %2, 128, q;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+               : "=r"(out) : "r"((uint32_t)flag), "r"(id) : "memory");
+  return out != 0;
+}
 
 // Key tiles of a CTA: visual tiles [0, nv), full-precision ones [nv, n_all); this CTA's are [t0, t0 + n).
 struct Range {
@@ -103,7 +109,10 @@ __device__ __forceinline__ void fill_fp_tile(const Params& p, const void* base, 
     for (int it = 0; it < 4; ++it) {
       const int t = t_first + (half * 4 + it) * 16 + (ptid >> 4);
       v[it] = make_uint4(0, 0, 0, 0);
-      if (t < live && (!values || takes_part<BF16, MASK>(p, b, p.t_vis + t))) v[it] = *reinterpret_cast<const uint4*>(src + (int64_t)t * 128 + (ptid & 15) * 8);
+      if (t < live) {
+        v[it] = *reinterpret_cast<const uint4*>(src + (int64_t)t * 128 + (ptid & 15) * 8);
+        if (values && !takes_part<BF16, MASK>(p, b, p.t_vis + t)) v[it] = make_uint4(0, 0, 0, 0);
+      }
       if (values) order_values(v[it]);
     }
 #pragma unroll
@@ -232,6 +241,7 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
     clear_q(ptid, 256);
 
     Unit ku[2], vu[2];                        // requested: the warp's two units
+    bool taken[2] = {true, true};
     const auto request_k = [&](int j) {
       const int tile = k.t0 + j;
       if (j < k.n && tile < k.nv) {
@@ -245,7 +255,8 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
 #pragma unroll
         for (int u = 0; u < 2; ++u) {
           const int key = tile * 128 + (pw + 8 * u) * 8 + (lane >> 2);
-          load_v_unit(p, bh, tile, pw + 8 * u, lane, key < p.t_vis && takes_part<BF16, MASK>(p, b, key), vu[u]);
+          load_v_unit(p, bh, tile, pw + 8 * u, lane, true, vu[u]);
+          if (MASK) taken[u] = key < p.t_vis && takes_part<BF16, MASK>(p, b, key);      // looked at when the unit is stored
         }
       }
     };
@@ -283,6 +294,9 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
         wait_free(&bar_vfree[buf], PAIR ? j : j >> 1);
         if (!ok) break;
         if (tile < k.nv) {
+#pragma unroll
+          for (int u = 0; u < 2; ++u)
+            if (MASK && !taken[u]) { vu[u].w = make_uint4(0, 0, 0, 0); vu[u].scale = vu[u].mn = 0; }
           store_v_unit<BF16>(dst, vu[0], pw, lane);
           store_v_unit<BF16>(dst, vu[1], pw + 8, lane);
         } else {
@@ -451,8 +465,8 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
     const bool valid_row = r_in < a.tile_rows && i < p.q_len;
     const int limit = live - p.q_len + i + 1;                     // full-precision tokens that the row sees
     const int n_x = PAIR ? k.n : (k.n + 1 - x) >> 1;
-    // Units: without a mask, scores as the tensor core gives them times `factor` are powers of two; with one they are scaled and
-    // masked first (a mask of the type's lowest value times log2 e would leave fp32's range).
+    // Units of the reference: without a mask, scores as the tensor core gives them; with one they are scaled and masked first (a mask of
+    // the type's lowest value times log2 e would leave fp32's range).  `factor` makes powers of two of either.
     const float factor = MASK ? LOG2E : a.scale * LOG2E;
     bool ok = true;
     float m_ref = -INFINITY, l_run = 0.f;
@@ -462,21 +476,23 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
       if (j >= n_x || (tile < k.nv ? key >= p.t_vis : key - p.t_vis >= live)) return Elem<T>::from_f(-INFINITY);
       return static_cast<const T*>(p.mask)[b * p.mask_sb + mask_index(p, key)];
     };
+    const auto lim_tile = [&](int tile) { return tile < k.nv ? p.t_vis - tile * 128 : live - (tile - k.nv) * 128; };      // keys that are there
     T mask_next = MASK ? mask_of(0) : Elem<T>::from_f(0.f);
     for (int j = 0; j < n_x; ++j) {
       const int tile = k.t0 + (PAIR ? j : 2 * j + x);
       const int lim = min(128, tile < k.nv ? p.t_vis - tile * 128 : limit - (tile - k.nv) * 128);      // columns from lim on are not seen
       const T* mk = mask_s[MASK ? x : 0][MASK ? j & 1 : 0];
+      bool masked = false;                    // some mask of the tile is not zero; most tiles of a padded request have none
       if (MASK) {
         mask_s[x][j & 1][r_in] = mask_next;
+        masked = tile_any(1 + x, Elem<T>::to_f(mask_next) != 0.f && r_in < lim_tile(tile));
         mask_next = mask_of(j + 1);
-        tile_barrier(1 + x);
       }
       const bool need = __any_sync(0xffffffffu, lim < 128);
       if (ok) ok = mbar_wait_cycles(&bar_s[x], j & 1, WAIT_CYCLES);
       tc_fence_after();
       const auto shown = [&](int cc, uint32_t (&s)[32]) {          // 32 scores with the mask
-        if (MASK) {
+        if (MASK && masked) {
 #pragma unroll
           for (int c = 0; c < 32; c += 4) {
             const uint2 m4 = *reinterpret_cast<const uint2*>(mk + cc * 32 + c);
@@ -513,7 +529,7 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
           for (int c = 0; c < 32; c += 2) mx4[(c >> 1) & 3] = max3(mx4[(c >> 1) & 3], __uint_as_float(v[c]), __uint_as_float(v[c + 1]));
         }
       }
-      const float m_true = fmaxf(m_ref, fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])));
+      const float top = fmaxf(fmaxf(mx4[0], mx4[1]), fmaxf(mx4[2], mx4[3])), m_true = fmaxf(m_ref, MASK && !masked ? top * a.scale : top);
       // a row keeps its reference until the true maximum is 2^8 above it (probabilities stay below 256), or for the first time
       const bool grow = (m_true - m_ref) * factor > 8.f;
       if (j > 0 && __any_sync(0xffffffffu, grow)) {
@@ -547,11 +563,11 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
 #pragma unroll
           for (int c = 0; c < 32; c += 2) {
             float e0 = __uint_as_float(v[c]), e1 = __uint_as_float(v[c + 1]);
-            if (MASK) {
+            if (MASK && masked) {
               e0 = (e0 - m_use) * factor;
               e1 = (e1 - m_use) * factor;
             } else {
-              fma_pair(e0, e1, e0, e1, factor, factor, neg, neg);
+              fma_pair(e0, e1, e0, e1, a.scale * LOG2E, a.scale * LOG2E, neg, neg);
             }
             e0 = ex2_approx(e0);
             e1 = ex2_approx(e1);
