@@ -277,6 +277,8 @@ class GraphedDecoder:
         self.out = torch.zeros((max_new_tokens + 2, B), device=dev, dtype=torch.long)
         self.step_idx = torch.zeros(1, device=dev, dtype=torch.long)
         state0 = (self.tok.clone(), self.caches[0].length)
+        tracked = [layer.attention for layer in lm.model.layers if getattr(layer.attention, "_track_weights", False)]
+        weights0 = [None if a._key_weights is None else tuple(t.clone() for t in a._key_weights) for a in tracked]
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())
         with torch.cuda.stream(side):                       # warm-up outside capture, then roll back
@@ -285,6 +287,11 @@ class GraphedDecoder:
         torch.cuda.current_stream().wait_stream(side)
         torch.cuda.synchronize()
         self._reset(state0, start_pos)
+        for a, w0 in zip(tracked, weights0):                # the warm-up's tokens were not real ones
+            for i, t in enumerate(a._key_weights):
+                t.zero_()
+                if w0 is not None:
+                    t[..., :w0[i].shape[-1]] = w0[i]
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph, stream=side):     # the warm-up's stream: its scratch buffers are reused
             self._step()

@@ -15,7 +15,10 @@ What changes underneath:
 * a decode step is ONE call (``ops.decode_attention``) covering scores with post-scaling, logit
   calibration, softmax, packed attn.V and the fp16 system/text segments -- no ``repeat_kv`` copies,
   no transposes, no per-step ``torch.cat`` of the text cache (it lives in a pre-allocated buffer);
-* prefill attention is ``ops.prefill_attention`` (causal over the whole sequence, no chunk loop).
+* prefill attention is ``ops.prefill_attention`` (causal over the whole sequence, no chunk loop);
+* several tokens on a cache that exists already (a second question to the same picture; the reference takes one prompt and
+  then single tokens) are ONE call (``ops.chunk_attention``) where the visual span is held at 4 bits;
+* ``track_key_weights`` has every call add up how much attention each cached key gets, ``evict_cache`` drops what got least.
 """
 
 from __future__ import annotations
@@ -239,6 +242,104 @@ def _pop_padding_mask(kwargs, attention_mask):
     return attention_mask
 
 
+def _chunk_cache(self):
+    """Packed keys and values of this layer for the calls that take several tokens, or an error where they do not serve them."""
+    if getattr(self, "_u8_state", None) is not None:
+        raise NotImplementedError("several tokens on a cache, or tracked weights: the group format only, not uint8")
+    if self.k_pack is None or self.k_pack[0].numel() == 0:
+        return None, None
+    if BITS_KV != 4:
+        raise NotImplementedError(f"several tokens on a cache, or tracked weights: a visual span of 4 bits, not {BITS_KV}")
+    return self.k_pack, self.v_pack
+
+
+def _attend_tracked(self, q, t_fp, mask=None, t_fp_dev=None):
+    """Attention of the last tokens of the cache, q [B,L,Hq,D], whose weights are added up in ``self._key_weights``."""
+    k_pack, v_pack = _chunk_cache(self)
+    tc, t_sys = self._text_cache, self.sprompt_len if LOW_BITS else 0
+    attn, lse = ops.chunk_attention(q, k_pack, v_pack, tc.k, tc.v, t_sys, mask=mask, t_fp=t_fp, t_fp_dev=t_fp_dev, return_lse=True)
+    B, H, capacity = tc.k.shape[:3]
+    w = getattr(self, "_key_weights", None)
+    if w is None or w[1].shape[2] < capacity:
+        full = torch.zeros((B, H, capacity), dtype=torch.float32, device=q.device)
+        if w is not None:
+            full[:, :, :w[1].shape[2]] = w[1]
+        vis = w[0] if w is not None else torch.zeros((B, H, 0 if k_pack is None else v_pack[0].shape[2]), dtype=torch.float32, device=q.device)
+        self.__dict__["_key_weights"] = w = (vis, full)
+    ops.key_weights(q, lse, k_pack, tc.k, t_sys, mask=mask, weights=w, out=w, t_fp=t_fp, t_fp_dev=t_fp_dev)
+    return attn
+
+
+def _forward_chunk(self, hidden_states, attention_mask, position_ids, past_key_value, use_cache):
+    """Several new tokens on the cache of this layer."""
+    k_pack, v_pack = _chunk_cache(self)
+    bsz, q_len, _ = hidden_states.size()
+    n_rep, tc = self.num_key_value_groups, self._text_cache
+    n_kv = self.wqkv.out_features // ((n_rep + 2) * self.head_dim)
+    kv_seq_len = q_len + past_key_value[0].shape[-2] + (self.image_token_num if LOW_BITS else 0) + self._evicted
+    mask = None
+    if attention_mask is not None:
+        if getattr(self, "_keys_differ", False):
+            raise ValueError("heads keep different tokens after an eviction: a mask over keys has no place any more")
+        if attention_mask.size() != (bsz, 1, q_len, kv_seq_len):
+            raise ValueError(f"Attention mask should be of size {(bsz, 1, q_len, kv_seq_len)}, but is {attention_mask.size()}")
+        mask = attention_mask[:, 0, -1]
+    cos, sin = self.rotary_emb(hidden_states, seq_len=kv_seq_len)
+    if position_ids is None:
+        position_ids = torch.arange(kv_seq_len - q_len, kv_seq_len, device=hidden_states.device).expand(bsz, q_len)
+    tc.reserve(q_len)
+    q, _, _ = ops.prefill_rope_split(self.wqkv(hidden_states), cos, sin, position_ids, n_kv, n_rep, tc.k[:, :, tc.length:], tc.v[:, :, tc.length:])
+    tc.length += q_len
+    if getattr(self, "_track_weights", False):
+        attn = _attend_tracked(self, q, tc.length, mask=mask)
+    else:
+        attn = ops.chunk_attention(q, k_pack, v_pack, tc.k, tc.v, self.sprompt_len if LOW_BITS else 0, mask=mask, t_fp=tc.length)
+    attn = _gather_heads(self, attn.reshape(bsz, q_len, -1))
+    return self.wo(attn), None, tc.views() if use_cache else None
+
+
+def _attentions(model):
+    lm = getattr(model, "language_model", model)
+    return [layer.attention for layer in lm.model.layers]
+
+
+def track_key_weights(model, on: bool = True):
+    """Have every attention layer of the patched model add up, per KV head, how much attention each cached key gets: from the question of
+    the next prompt on (its tokens behind the visual span), over chunks and single tokens.  4-bit group format.  What
+    has been added up is in ``attention._key_weights`` (visual, full-precision); ``evict_cache`` uses it."""
+    for attn in _attentions(model):
+        attn._track_weights = bool(on)
+        attn._key_weights = None
+
+
+def evict_cache(model, keep_groups=None, keep_tokens=None, recent=32):
+    """Drop from the cache of every layer and KV head what ``track_key_weights`` saw the least attention on: all but ``keep_groups`` groups of 32
+    visual tokens and / or all but ``keep_tokens`` full-precision tokens, of which the system prompt's and the last
+    ``recent`` always stay.  Positions are those of the tokens as they were.  Returns the layers' new ``past_key_values``."""
+    past = []
+    for attn in _attentions(model):
+        tc, w = attn._text_cache, getattr(attn, "_key_weights", None)
+        if w is None:
+            raise ValueError("no key weights: track_key_weights has to be on while the cache is used")
+        if getattr(attn, "_static_decode", False):
+            raise ValueError("the cache of a captured decoder stays where it is: close the decoder first")
+        w_vis, w_fp = w
+        if keep_groups is not None and attn.k_pack is not None:
+            attn.k_pack, attn.v_pack, w_vis, _ = ops.evict_groups(attn.k_pack, attn.v_pack, w_vis, keep_groups, bits=BITS_KV)
+            attn._keys_differ = True
+        if keep_tokens is not None:
+            t_sys = attn.sprompt_len if LOW_BITS else 0
+            k, v, kept_w, _ = ops.evict_tokens(tc.k, tc.v, w_fp, keep_tokens, t_sys=t_sys, recent=recent, t_fp=tc.length)
+            attn._evicted += tc.length - keep_tokens
+            attn._keys_differ = True
+            attn._text_cache = tc = _TextCache(k, v)
+            w_fp = torch.zeros((*tc.k.shape[:3],), dtype=torch.float32, device=k.device)
+            w_fp[:, :, :keep_tokens] = kept_w
+        attn._key_weights = (w_vis, w_fp)
+        past.append(tc.views())
+    return past
+
+
 def forward_internlm2_calibquant(self, hidden_states: torch.Tensor,
                                  attention_mask: Optional[torch.LongTensor] = None,
                                  position_ids: Optional[torch.LongTensor] = None,
@@ -246,6 +347,9 @@ def forward_internlm2_calibquant(self, hidden_states: torch.Tensor,
                                  output_attentions: bool = False, use_cache: bool = False, **kwargs):
     """Patched ``InternLM2FlashAttention2.forward`` (``patch_internvl.py:141-484``).
 
+    Several tokens on an existing cache (q_len > 1, ``past_key_value`` given): RoPE, append to the fp cache, one attention call
+    over [system | quantized visual | text] that is causal among the new tokens; at 4 bits, without logit calibration.  Of an
+    ``attention_mask`` [B,1,q_len,keys] the last row, which no causality narrows, says which keys count.
     Prefill (q_len > 1): RoPE, quantize the visual span ``[SPROMPT_LEN, SPROMPT_LEN+IMAGE_TOKEN_NUM)``
     of K (per channel) and V (per token) at ``BITS_KV`` bits, keep system+text K/V in fp, run causal
     attention over the unquantized K/V.  Decode (q_len == 1): one fused attention call over
@@ -273,7 +377,9 @@ def forward_internlm2_calibquant(self, hidden_states: torch.Tensor,
         q = ops.rope_split_append(self.wqkv(hidden_states), cos, sin, position_ids,
                                   self.wqkv.out_features // ((n_rep + 2) * self.head_dim), n_rep,
                                   tc.k, tc.v, t_fp_dev=tc.len_dev)
-        if getattr(self, "_u8_state", None) is not None:
+        if getattr(self, "_track_weights", False):
+            attn = _attend_tracked(self, q.transpose(1, 2), tc.k.shape[2], t_fp_dev=tc.len_dev).transpose(1, 2)
+        elif getattr(self, "_u8_state", None) is not None:
             from . import calibquant as _cq
             attn = _cq.decode_attention(q, self._u8_state, tc.k, tc.v, BITS_KV, self.sprompt_len,
                                         normalize=self.normalize, t_fp_dev=tc.len_dev).to(q.dtype)
@@ -289,7 +395,7 @@ def forward_internlm2_calibquant(self, hidden_states: torch.Tensor,
         # of the fp cache; the pack kernels then read the visual span of the rotated keys and (in
         # place, through strides) of the values; the dense attention reads the same buffers.
         if past_key_value is not None:
-            raise NotImplementedError("chunked prefill on top of an existing cache is not supported")
+            return _forward_chunk(self, hidden_states, attention_mask, position_ids, past_key_value, use_cache)
         n_rep = self.num_key_value_groups
         n_kv = self.wqkv.out_features // ((n_rep + 2) * self.head_dim)
         s0, n_vis = (self.sprompt_len, self.image_token_num) if LOW_BITS else (0, 0)
@@ -313,8 +419,11 @@ def forward_internlm2_calibquant(self, hidden_states: torch.Tensor,
             self.k_pack = ops.pack_k_per_channel(k.transpose(1, 2)[:, :, s0:s0 + n_vis], GROUP_SIZE, BITS_KV)
             self.v_pack = ops.pack_v_per_token(v.transpose(1, 2)[:, :, s0:s0 + n_vis], GROUP_SIZE, BITS_KV)
         self._text_cache = tc
+        state["_key_weights"], state["_evicted"], state["_keys_differ"] = None, 0, False      # _evicted: full-precision tokens
         past_key_value = tc.views() if use_cache else None
         attn = ops.prefill_attention(q, k, v)
+        if getattr(self, "_track_weights", False) and q_len > s0 + n_vis:
+            _attend_tracked(self, q[:, s0 + n_vis:], tc.length)      # the question's own look at the cache
         attn = _gather_heads(self, attn.reshape(bsz, q_len, -1))
         attn_output = self.wo(attn.reshape(bsz, q_len, -1))
         return attn_output, None, past_key_value
@@ -322,8 +431,10 @@ def forward_internlm2_calibquant(self, hidden_states: torch.Tensor,
     # ---- decode step -------------------------------------------------------------------------
     kv_seq_len = q_len
     if past_key_value is not None:
-        kv_seq_len += past_key_value[0].shape[-2] + (self.image_token_num if LOW_BITS else 0)
+        kv_seq_len += past_key_value[0].shape[-2] + (self.image_token_num if LOW_BITS else 0) + getattr(self, "_evicted", 0)
     tc = self._text_cache
+    if attention_mask is not None and getattr(self, "_keys_differ", False):
+        raise ValueError("heads keep different tokens after an eviction: a mask over keys has no place any more")
     cos, sin = self.rotary_emb(hidden_states, seq_len=kv_seq_len)
     if self.head_dim == 128 and cos.dtype == sin.dtype == hidden_states.dtype == tc.k.dtype:
         # one launch splits the projection, rotates q and k and appends k, v to the text cache (the torch ops
@@ -348,7 +459,9 @@ def forward_internlm2_calibquant(self, hidden_states: torch.Tensor,
         raise ValueError(f"Attention mask should be of size {(bsz, 1, q_len, kv_seq_len)}, "
                          f"but is {attention_mask.size()}")
     t_sys = self.sprompt_len if LOW_BITS else 0
-    if getattr(self, "_u8_state", None) is not None:
+    if getattr(self, "_track_weights", False):
+        attn = _attend_tracked(self, q.transpose(1, 2), tc.length, mask=attention_mask).transpose(1, 2)
+    elif getattr(self, "_u8_state", None) is not None:
         from . import calibquant as _cq
         k_fp, v_fp = past_key_value or tc.views()
         attn = _cq.decode_attention(q, self._u8_state, k_fp, v_fp, BITS_KV, t_sys, normalize=self.normalize,
@@ -361,7 +474,7 @@ def forward_internlm2_calibquant(self, hidden_states: torch.Tensor,
     if attn.shape != (bsz, local_heads, q_len, self.head_dim):
         raise ValueError(f"`attn_output` should be of size {(bsz, local_heads, q_len, self.head_dim)}, "
                          f"but is {attn.size()}")
-    attn = _gather_heads(self, attn.view(bsz, q_len, -1))
+    attn = _gather_heads(self, attn.reshape(bsz, q_len, -1))
     wo = self.wo
     w = _plain_weight(wo, attn) if bsz <= 4 else None
     return wo(attn) if w is None else ops.linear_small(attn, w), None, past_key_value

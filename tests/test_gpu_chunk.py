@@ -175,6 +175,88 @@ def test_agrees_with_the_decode_step():
     assert err < 1e-2
 
 
+@pytest.mark.parametrize("L,B", [(1, 2), (9, 1), (40, 2), (300, 1)])
+def test_captured_and_replayed(L, B):
+    """Both calls in a CUDA graph whose inputs and live count change between replays, beside eager calls on another stream."""
+    from calibquant_b200 import ops
+    q, kp, vp, k_fp, v_fp = make(B, 8, 2, L, 160, 100, BF16, seed=L, cap=500)
+    counter = torch.tensor([100 + L], dtype=torch.int32, device="cuda")
+    acc = (torch.zeros(B, 2, 160, device="cuda"), torch.zeros(B, 2, 500, device="cuda"))
+
+    def both():
+        out, lse = ops.chunk_attention(q, kp, vp, k_fp, v_fp, 41, t_fp_dev=counter, return_lse=True)
+        ops.key_weights(q, lse, kp, k_fp, 41, weights=acc, out=acc, t_fp_dev=counter)
+        return out, lse
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        both()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=side):
+        out, lse = both()
+    for step, live in enumerate((100 + L, 300, 450)):
+        counter.fill_(live)
+        q.copy_(torch.randn(q.shape, generator=torch.Generator().manual_seed(step)))
+        for t in acc:
+            t.zero_()
+        graph.replay()
+        with torch.cuda.stream(side):
+            side.wait_stream(torch.cuda.current_stream())
+            again = both()
+            again_acc = [t.clone() for t in acc]
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
+        assert all(torch.equal(2 * t, u) for t, u in zip(ops.key_weights(q, lse, kp, k_fp, 41, t_fp_dev=counter), again_acc))
+        want, want_l, room, room_l = ref.attention64(q, kp, vp, k_fp, v_fp, 41, live=live)
+        assert ref.within(out, want, room) and ref.within(lse, want_l, room_l)
+
+
+def test_two_streams_at_once():
+    """Calls that overlap on two streams have workspaces of their own; results do not depend on when they run."""
+    from calibquant_b200 import ops
+    cases = [make(4, 8, 2, L, 1312, 100, HALF, seed=L) for L in (1, 60, 700)]
+    want = [ops.chunk_attention(q, kp, vp, k, v, 41, return_lse=True) for q, kp, vp, k, v in cases]
+    want_w = [ops.key_weights(c[0], w[1], c[1], c[3], 41) for c, w in zip(cases, want)]
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+    for rep in range(4):
+        for s in streams:
+            with torch.cuda.stream(s):
+                for (q, kp, vp, k, v), w in zip(cases, want):
+                    got.append((ops.chunk_attention(q, kp, vp, k, v, 41, return_lse=True), ops.key_weights(q, w[1], kp, k, 41)))
+    torch.cuda.synchronize()
+    for i, (o, w) in enumerate(got):
+        assert torch.equal(o[0], want[i % 3][0]) and torch.equal(o[1], want[i % 3][1])
+        assert all(torch.equal(a, b) for a, b in zip(w, want_w[i % 3]))
+
+
+@pytest.mark.parametrize("L", [2, 70, 260])
+def test_offsets_past_32_bits(L):
+    """The second request's full-precision tokens lie more than 2^31 elements behind the first one's."""
+    from calibquant_b200 import ops
+    q, kp, vp, k_fp, v_fp = make(2, 4, 1, L, 64, 40, BF16, seed=L)
+    n, far = k_fp.shape[2], 2 ** 31 + 2 ** 20
+    views = []
+    for t in (k_fp, v_fp):
+        big = torch.empty(far + n * 128, dtype=BF16, device="cuda").as_strided((2, 1, n, 128), (far, n * 128, 128, 1))
+        views.append(big.copy_(t))
+    a, la = ops.chunk_attention(q, kp, vp, *views, 41, return_lse=True)
+    b, lb = ops.chunk_attention(q, kp, vp, k_fp, v_fp, 41, return_lse=True)
+    assert torch.equal(a, b) and torch.equal(la, lb)
+    assert all(torch.equal(x, y) for x, y in zip(ops.key_weights(q, la, kp, views[0], 41), ops.key_weights(q, lb, kp, k_fp, 41)))
+
+
+def test_many_small_requests():
+    """More (request, head) pairs than a launch has SMs, one key each."""
+    q, kp, vp, k_fp, v_fp = make(70, 8, 8, 1, 0, 0, HALF, seed=4)
+    check(q, kp, vp, k_fp, v_fp, 0)
+    q, kp, vp, k_fp, v_fp = make(40, 16, 4, 2, 32, 1, BF16, seed=4)
+    check(q, kp, vp, k_fp, v_fp, 1)
+
+
 def test_empty_batch():
     from calibquant_b200 import ops
     q, k = torch.empty(0, 3, 8, 128, dtype=HALF, device="cuda"), torch.empty(0, 2, 9, 128, dtype=HALF, device="cuda")
