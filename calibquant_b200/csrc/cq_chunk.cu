@@ -13,6 +13,16 @@
 //   warp 16          issues the products
 // S = Q K^T with packed keys as two 16-bit terms (their sum is scale * code + minimum exactly), so scores carry no rounding but
 // that of fp32 sums; O += P V with P in tensor memory.  S_A [0,128) S_B [128,256) O_A [256,384) O_B [384,512) TMEM columns.
+// Key tiles that three or more row blocks would unpack are unpacked once, by chunk_unpack_kernel, into images of the shared-memory tiles (96 KB per
+// 128 visual tokens), which the attention then loads in bulk.
+//
+// What bounds it.  With images: 48 products of 64 cycles a key tile and pair of query tiles, 3072 cycles; measured 4100 (8 x 1024 queries on
+// 3328 + 1280 keys, bfloat16, at 1.75 GHz under the power cap: 588 us, and 52 for the images at 4.5 TB/s).  What is above is the chain of one query tile
+// (S -> softmax, 1900 cycles -> P V -> next S) that the other one does not cover.  Without images: the issue slots that unpacking
+// (39 instructions per word of eight keys, twice rounded) and softmax share, about 9000 cycles a tile; with images for one row block
+// too, 37 queries of four requests on 6656 tokens took 101 us instead of 67.
+// Taken for granted by neither: a slot or tile as an index instead of a constant costs the issuing lane 104 cycles a product (917 -> 1036 us
+// when the slot became a switch, 676 with constants); a ring of five slots held up the keys (980 -> 945).
 // Every wait is bounded; one that runs out sets CQ_ERR_TIMEOUT in the workspace's first word, and the CTA ends.
 #include <math.h>
 

@@ -8,6 +8,11 @@
 //   warp 16     issues the products
 //   warp 17     has TMA bring the query blocks into two slots
 // A block is the query heads of the KV head for as many queries as NB rows hold: a row of a block is the same head for every block.
+// Bound: 64 products of 64 cycles per pair of packed key tiles and 256 rows, whose operands take all of shared memory's bandwidth
+// (8 KB a product); the query blocks that TMA writes and the log-sum-exps that the sums read come on top: 82 cycles a product measured.
+// The 2 x 128 x 128 exponentials of a block take as long as its products (2048 cycles) and run beside them.  8 x 1024 queries on 3328
+// + 1280 keys, bfloat16: 411 us when cool, 460 in a row of launches, of which 12 % are the CTAs' starts (key tiles, first block).
+// Without the exponentials 478 against 488, without reading the log-sum-exps 470, with half the products 411 (one run).
 // TMEM: tile X's scores in columns X * 256 + buffer * 128.  Where the key tiles are fewer than the SMs, the rows are cut into parts whose
 // sums finish_kernel adds in their order.
 #include <cuda.h>
