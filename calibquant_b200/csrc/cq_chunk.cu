@@ -16,7 +16,7 @@
 // Key tiles that three or more row blocks would unpack are unpacked once, by chunk_unpack_kernel, into images of the shared-memory tiles (96 KB per
 // 128 visual tokens), which the attention then loads in bulk.
 //
-// What bounds it.  With images: 48 products of 64 cycles a key tile and pair of query tiles, 3072 cycles; measured 4100 (8 x 1024 queries on
+// What bounds it.  With images: 48 products of 64 cycles a key tile and pair of query tiles; measured 4100 cycles (8 x 1024 queries on
 // 3328 + 1280 keys, bfloat16, at 1.75 GHz under the power cap: 588 us, and 52 for the images at 4.5 TB/s).  What is above is the chain of one query tile
 // (S -> softmax, 1900 cycles -> P V -> next S) that the other one does not cover.  Without images: the issue slots that unpacking
 // (39 instructions per word of eight keys, twice rounded) and softmax share, about 9000 cycles a tile; with images for one row block

@@ -26,7 +26,7 @@ def chunk_args(p, **changes):
     a.bits, a.group_size, a.dtype = 4, 32, _lib.CQ_DTYPE_BF16
     for name in ("q", "k_code", "k_scale", "k_mn", "v_code", "v_scale", "v_mn", "k_fp", "v_fp", "out", "lse"):
         setattr(a, name, p)
-    a.q_strides = a.out_strides = (ctypes.c_int64 * 3)(3 * 1024, 1024, 128)
+    a.q_strides = a.out_strides = (ctypes.c_int64 * 3)(4096, 1024, 128)
     a.fp_stride_b, a.fp_stride_h = 2 * 1280, 1280
     for name, value in changes.items():
         setattr(a, name, (ctypes.c_int64 * 3)(*value) if name.endswith("strides") else value)
@@ -34,8 +34,8 @@ def chunk_args(p, **changes):
 
 
 BAD = [dict(batch=-1), dict(n_q_heads=7), dict(n_kv_heads=0), dict(q_len=0), dict(q_len=11), dict(t_vis=-32), dict(t_sys=11), dict(reserved=1), dict(dtype=2),
-       dict(q=None), dict(k_fp=None), dict(k_scale=None), dict(fp_stride_h=1284), dict(q_strides=(3072, 1024, 127)), dict(q_strides=(3072, 0, 128)),
-       dict(q_strides=(3072, -1024, 128)), dict(q_strides=(3072, 1024, 0))]
+       dict(q=None), dict(k_fp=None), dict(k_scale=None), dict(fp_stride_h=1284), dict(q_strides=(4096, 1024, 127)), dict(q_strides=(4096, 0, 128)),
+       dict(q_strides=(4096, -1024, 128)), dict(q_strides=(4096, 1024, 0))]
 UNSUPPORTED = [dict(head_dim=64), dict(group_size=64), dict(bits=2), dict(bits=8), dict(t_vis=65), dict(n_q_heads=258, n_kv_heads=2)]
 
 
@@ -58,7 +58,7 @@ def test_unsupported(lib, p16, changes):
 
 def test_each_call_on_its_own(lib, p16):
     ref = lambda **c: ctypes.byref(chunk_args(p16, **c))
-    for c in (dict(out=None), dict(v_fp=None), dict(v_code=None), dict(out=p16 + 2), dict(out_strides=(3072, 1024, 4))):
+    for c in (dict(out=None), dict(v_fp=None), dict(v_code=None), dict(out=p16 + 2), dict(out_strides=(4096, 1024, 4))):
         assert lib.cq_chunk_attn(ref(**c), p16, 1 << 30, None) == _lib.CQ_ERR_BAD_ARG
     assert lib.cq_chunk_attn(None, p16, 1 << 30, None) == _lib.CQ_ERR_BAD_ARG
     need = lib.cq_chunk_attn_workspace_bytes(ref())
