@@ -243,9 +243,15 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
     const int there = vis ? min(32, p.t_vis - key0) : min(32, live - (key0 - p.t_vis));
     const St& st = stages[(t - t0) & 1];
     const uint32_t (*sc_s)[64] = reinterpret_cast<const uint32_t (*)[64]>(scales[(t - t0) & 1].x);      // [scale or minimum, group][channel pair]
-    if (vis && ok) {
+    if (vis) {                                  // after a time-out too, so that no copy is under way when the block ends
       const int use = (t - max(t0, nf)) >> 1;    // visual tiles that came through this stage before
-      ok = mbar_wait_bounded(&bar[(t - t0) & 1], use & 1, WAIT_TRIES);
+      if (!mbar_wait_bounded(&bar[(t - t0) & 1], use & 1, ok ? WAIT_TRIES : 1024u)) {
+        ok = false;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) lse[nt][e] = l_run[nt][e] = NAN;      // and so are the results
+      }
     }
     if (there <= 0 && !(WEIGHTS && !vis && key0 - p.t_vis < a.capacity)) continue;
 
@@ -513,19 +519,20 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
     for (int w = 0; w < WARPS; ++w) m = fmaxf(m, ml_s[(w * ROWS + r) * 2]);
     for (int w = 0; w < WARPS; ++w) {
       const float mw = ml_s[(w * ROWS + r) * 2];
-      if (mw == -INFINITY) continue;
+      const float lw = ml_s[(w * ROWS + r) * 2 + 1];
+      if (mw == -INFINITY && lw == lw) continue;
       const float f = ex2_approx((mw - m) * LOG2E);
       const float4 v = *reinterpret_cast<const float4*>(merge_s + (w * ROWS + r) * 128 + lane * 4);
-      l = fmaf(ml_s[(w * ROWS + r) * 2 + 1], f, l);
+      l = fmaf(lw, f, l);
       x[0] = fmaf(v.x, f, x[0]); x[1] = fmaf(v.y, f, x[1]); x[2] = fmaf(v.z, f, x[2]); x[3] = fmaf(v.w, f, x[3]);
     }
     const int i = r / p.n_rep;
     const int64_t h = hk * p.n_rep + r - i * p.n_rep;
     if (gridDim.y == 1) {
-      const float inv = l > 0.f ? 1.f / l : 0.f;
+      const float inv = l != l ? l : l > 0.f ? 1.f / l : 0.f;
       T* dst = static_cast<T*>(p.out) + b * p.o_sb + i * p.o_st + h * p.o_sh + lane * 4;
       *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<BF16>(x[0] * inv, x[1] * inv), pack16<BF16>(x[2] * inv, x[3] * inv));
-      if (p.lse && lane == 0) p.lse[(b * (int64_t)p.hq + h) * p.q_len + i] = l > 0.f ? m + logf(l) : -INFINITY;
+      if (p.lse && lane == 0) p.lse[(b * (int64_t)p.hq + h) * p.q_len + i] = l != l ? l : l > 0.f ? m + logf(l) : -INFINITY;
     } else {
       const int64_t at = (bh * p.rows + r) * a.parts + part;
       *reinterpret_cast<float4*>(a.part_o + at * 128 + lane * 4) = make_float4(x[0], x[1], x[2], x[3]);
