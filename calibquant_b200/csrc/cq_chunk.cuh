@@ -41,6 +41,7 @@ inline bool valid(const cq_chunk_args* a) {
     if (a->q_strides[i] % 8 || a->q_strides[i] < 0) return false;
   if ((a->q_strides[0] == 0 && a->batch > 1) || (a->q_strides[1] == 0 && a->q_len > 1) || (a->q_strides[2] == 0 && a->n_q_heads > 1)) return false;
   if (a->mask && reinterpret_cast<uintptr_t>(a->mask) % 2) return false;
+  if (reinterpret_cast<uintptr_t>(a->lse) % 4 || reinterpret_cast<uintptr_t>(a->t_fp_dev) % 4) return false;
   if (a->t_vis && (!a->k_code || !a->k_scale || !a->k_mn || !aligned16(a->k_code) || !aligned16(a->k_scale) || !aligned16(a->k_mn))) return false;
   return true;
 }

@@ -327,7 +327,8 @@ extern "C" int cq_evict_tokens(const void* k, const void* v, int64_t stride_b, i
     return CQ_ERR_BAD_ARG;
   for (const void* q : {k, v, (const void*)k_out, (const void*)v_out})
     if (!q || !aligned16(q)) return CQ_ERR_BAD_ARG;
-  if (!weights || !w_out || !kept) return CQ_ERR_BAD_ARG;
+  if (!weights || !w_out || !kept || reinterpret_cast<uintptr_t>(weights) % 4 || reinterpret_cast<uintptr_t>(w_out) % 4 || reinterpret_cast<uintptr_t>(kept) % 8)
+    return CQ_ERR_BAD_ARG;
   const size_t smem = (size_t)t_fp * 4 + (size_t)(keep - t_sys - recent) * 4;
   if (head_dim != kHeadDim || t_fp > evict::MAX_TOKENS || (int64_t)batch * heads > 65535)
     return CQ_ERR_UNSUPPORTED;

@@ -372,6 +372,8 @@ extern "C" int cq_key_weights(const cq_chunk_args* a, const float* w_vis_in, con
                               int64_t w_capacity, void* workspace, size_t workspace_bytes, void* stream) {
   using namespace chunk::kw;
   if (!chunk::valid(a) || !a->lse || (a->t_vis && !w_vis) || !w_fp || w_capacity < a->t_fp) return CQ_ERR_BAD_ARG;
+  for (const float* w : {w_vis_in, w_fp_in, (const float*)w_vis, (const float*)w_fp})
+    if (reinterpret_cast<uintptr_t>(w) % 4) return CQ_ERR_BAD_ARG;
   if (!weights_supported(a, w_capacity)) return CQ_ERR_UNSUPPORTED;
   const Plan pl = make_plan(a, w_capacity);
   cudaStream_t st = static_cast<cudaStream_t>(stream);

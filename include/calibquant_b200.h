@@ -511,7 +511,7 @@ int cq_qjl_gqa_score(const uint8_t* key_quant, const uint8_t* key_outlier_quant,
  *           zero where the extent is above one)
  *   lse     fp32 [B,Hq,q_len], or NULL
  * bits == 4, group_size == 32, head_dim == 128, t_vis a multiple of 32 (0: no packed operands), 0 < q_len <= t_fp, every
- * pointer 16-byte aligned (mask 2-byte), up to 128 query heads per KV head.
+ * pointer 16-byte aligned (mask 2-byte, lse, t_fp_dev and weights 4-byte), up to 128 query heads per KV head.
  * The first word of the workspace is a sticky status word as in cq_decode_attn; two calls that overlap on the GPU need two workspaces.
  */
 typedef struct cq_chunk_args {
@@ -565,7 +565,8 @@ int cq_key_weights(const cq_chunk_args* args, const float* w_vis_in, const float
  * cq_evict_tokens: the same for single full-precision tokens: of t_fp tokens the first t_sys and the last `recent` stay whatever
  * their weight, and those with the largest weights fill up to `keep`.
  *   k, v     token (b,h,t,:) at base + b*stride_b + h*stride_h + t*128; weights fp32, row (b,h) at weights + (b*H + h)*w_stride
- *   k_out, v_out [B,H,keep,128], w_out [B,H,keep], kept int64 [B,H,keep].  t_fp <= 24576.
+ *   k_out, v_out [B,H,keep,128], w_out [B,H,keep], kept int64 [B,H,keep].  t_fp <= 24576.  k, v and what becomes of them 16-byte
+ *   aligned, weights 4-byte, kept 8-byte.
  */
 int cq_evict_groups(const int32_t* k_code, const void* k_scale, const void* k_mn, const int32_t* v_code, const void* v_scale,
                     const void* v_mn, const float* weights, int batch, int heads, int head_dim, int t_vis, int keep, int bits,

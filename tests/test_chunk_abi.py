@@ -90,3 +90,20 @@ def test_evictions(lib, p16):
         assert tokens(**kw) == _lib.CQ_ERR_BAD_ARG
     for kw in (dict(dim=64), dict(t=24577, ws=24577)):
         assert tokens(**kw) == _lib.CQ_ERR_UNSUPPORTED
+
+
+def test_what_is_narrower_than_16_bytes(lib, p16):
+    """Pointers to 4- and 8-byte numbers may start anywhere that their type may."""
+    w = lambda a, vis_in=None, fp_in=None, vis=p16, fp=p16: lib.cq_key_weights(a, vis_in, fp_in, vis, fp, 16, p16, 1 << 30, None)
+    for c in (dict(lse=p16 + 2), dict(t_fp_dev=p16 + 1)):
+        assert lib.cq_chunk_attn(ctypes.byref(chunk_args(p16, **c)), p16, 1 << 30, None) == _lib.CQ_ERR_BAD_ARG
+        assert w(ctypes.byref(chunk_args(p16, **c))) == _lib.CQ_ERR_BAD_ARG
+    for kw in (dict(vis_in=p16 + 2), dict(fp_in=p16 + 1), dict(vis=p16 + 2), dict(fp=p16 + 3)):
+        assert w(ctypes.byref(chunk_args(p16, batch=0)), **kw) == _lib.CQ_ERR_BAD_ARG
+    assert w(ctypes.byref(chunk_args(p16, batch=0, lse=p16 + 4, t_fp_dev=p16 + 4)), vis=p16 + 4) == _lib.CQ_OK
+
+    def tokens(w=p16, w_out=p16, kept=p16):
+        return lib.cq_evict_tokens(p16, p16, 6400, 6400, w, 50, 0, 1, 128, 50, 20, 5, 5, p16, p16, w_out, kept, None)
+    assert tokens(w=p16 + 4, w_out=p16 + 4, kept=p16 + 8) == _lib.CQ_OK
+    for kw in (dict(w=p16 + 2), dict(w_out=p16 + 2), dict(kept=p16 + 4)):
+        assert tokens(**kw) == _lib.CQ_ERR_BAD_ARG
