@@ -292,6 +292,9 @@ class GraphedDecoder:
                 t.zero_()
                 if w0 is not None:
                     t[..., :w0[i].shape[-1]] = w0[i]
+        # what the graph reads and writes, whatever prompt the layers see meanwhile
+        self.held = [(a.__dict__.get("k_pack"), a.__dict__.get("v_pack"), a.__dict__.get("_u8_state"), a.__dict__.get("_key_weights"))
+                     for a in (layer.attention for layer in lm.model.layers)]
         self.graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(self.graph, stream=side):     # the warm-up's stream: its scratch buffers are reused
             self._step()

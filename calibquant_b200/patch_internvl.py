@@ -272,6 +272,8 @@ def _attend_tracked(self, q, t_fp, mask=None, t_fp_dev=None):
 
 def _forward_chunk(self, hidden_states, attention_mask, position_ids, past_key_value, use_cache):
     """Several new tokens on the cache of this layer."""
+    if getattr(self, "_static_decode", False):
+        raise ValueError("the cache belongs to a captured decoder, which counts its tokens on the device: close the decoder first")
     k_pack, v_pack = _chunk_cache(self)
     bsz, q_len, _ = hidden_states.size()
     n_rep, tc = self.num_key_value_groups, self._text_cache
@@ -307,6 +309,8 @@ def track_key_weights(model, on: bool = True):
     """Have every attention layer of the patched model add up, per KV head, how much attention each cached key gets: from the question of
     the next prompt on (its tokens behind the visual span), over chunks and single tokens.  4-bit group format.  What
     has been added up is in ``attention._key_weights`` (visual, full-precision); ``evict_cache`` uses it."""
+    if any(getattr(attn, "_static_decode", False) for attn in _attentions(model)):
+        raise ValueError("a captured decoder adds up weights, or does not, as it was captured: close the decoder first")
     for attn in _attentions(model):
         attn._track_weights = bool(on)
         attn._key_weights = None

@@ -200,3 +200,28 @@ def test_what_is_not_served(monkeypatch):
     (_, past), at = prompt(shell)
     with pytest.raises(NotImplementedError):
         lm.forward_step(embeds(2, 3, shell, 1), positions(2, at, 3), past)
+
+
+def test_an_open_decoder_keeps_cache_and_weights():
+    """What would move or drop what a captured graph writes is refused until the decoder is closed; a prompt in between is not."""
+    from calibquant_b200 import internlm2, patch_internvl as pi
+    shell = build()
+    pi.track_key_weights(shell)
+    lm = shell.language_model
+    (logits, past), at = prompt(shell, text=17)
+    dec = internlm2.GraphedDecoder(lm, past, logits[:, -1].argmax(-1), at, 12, fused=False)
+    attn = lm.model.layers[0].attention
+    weights, before = attn._key_weights, [t.clone() for t in attn._key_weights]
+    for refused in (lambda: lm.forward_step(embeds(2, 3, shell, 1), positions(2, at, 3), past), lambda: pi.track_key_weights(shell, False),
+                    lambda: pi.track_key_weights(shell), lambda: pi.evict_cache(shell, keep_groups=1)):
+        with pytest.raises(ValueError):
+            refused()
+    assert attn._key_weights is weights and all(torch.equal(a, b) for a, b in zip(weights, before))
+    dec.run(2)
+    assert not torch.equal(weights[1], before[1])
+    ids = [t.data_ptr() for t in weights]
+    del weights
+    prompt(shell, text=5)                          # its layers start new caches and weights, those of the graph stay
+    assert [t.data_ptr() for t in dec.held[0][3]] == ids
+    dec.run(1)
+    torch.cuda.synchronize()
