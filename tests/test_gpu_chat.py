@@ -225,3 +225,21 @@ def test_an_open_decoder_keeps_cache_and_weights():
     assert [t.data_ptr() for t in dec.held[0][3]] == ids
     dec.run(1)
     torch.cuda.synchronize()
+
+
+def test_a_refused_eviction_changes_nothing():
+    from calibquant_b200 import patch_internvl as pi
+    shell = build(layers=2)
+    pi.track_key_weights(shell)
+    (_, past), _ = prompt(shell, text=20)
+    layers = [l.attention for l in shell.language_model.model.layers]
+    before = [(a.k_pack, a.v_pack, a._text_cache, a._text_cache.length, a._key_weights) for a in layers]
+    n = SYS + 20
+    for kw in (dict(keep_groups=0), dict(keep_groups=VIS // 32 + 1), dict(keep_groups=1, keep_tokens=n + 1), dict(keep_groups=1, keep_tokens=SYS + 3, recent=4),
+               dict(keep_groups=1, keep_tokens=0, recent=0), dict(keep_groups=1, keep_tokens=n, recent=-1)):
+        with pytest.raises(ValueError):
+            pi.evict_cache(shell, **kw)
+    for a, b in zip(layers, before):
+        assert all(x is y for x, y in zip((a.k_pack, a.v_pack, a._text_cache, a._text_cache.length, a._key_weights), b)) and a._evicted == 0
+    pi.evict_cache(shell, keep_groups=1, keep_tokens=SYS + 4, recent=4)
+    assert all(a._text_cache.length == SYS + 4 for a in layers)
