@@ -952,7 +952,11 @@ PyObject* py_key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
     out[0] = fresh({d.batch, d.n_kv_heads, d.t_vis}, c.q, at::kFloat);
     out[1] = fresh({d.batch, d.n_kv_heads, given ? in[1].size(2) : d.t_fp}, c.q, at::kFloat);
   }
-  if (d.batch > 0) {
+  if (d.q_len == 0) {      // no queries: what there was
+    for (int i : {0, 1})
+      if (!given) out[i].zero_();
+      else if (!out[i].is_same(in[i])) out[i].copy_(in[i]);
+  } else if (d.batch > 0) {
     const size_t nbytes = cq_key_weights_workspace_bytes(&d, out[1].size(2));
     if (nbytes == 0) {
       const int rc = cq_key_weights(&d, nullptr, nullptr, out[0].data_ptr<float>(), out[1].data_ptr<float>(), out[1].size(2), nullptr, 0, call.stream);

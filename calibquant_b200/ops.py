@@ -280,8 +280,8 @@ def chunk_attention(q, k_pack, v_pack, k_fp, v_fp, t_sys, bits=4, group_size=32,
     q [B,L,Hq,D] as :func:`prefill_rope_split` gives it; k_pack/v_pack = (code, scale, mn) as for
     :func:`decode_attention`, or None; k_fp/v_fp [B,Hkv,T,D] hold the system tokens, the text tokens and, as the last
     ``L`` of the first ``t_fp`` (default: all), the new tokens themselves.  A new token sees every visual token, and the
-    full-precision tokens up to itself.  ``mask``: optional additive [B, t_fp+T_vis] in key order [sys | visual | text]; a key at
-    -infinity takes no part whatever it holds, a row without keys gives zeros (and a log-sum-exp of -infinity).  Keys and values
+    full-precision tokens up to itself.  ``mask``: optional additive [B, t_fp+T_vis] in key order [sys | visual | text], rounded to q's
+    type (whose lowest number is a number, fp32's is -infinity in it); a key at -infinity takes no part whatever it holds, a row without keys gives zeros (and a log-sum-exp of -infinity).  Keys and values
     in the cache that nobody may see need not be numbers, those of the new tokens have to be finite.  ``t_fp_dev``: int32
     device scalar with the live token count; ``t_fp`` is then the capacity.  No logit calibration.
     Returns o [B,L,Hq,D], with ``return_lse`` also the scores' log-sum-exp fp32 [B,Hq,L], which :func:`key_weights` takes.

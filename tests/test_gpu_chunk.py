@@ -265,6 +265,19 @@ def test_empty_batch():
     assert [t.shape for t in ops.key_weights(q, lse, None, k, 4)] == [(0, 2, 0), (0, 2, 9)]
 
 
+def test_no_queries():
+    """Nothing to attend: an empty result, weights as they were."""
+    from calibquant_b200 import ops
+    q, kp, vp, k_fp, v_fp = make(2, 8, 2, 1, 64, 20, HALF)
+    out, lse = ops.chunk_attention(q[:, :0], kp, vp, k_fp, v_fp, 4, return_lse=True)
+    assert out.shape == (2, 0, 8, 128) and lse.shape == (2, 8, 0)
+    fresh = ops.key_weights(q[:, :0], lse, kp, k_fp, 4)
+    assert not fresh[0].any() and not fresh[1].any() and fresh[1].shape == (2, 2, 21)
+    w = (torch.rand(2, 2, 64, device="cuda"), torch.rand(2, 2, 30, device="cuda"))
+    for got in (ops.key_weights(q[:, :0], lse, kp, k_fp, 4, weights=w), ops.key_weights(q[:, :0], lse, kp, k_fp, 4, weights=w, out=w)):
+        assert torch.equal(got[0], w[0]) and torch.equal(got[1], w[1])
+
+
 def test_refusals():
     from calibquant_b200 import ops
     q, kp, vp, k_fp, v_fp = make(1, 8, 2, 3, 64, 20, HALF)
