@@ -8,11 +8,14 @@
 //   warp 16     issues the products
 //   warp 17     has TMA bring the query blocks into two slots
 // A block is the query heads of the KV head for as many queries as NB rows hold: a row of a block is the same head for every block.
-// Bound: 64 products of 64 cycles per pair of packed key tiles and 256 rows, whose operands take all of shared memory's bandwidth
-// (8 KB a product); the query blocks that TMA writes and the log-sum-exps that the sums read come on top: 82 cycles a product measured.
-// The 2 x 128 x 128 exponentials of a block take as long as its products (2048 cycles) and run beside them.  8 x 1024 queries on 3328
-// + 1280 keys, bfloat16: 411 us when cool, 460 in a row of launches, of which 12 % are the CTAs' starts (key tiles, first block).
-// Without the exponentials 478 against 488, without reading the log-sum-exps 470, with half the products 411 (one run).
+// Bound: 64 products of 64 cycles per pair of packed key tiles and 256 rows, and the 2 x 128 x 128 exponentials of a block of 128 rows, which
+// take the special-function units as long as its products take the tensor cores (2048 cycles) and run beside them; 2750 cycles a block
+// measured.  8 x 1024 queries on 3328 + 1280 keys, bfloat16: 422 us apart, 460 in a row of launches under the power cap, of which 10 % are
+// the CTAs' starts (key tiles, first block).  Half the products: 407, no exponentials: 385.  Keys in tensor memory as the products' other
+// operand (nothing but queries read from shared memory), four query slots, a quarter of the exponentials by a polynomial: 410 to 424, and 4 us
+// more for 20 to 100 queries, whose key tiles go through shared memory first.  Scores in halves of 64 rows: 474.
+// The rows' log-sum-exp come by cp.async one chunk ahead, both key tiles are requested before one is unpacked: 41 -> 39 us (2 x 517
+// queries on 1312 + 600), 28.6 -> 26.7 (300 on 3328 + 360).
 // TMEM: tile X's scores in columns X * 256 + buffer * 128.  Where the key tiles are fewer than the SMs, the rows are cut into parts whose
 // sums finish_kernel adds in their order.
 #include <cuda.h>
@@ -51,6 +54,10 @@ struct WeightParams {
   int* status;
 };
 
+__device__ __forceinline__ void cp_async4(void* dst, const void* src) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], 4;" ::"r"(smem_u32(dst)), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_all;" ::: "memory"); }
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -74,7 +81,7 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
   // bar_k the key tiles are there; bar_q/free[slot] query blocks; bar_d/dfree[X][buffer] scores ready / read
   __shared__ __align__(8) uint64_t bar_k, bar_q[2], bar_free[2], bar_d[2][2], bar_dfree[2][2];
   __shared__ uint32_t tmem_base_s;
-  __shared__ __align__(16) float lse_s[LSE_BLOCKS * NB];
+  __shared__ __align__(16) float lse_s[2][LSE_BLOCKS * NB];
   __shared__ float half_s[256];
 
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -185,14 +192,37 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
     if (!ok && lead) atomicExch(a.status, CQ_ERR_TIMEOUT);
     __syncwarp();
   } else {
+    // rows' log-sum-exp of the blocks from n0 on, on their way; what adds nothing -inf
+    const auto request_lse = [&](int n0, int buf) {
+      for (int c = tid; c < LSE_BLOCKS * NB; c += 512) {
+        const int r = c % NB, i = (blk0 + n0 + c / NB) * a.block_queries + r / p.n_rep;
+        if (r < a.block_rows && n0 + c / NB < nb && i < p.q_len)
+          cp_async4(&lse_s[buf][c], p.lse + ((int64_t)b * p.hq + hk * p.n_rep + r % p.n_rep) * p.q_len + i);
+        else
+          lse_s[buf][c] = -INFINITY;
+      }
+    };
+    // minus them in units of the exponent (with a mask: as they are); a row that adds nothing: an argument of -inf
+    const auto take_lse = [&](int buf) {
+      cp_async_wait();
+      for (int c = tid; c < LSE_BLOCKS * NB; c += 512) {
+        const float v = lse_s[buf][c];
+        lse_s[buf][c] = v == -INFINITY ? (MASK ? INFINITY : -INFINITY) : MASK ? v : -v * LOG2E;
+      }
+    };
+    if (nb > 0) request_lse(0, 0);
     // ================= the key tiles =================
     if (nb > 0) {
-      for (int x = 0; x < n_x; ++x) {
+      Unit u[2];
+#pragma unroll
+      for (int x = 0; x < 2; ++x)
+        if (x < n_x && tile0 + x < nv) load_k_unit(p, bh, tile0 + x, warp, lane, u[x]);
+#pragma unroll
+      for (int x = 0; x < 2; ++x) {
+        if (x >= n_x) break;
         const uint32_t hi = k_s + x * 2 * TILE_BYTES, lo = hi + TILE_BYTES;
         if (tile0 + x < nv) {
-          Unit u;
-          load_k_unit(p, bh, tile0 + x, warp, lane, u);
-          store_k_unit<BF16>(hi, lo, u, warp, lane);
+          store_k_unit<BF16>(hi, lo, u[x], warp, lane);
         } else {
           const T* src = static_cast<const T*>(p.k_fp) + b * p.fp_sb + hk * p.fp_sh;
 #pragma unroll
@@ -226,15 +256,10 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
     bool ok = true;
     float acc[4] = {};
     for (int n0 = 0; n0 < nb; n0 += LSE_BLOCKS) {
-      // minus the rows' log-sum-exp in units of the exponent (log-sum-exp as it is with a mask); a row that adds nothing: -inf
-      worker_barrier();
-      for (int c = tid; c < LSE_BLOCKS * NB; c += 512) {
-        const int r = c % NB, i = (blk0 + n0 + c / NB) * a.block_queries + r / p.n_rep;
-        float v = -INFINITY;
-        if (r < a.block_rows && n0 + c / NB < nb && i < p.q_len) v = p.lse[((int64_t)b * p.hq + hk * p.n_rep + r % p.n_rep) * p.q_len + i];
-        lse_s[c] = v == -INFINITY ? (MASK ? INFINITY : -INFINITY) : MASK ? v : -v * LOG2E;
-      }
-      worker_barrier();
+      const int buf = (n0 / LSE_BLOCKS) & 1;
+      take_lse(buf);
+      worker_barrier();                       // nobody reads the other half any more
+      if (n0 + LSE_BLOCKS < nb) request_lse(n0 + LSE_BLOCKS, buf ^ 1);
       if (x >= n_x) continue;
       for (int n = n0; n < min(nb, n0 + LSE_BLOCKS); ++n) {
         const int s = n & 1;
@@ -256,7 +281,7 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
 #pragma unroll
           for (int cc = 0; cc < 2; ++cc) {
             const int col0 = cc * 2 * COLS + half * COLS;
-            const float* l_s = lse_s + (n - n0) * NB + col0;
+            const float* l_s = &lse_s[buf][(n - n0) * NB + col0];
 #pragma unroll
             for (int c = 0; c < COLS; c += 4) {
               const float4 l = *reinterpret_cast<const float4*>(l_s + c);
