@@ -145,8 +145,9 @@ __global__ void __launch_bounds__(256) chunk_unpack_kernel(const __grid_constant
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, nv = (p.t_vis + 127) >> 7, tile = blockIdx.x;
   const int hk = blockIdx.y % p.hkv, b = blockIdx.y / p.hkv;
   const int64_t bh = (int64_t)b * p.hkv + hk;
-  const int live = live_tokens(p);
   pdl_launch_dependents();
+  pdl_wait();
+  const int live = live_tokens(p);
   unsigned char* dst = a.image + bh * image_bytes(nv, a.image_fp_tiles);
   int n;
   if (tile < nv) {
@@ -215,8 +216,8 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
     }
     mbar_fence_init();
   }
-  if (IMAGE) pdl_wait();                      // the images are the launch's before this one
   pdl_launch_dependents();
+  pdl_wait();
   const int live = live_tokens(p);
   if (warp == MMA_WARP) tmem_alloc(&tmem_base_s, 512);
   tc_fence_before();
@@ -693,7 +694,7 @@ constexpr int IMAGE_BLOCKS = 3;
 
 // ---- host ---------------------------------------------------------------------------------------------------------
 struct Plan {
-  bool few, pair, image;      // few: cq_chunk_few.cu
+  bool few, pair, image, cluster;      // few: cq_chunk_few.cu; cluster: it merges its parts itself
   int queries, row_blocks, grid_parts, parts;      // queries of a tile
 };
 // Split of the key tiles: as many CTAs as fill the SMs, in whole rounds where there are several; a CTA costs about three key tiles beside
@@ -702,10 +703,11 @@ static Plan make_plan(const cq_chunk_args* a) {
   Plan pl;
   const int64_t rows = (int64_t)a->q_len * (a->n_q_heads / a->n_kv_heads);
   pl.few = rows <= FEW_ROWS;
-  pl.pair = pl.image = false;
+  pl.pair = pl.image = pl.cluster = false;
   if (pl.few) {
     pl.queries = pl.row_blocks = 0;
-    pl.grid_parts = pl.parts = few_parts((int64_t)a->batch * a->n_kv_heads, a->t_vis, a->t_fp, rows > 8);
+    pl.grid_parts = pl.parts = few_parts((int64_t)a->batch * a->n_kv_heads, a->t_vis, a->t_fp, rows > 8, true);
+    pl.cluster = pl.parts > 1 && pl.parts <= FEW_CLUSTER;
     return pl;
   }
   pl.queries = 128 / (a->n_q_heads / a->n_kv_heads);
@@ -734,7 +736,7 @@ static size_t images_of(const cq_chunk_args* a, const Plan& pl) {
 }
 static size_t workspace_bytes(const cq_chunk_args* a, const Plan& pl) {
   const size_t rows = (size_t)a->batch * a->n_q_heads * a->q_len;
-  return 256 + images_of(a, pl) + (pl.parts == 1 ? 0 : rows * pl.parts * (128 * sizeof(float) + sizeof(float2)));
+  return 256 + images_of(a, pl) + (pl.parts == 1 || pl.cluster ? 0 : rows * pl.parts * (128 * sizeof(float) + sizeof(float2)));
 }
 
 template <bool BF16>
@@ -758,13 +760,9 @@ static int launch_attn(const CUtensorMap& tm, const AttnParams& p, const Plan& p
   const dim3 grid(pl.row_blocks, batch * p.p.hkv, pl.grid_parts);
   if (IMAGE) {
     const dim3 tiles((p.p.t_vis + 127) / 128 + p.image_fp_tiles, batch * p.p.hkv);
-    chunk_unpack_kernel<BF16, MASK><<<tiles, 256, 3 * TILE_BYTES + 1024, st>>>(p);
-    if (const int rc = check_launch()) return rc;
-    if (const int rc = launched(launch_pdl(chunk_attn_kernel<BF16, MASK, PAIR, IMAGE>, grid, dim3(Roles<IMAGE>::THREADS), SMEM_BYTES, st, tm, p))) return rc;
-  } else {
-    chunk_attn_kernel<BF16, MASK, PAIR, IMAGE><<<grid, Roles<IMAGE>::THREADS, SMEM_BYTES, st>>>(tm, p);
-    if (const int rc = check_launch()) return rc;
+    if (const int rc = launched(launch_pdl(chunk_unpack_kernel<BF16, MASK>, tiles, dim3(256), 3 * TILE_BYTES + 1024, st, p))) return rc;
   }
+  if (const int rc = launched(launch_pdl(chunk_attn_kernel<BF16, MASK, PAIR, IMAGE>, grid, dim3(Roles<IMAGE>::THREADS), SMEM_BYTES, st, tm, p))) return rc;
   return launch_combine<BF16>(p, batch, st);
 }
 
@@ -811,8 +809,9 @@ extern "C" int cq_chunk_attn(const cq_chunk_args* a, void* workspace, size_t wor
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (pl.few) {
     chunk::FewParams f = {};
-    f.p = p.p; f.part_o = p.part_o; f.part_ml = p.part_ml; f.status = p.status; f.parts = pl.parts;
-    if (const int rc = chunk::few_run(f, a->batch, bf16, false, st)) return rc;
+    f.p = p.p; f.part_o = p.part_o; f.part_ml = p.part_ml; f.status = p.status; f.parts = pl.parts; f.cluster = pl.cluster;
+    const int rc = chunk::few_run(f, a->batch, bf16, false, st);
+    if (rc || pl.cluster) return rc;
     return bf16 ? chunk::launch_combine<true>(p, a->batch, st) : chunk::launch_combine<false>(p, a->batch, st);
   }
   CUtensorMap tm;

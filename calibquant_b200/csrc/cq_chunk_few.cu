@@ -11,9 +11,11 @@
 // Which key (channel) a lane's row of A is, is free to choose: lane (g, c) takes the codes of word g % 4 of its group, the lower or the
 // upper four by g / 4.  So it loads one word per channel (key), half of which it uses, and a byte permute of two words leaves the pairs of
 // four A registers: one operation per code.  Register j = 2 * block + half of a lane stands for key (channel) index_of(g, j).
-// Each warp has a softmax of its own (running maximum and sum), merged in shared memory at the end; CTAs are merged by the combine launch.
+// Each warp has a softmax of its own (running maximum and sum), merged in shared memory at the end.  Up to eight CTAs of a KV head are a cluster
+// and merge through each other's shared memory, more by the combine launch.  One request of 256 + 23 keys, which two CTAs share that way:
+// 7.9 us, 10.2 with one (14 000 cycles: 2600 until the queries are there, 4400 full-precision keys, 3600 packed ones, 2700 merge).
 // Bound: instruction issue (0.55 a cycle and scheduler): about 1000 a group, of which 128 codes a lane of keys and as many of values take two each.
-// 16 requests x 8 heads x 3328 + 193 keys, four rows, bfloat16: 38 us (2.1 TB/s; the tile kernel 77), the weights of the keys 22.6; 8 x 32 768
+// 16 requests x 8 heads x 3328 + 193 keys, four rows, bfloat16: 38 us (2.1 TB/s; the tile kernel 77), the weights of the keys 22.3; 8 x 32 768
 // keys: 134 us.  On the way: every lane its own words from global memory 60, scales multiplied into the codes 55, one or two groups
 // a TMA request 51, whole rows 48, one address under eight exclusive ors 45.
 // TMA brings the codes of the next tile in while one is worked on, whole 128-byte rows (with the 16 or 32 bytes of one or two groups a
@@ -73,6 +75,26 @@ __device__ __forceinline__ uint32_t code_pair(uint32_t z, int j) {
 // Place within a group of 32 of row g (0..7) of register j = 2 * block + half
 __device__ __forceinline__ int index_of(int g, int j) { return (g & 3) * 8 + (g >> 2) * 4 + j; }
 
+// Shared memory of block `rank` of the cluster, at the same place as this block's
+__device__ __forceinline__ uint32_t peer(uint32_t addr, int rank) {
+  uint32_t r;
+  asm("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(r) : "r"(addr), "r"(rank));
+  return r;
+}
+__device__ __forceinline__ float peer_f32(uint32_t addr, int rank) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(peer(addr, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ float4 peer_f32x4(uint32_t addr, int rank) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(peer(addr, rank)) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cluster_sync() {
+  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+
 // A tile: codes [channel][32 words] and [two keys][32 words] (128-byte swizzle), scales and minima of the values [key][4].
 struct __align__(1024) Stage {
   uint32_t k[128][32];
@@ -104,6 +126,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
   const int hk = blockIdx.x % p.hkv, b = blockIdx.x / p.hkv, part = blockIdx.y;
   const int64_t bh = blockIdx.x;
   pdl_launch_dependents();
+  pdl_wait();
   const int live = live_tokens(p), groups = p.t_vis >> 5;
   // tiles: full-precision ones first (of what is to be written, for weights), under which the codes of the first visual one come in
   const int nf = (int)(((WEIGHTS ? a.capacity : (int64_t)live) + 255) >> 8), tiles = nf + ((groups + 7) >> 3), per = (tiles + (int)gridDim.y - 1) / (int)gridDim.y;
@@ -514,6 +537,15 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
         for (int h = 0; h < 2; ++h) merge_s[(warp * ROWS + r) * 128 + (i >> 1) * 32 + index_of(g, 2 * (i & 1) + h)] = o[i][nt][e + 2 * h];
     }
   __syncthreads();
+  float* own_s = ml_s + WARPS * ROWS * 2;       // the block's result, for the others of its cluster: [row][128, maximum, sum, 2 unused]
+  const auto result = [&](int r, float m, float l, const float (&x)[4]) {
+    const int i = r / p.n_rep;
+    const int64_t h = hk * p.n_rep + r - i * p.n_rep;
+    const float inv = l != l ? l : l > 0.f ? 1.f / l : 0.f;
+    T* dst = static_cast<T*>(p.out) + b * p.o_sb + i * p.o_st + h * p.o_sh + lane * 4;
+    *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<BF16>(x[0] * inv, x[1] * inv), pack16<BF16>(x[2] * inv, x[3] * inv));
+    if (p.lse && lane == 0) p.lse[(b * (int64_t)p.hq + h) * p.q_len + i] = l != l ? l : l > 0.f ? m + logf(l) : -INFINITY;
+  };
   for (int r = warp; r < min(ROWS, p.rows); r += WARPS) {
     float m = -INFINITY, l = 0.f, x[4] = {};
     for (int w = 0; w < WARPS; ++w) m = fmaxf(m, ml_s[(w * ROWS + r) * 2]);
@@ -526,19 +558,36 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
       l = fmaf(lw, f, l);
       x[0] = fmaf(v.x, f, x[0]); x[1] = fmaf(v.y, f, x[1]); x[2] = fmaf(v.z, f, x[2]); x[3] = fmaf(v.w, f, x[3]);
     }
-    const int i = r / p.n_rep;
-    const int64_t h = hk * p.n_rep + r - i * p.n_rep;
     if (gridDim.y == 1) {
-      const float inv = l != l ? l : l > 0.f ? 1.f / l : 0.f;
-      T* dst = static_cast<T*>(p.out) + b * p.o_sb + i * p.o_st + h * p.o_sh + lane * 4;
-      *reinterpret_cast<uint2*>(dst) = make_uint2(pack16<BF16>(x[0] * inv, x[1] * inv), pack16<BF16>(x[2] * inv, x[3] * inv));
-      if (p.lse && lane == 0) p.lse[(b * (int64_t)p.hq + h) * p.q_len + i] = l != l ? l : l > 0.f ? m + logf(l) : -INFINITY;
+      result(r, m, l, x);
+    } else if (a.cluster) {
+      float* own = own_s + r * 132;
+      *reinterpret_cast<float4*>(own + lane * 4) = make_float4(x[0], x[1], x[2], x[3]);
+      if (lane == 0) { own[128] = m; own[129] = l; }
     } else {
       const int64_t at = (bh * p.rows + r) * a.parts + part;
       *reinterpret_cast<float4*>(a.part_o + at * 128 + lane * 4) = make_float4(x[0], x[1], x[2], x[3]);
       if (lane == 0) a.part_ml[at] = make_float2(m, l);
     }
   }
+  if (!a.cluster) return;
+  // the blocks of a KV head are a cluster: block r % parts merges row r, in the order of the blocks
+  cluster_sync();
+  for (int r = part + warp * a.parts; r < min(ROWS, p.rows); r += WARPS * a.parts) {
+    const uint32_t own = smem_u32(own_s + r * 132);
+    float m = -INFINITY, l = 0.f, x[4] = {};
+    for (int s = 0; s < a.parts; ++s) m = fmaxf(m, peer_f32(own + 512, s));
+    for (int s = 0; s < a.parts; ++s) {
+      const float ms = peer_f32(own + 512, s), ls = peer_f32(own + 516, s);
+      if (ms == -INFINITY && ls == ls) continue;
+      const float f = ex2_approx((ms - m) * LOG2E);
+      const float4 v = peer_f32x4(own + lane * 16, s);
+      l = fmaf(ls, f, l);
+      x[0] = fmaf(v.x, f, x[0]); x[1] = fmaf(v.y, f, x[1]); x[2] = fmaf(v.z, f, x[2]); x[3] = fmaf(v.w, f, x[3]);
+    }
+    result(r, m, l, x);
+  }
+  cluster_sync();                               // nobody leaves while its memory is read
 }
 
 // Packed codes as a map of 32-bit words: `words` of a row, `rows` rows, `heads` of those (0: a map of two dimensions); a box of box_words x box_rows
@@ -561,7 +610,7 @@ static int run(const FewParams& p, int batch, cudaStream_t st) {
   if (!code_map(&tk, p.p.k_code, p.p.t_vis / 8, 128 * (int64_t)batch * p.p.hkv, 0, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B) ||
       !code_map(&tv, p.p.v_code, 32, p.p.t_vis / 2, (int64_t)batch * p.p.hkv, 32, 128, CU_TENSOR_MAP_SWIZZLE_128B))
     return CQ_ERR_LAUNCH;
-  constexpr int stages = 1024 + 2 * (int)(sizeof(Scales) + sizeof(StageOf<WEIGHTS>)), results = WEIGHTS ? 0 : 1024 + WARPS * 8 * NT * 130 * (int)sizeof(float);
+  constexpr int stages = 1024 + 2 * (int)(sizeof(Scales) + sizeof(StageOf<WEIGHTS>)), results = WEIGHTS ? 0 : 1024 + 8 * NT * (WARPS * 130 + 132) * (int)sizeof(float);
   constexpr int smem = stages > results ? stages : results;
   if (smem > 24 * 1024) {
     static bool configured[64] = {};
@@ -572,21 +621,33 @@ static int run(const FewParams& p, int batch, cudaStream_t st) {
       configured[dev] = true;
     }
   }
-  few_kernel<BF16, MASK, NT, WEIGHTS><<<dim3((unsigned)(batch * p.p.hkv), p.parts), THREADS, smem, st>>>(tk, tv, p);
-  return check_launch();
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(batch * p.p.hkv), p.parts);
+  cfg.blockDim = dim3(THREADS);
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute attr[2];
+  attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  attr[0].val.programmaticStreamSerializationAllowed = 1;
+  attr[1].id = cudaLaunchAttributeClusterDimension;
+  attr[1].val.clusterDim.x = 1; attr[1].val.clusterDim.y = p.cluster ? p.parts : 1; attr[1].val.clusterDim.z = 1;
+  cfg.attrs = attr;
+  cfg.numAttrs = p.cluster ? 2 : 1;
+  return launched(cudaLaunchKernelEx(&cfg, few_kernel<BF16, MASK, NT, WEIGHTS>, tk, tv, p));
 }
 
 }  // namespace few
 
 // CTAs per KV head: two an SM (one for the attention of more than eight rows), in whole rounds; a CTA costs about a tile of 256 keys beside its own.
-int few_parts(int64_t heads, int64_t t_vis, int64_t fp_keys, bool one) {
+// The blocks of an attention's KV head, up to FEW_CLUSTER, merge their results as a cluster; more take a second launch.
+int few_parts(int64_t heads, int64_t t_vis, int64_t fp_keys, bool one, bool merged) {
   const int64_t slots = (int64_t)sm_count() * (one ? 1 : 2), tiles = (t_vis + 255) / 256 + (fp_keys + 255) / 256;
   double cost = 1e300;
   int best = 1;
   for (int s = 1; s <= 64 && s <= tiles; ++s) {
     const int64_t per = (tiles + s - 1) / s;
     if ((tiles + per - 1) / per != s) continue;      // leaves a part empty
-    const double c = (double)((heads * s + slots - 1) / slots) * (per + 1.0) + (s > 1 ? 1.0 : 0.0);
+    const double c = (double)((heads * s + slots - 1) / slots) * (per + 1.0) + (!merged || s == 1 ? 0.0 : s <= FEW_CLUSTER ? 0.25 : 1.5);
     if (c < cost) { cost = c; best = s; }
   }
   return best;

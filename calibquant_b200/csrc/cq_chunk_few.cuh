@@ -6,7 +6,7 @@
 namespace cq {
 namespace chunk {
 
-constexpr int FEW_ROWS = 16;
+constexpr int FEW_ROWS = 16, FEW_CLUSTER = 8;
 
 struct FewParams {
   Params p;
@@ -17,9 +17,10 @@ struct FewParams {
   float *vis, *fp;
   int64_t capacity;
   int* status;
+  int cluster;                                 // attention: the parts of a KV head merge as a cluster, part_o and part_ml are not used
 };
 
-int few_parts(int64_t heads, int64_t t_vis, int64_t fp_keys, bool one);
+int few_parts(int64_t heads, int64_t t_vis, int64_t fp_keys, bool one, bool merged);
 int few_run(const FewParams& p, int batch, bool bf16, bool weights, cudaStream_t st);
 
 }  // namespace chunk

@@ -11,6 +11,7 @@
 // measured; four CTAs an SM, each selecting for itself: 82).  16 x 8 heads of 4099 full-precision tokens, a quarter kept: 36 us, 3.9 TB/s.
 // One launch: every CTA of a (batch row, KV head) finds the selection itself and moves its share of the cache.
 #include "cq_common.cuh"
+#include "cq_ptx.cuh"
 
 namespace cq {
 namespace evict {
@@ -156,6 +157,8 @@ __global__ void __launch_bounds__(THREADS) groups_kernel(Groups p) {
   const int64_t bh = blockIdx.y;
   const int keep = p.keep, groups = p.groups, lane = threadIdx.x & 31;
   const float4* w = p.weights + bh * groups * 8;
+  ptx::pdl_launch_dependents();
+  ptx::pdl_wait();
   for (int g = threadIdx.x; g < groups; g += THREADS) {
     float4 v[8];
 #pragma unroll
@@ -233,6 +236,8 @@ __global__ void __launch_bounds__(THREADS) tokens_kernel(Tokens p) {
   int* list = reinterpret_cast<int*>(key32 + p.t_fp);
   const int64_t bh = blockIdx.y;
   const float* w = p.weights + bh * p.w_stride;
+  ptx::pdl_launch_dependents();
+  ptx::pdl_wait();
   // among the tokens that need not stay
   const int n = p.t_fp - p.t_sys - p.recent, m = p.keep - p.t_sys - p.recent;
   for (int t = threadIdx.x; t < n; t += THREADS) key32[t] = ordered(w[p.t_sys + t]);
@@ -283,8 +288,7 @@ static int run(void (*kern)(K...), dim3 grid, size_t smem, cudaStream_t st, A...
     (void)cudaGetLastError();
     return CQ_ERR_LAUNCH;
   }
-  kern<<<grid, THREADS, smem, st>>>(args...);
-  return check_launch();
+  return launched(launch_pdl(kern, grid, dim3(THREADS), smem, st, args...));
 }
 
 }  // namespace evict

@@ -87,6 +87,8 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int hk = blockIdx.y % p.hkv, b = blockIdx.y / p.hkv;
   const int64_t bh = (int64_t)b * p.hkv + hk;
+  pdl_launch_dependents();
+  pdl_wait();
   const int live = live_tokens(p), nv = (p.t_vis + 127) >> 7;
   // first key of tile X; keys of a tile that are there; first row that sees one of them
   const int tile0 = (int)blockIdx.x * 2;
@@ -98,7 +100,6 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
   const int blk1 = min(blocks_all, blk0 + per);
   if (tile0 >= nv) blk0 = max(blk0, (int)min((int64_t)blk1, first_row((tile0 - nv) * 128) / a.block_rows));
   const int n_x = !alive(0) ? 0 : alive(1) ? 2 : 1, nb = n_x ? blk1 - blk0 : 0;
-  pdl_launch_dependents();
 
   if (tid == 0) {
     mbar_init(&bar_k, WORKERS);
@@ -372,8 +373,7 @@ static int run(const CUtensorMap& tm, const WeightParams& p, const Plan& pl, cud
     configured[dev] = true;
   }
   const unsigned bh = (unsigned)(p.batch * p.p.hkv);
-  key_weights_kernel<BF16, MASK, NB><<<dim3(pl.pairs, bh, pl.parts), THREADS, SMEM_BYTES, st>>>(tm, p);
-  if (const int rc = check_launch()) return rc;
+  if (const int rc = launched(launch_pdl(key_weights_kernel<BF16, MASK, NB>, dim3(pl.pairs, bh, pl.parts), dim3(THREADS), SMEM_BYTES, st, tm, p))) return rc;
   if (pl.parts == 1) return CQ_OK;
   return launched(launch_pdl(key_weights_finish_kernel, dim3((unsigned)((p.p.t_vis + p.capacity + 255) / 256), bh), dim3(256), 0, st, p));
 }
@@ -410,7 +410,7 @@ extern "C" int cq_key_weights(const cq_chunk_args* a, const float* w_vis_in, con
     f.p = chunk::make_params(a);
     f.vis_in = w_vis_in; f.fp_in = w_fp_in; f.vis = w_vis; f.fp = w_fp; f.capacity = w_capacity;
     f.status = static_cast<int*>(workspace);
-    f.parts = chunk::few_parts((int64_t)a->batch * a->n_kv_heads, a->t_vis, w_capacity, false);
+    f.parts = chunk::few_parts((int64_t)a->batch * a->n_kv_heads, a->t_vis, w_capacity, false, false);
     return chunk::few_run(f, a->batch, bf16, true, st);
   }
   WeightParams p = {};
