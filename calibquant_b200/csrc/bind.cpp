@@ -142,6 +142,27 @@ Tensor empty(at::IntArrayRef size, const Tensor& like) { return at::empty(size, 
 Tensor empty(at::IntArrayRef size, const Tensor& like, at::ScalarType dt) { return at::empty(size, like.options().dtype(dt)); }
 // The same from the device's allocator without the dispatcher, for calls with many results
 Tensor fresh(at::IntArrayRef size, const Tensor& like, at::ScalarType dt) { return at::detail::empty_cuda(size, dt, like.device(), c10::nullopt); }
+// Results of a call that are kept or dropped together, in one allocation: sizes are asked for, then the tensors taken in that order.
+class Together {
+  std::vector<int64_t> at_;
+  int64_t bytes_ = 0;
+  size_t taken_ = 0;
+  Tensor base_;
+ public:
+  void want(at::IntArrayRef size, at::ScalarType dt) {
+    int64_t n = (int64_t)c10::elementSize(dt);
+    for (const int64_t d : size) n *= d;
+    at_.push_back(bytes_);
+    bytes_ += (n + 255) / 256 * 256;
+  }
+  Tensor take(at::IntArrayRef size, const Tensor& like, at::ScalarType dt) {
+    if (!base_.defined()) base_ = fresh({bytes_}, like, at::kByte);
+    Tensor t = at::detail::make_tensor<c10::TensorImpl>(c10::Storage(base_.storage()), c10::DispatchKeySet(c10::DispatchKey::CUDA), c10::scalarTypeToTypeMeta(dt));
+    t.unsafeGetTensorImpl()->set_sizes_contiguous(size);
+    t.unsafeGetTensorImpl()->set_storage_offset(at_[taken_++] / (int64_t)c10::elementSize(dt));
+    return t;
+  }
+};
 
 PyObject* wrap(Tensor t) { return THPVariable_Wrap(std::move(t)); }
 PyObject* wrap2(Tensor a, Tensor b) {
@@ -949,8 +970,10 @@ PyObject* py_key_weights(PyObject*, PyObject* const* a, Py_ssize_t n) {
       if (!t.is_contiguous()) raise(PyExc_ValueError, "out must be contiguous");
     if (given && out[1].size(2) != in[1].size(2)) raise(PyExc_ValueError, "weights and out must have the same shapes");
   } else {
-    out[0] = fresh({d.batch, d.n_kv_heads, d.t_vis}, c.q, at::kFloat);
-    out[1] = fresh({d.batch, d.n_kv_heads, given ? in[1].size(2) : d.t_fp}, c.q, at::kFloat);
+    const int64_t n[2] = {d.t_vis, given ? in[1].size(2) : d.t_fp};
+    Together both;
+    for (int i : {0, 1}) both.want({d.batch, d.n_kv_heads, n[i]}, at::kFloat);
+    for (int i : {0, 1}) out[i] = both.take({d.batch, d.n_kv_heads, n[i]}, c.q, at::kFloat);
   }
   if (d.q_len == 0) {      // no queries: what there was
     for (int i : {0, 1})
@@ -998,13 +1021,17 @@ PyObject* py_evict_groups(PyObject*, PyObject* const* a, Py_ssize_t n) {
   want_pack(vp, B, H, 32 * G, bits, false, like, "v_pack");
   want_size(tensor(a[2]), {B, H, 32 * G}, at::kFloat, like, "weights");
   const Tensor w = packed_rows(tensor(a[2]));
-  ko[0] = fresh({B, H, D, keep * bits}, like, at::kInt);
-  vo[0] = fresh({B, H, 32 * keep, 4 * bits}, like, at::kInt);
-  for (int i : {1, 2}) {
-    ko[i] = fresh({B, H, D, keep}, like, like.scalar_type());
-    vo[i] = fresh({B, H, 32 * keep, 4}, like, like.scalar_type());
-  }
-  const Tensor wo = fresh({B, H, 32 * keep}, like, at::kFloat), kept = fresh({B, H, keep}, like, at::kLong);
+  const at::ScalarType dt = like.scalar_type();
+  Together keys, values, rest;
+  keys.want({B, H, D, keep * bits}, at::kInt);
+  values.want({B, H, 32 * keep, 4 * bits}, at::kInt);
+  for (int i = 0; i < 2; ++i) { keys.want({B, H, D, keep}, dt); values.want({B, H, 32 * keep, 4}, dt); }
+  rest.want({B, H, 32 * keep}, at::kFloat);
+  rest.want({B, H, keep}, at::kLong);
+  ko[0] = keys.take({B, H, D, keep * bits}, like, at::kInt);
+  vo[0] = values.take({B, H, 32 * keep, 4 * bits}, like, at::kInt);
+  for (int i : {1, 2}) { ko[i] = keys.take({B, H, D, keep}, like, dt); vo[i] = values.take({B, H, 32 * keep, 4}, like, dt); }
+  const Tensor wo = rest.take({B, H, 32 * keep}, like, at::kFloat), kept = rest.take({B, H, keep}, like, at::kLong);
   if (B * H)
     launch([&] { return cq_evict_groups((const int32_t*)kp[0].data_ptr(), kp[1].data_ptr(), kp[2].data_ptr(), (const int32_t*)vp[0].data_ptr(), vp[1].data_ptr(),
                            vp[2].data_ptr(), w.data_ptr<float>(), (int)B, (int)H, (int)D, (int)(32 * G), (int)keep, (int)bits, (int)group,
@@ -1037,8 +1064,12 @@ PyObject* py_evict_tokens(PyObject*, PyObject* const* a, Py_ssize_t n) {
   want_size(w, {B, H, w.size(2)}, at::kFloat, c.k_fp, "weights");
   if (w.size(2) < t_fp) raise(PyExc_ValueError, "the weights must cover t_fp tokens");
   w = contiguous(w);
-  const Tensor ko = fresh({B, H, keep, D}, c.k_fp, c.k_fp.scalar_type()), vo = fresh({B, H, keep, D}, c.k_fp, c.k_fp.scalar_type());
-  const Tensor wo = fresh({B, H, keep}, c.k_fp, at::kFloat), kept = fresh({B, H, keep}, c.k_fp, at::kLong);
+  Together cache, rest;
+  for (int i = 0; i < 2; ++i) cache.want({B, H, keep, D}, c.k_fp.scalar_type());
+  rest.want({B, H, keep}, at::kFloat);
+  rest.want({B, H, keep}, at::kLong);
+  const Tensor ko = cache.take({B, H, keep, D}, c.k_fp, c.k_fp.scalar_type()), vo = cache.take({B, H, keep, D}, c.k_fp, c.k_fp.scalar_type());
+  const Tensor wo = rest.take({B, H, keep}, c.k_fp, at::kFloat), kept = rest.take({B, H, keep}, c.k_fp, at::kLong);
   if (B * H)
     launch([&] { return cq_evict_tokens(c.k_fp.data_ptr(), c.v_fp.data_ptr(), c.k_fp.stride(0), c.k_fp.stride(1), w.data_ptr<float>(), w.size(2), (int)B, (int)H,
                            (int)D, (int)t_fp, (int)keep, (int)sys, (int)recent, ko.data_ptr(), vo.data_ptr(), wo.data_ptr<float>(),

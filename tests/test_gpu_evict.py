@@ -112,3 +112,24 @@ def test_refusals():
     big = torch.empty(1, 1, 24577, 128, dtype=torch.float16, device="cuda")
     with pytest.raises(ValueError):
         ops.evict_tokens(big, big, torch.zeros(1, 1, 24577, device="cuda"), 5)
+
+
+def test_results_are_tensors_of_their_own():
+    """Results that share an allocation neither overlap nor know of one another: in-place changes, views, autograd's version counters, copies."""
+    from calibquant_b200 import ops
+    k = torch.randn(2, 2, 40, 128, device="cuda").half()
+    w = torch.rand(2, 2, 40, device="cuda")
+    k2, v2, w2, kept = ops.evict_tokens(k, -k, w, 7)
+    kp, vp = ops.pack_k_per_channel(k[:, :, :32].contiguous(), 32, 4), ops.pack_v_per_token(k[:, :, :32].contiguous(), 32, 4)
+    groups = ops.evict_groups(kp, vp, w[:, :, :32].contiguous(), 1)
+    for results in ((k2, v2, w2, kept), (*groups[0], *groups[1], *groups[2:])):
+        before = [t.clone() for t in results]
+        for i, t in enumerate(results):
+            versions = [u._version for u in results]
+            assert t.is_contiguous() and t.data_ptr() % 256 == 0 and t.device == k.device
+            t.zero_()
+            assert [u._version for u in results] == [v + (j == i) for j, v in enumerate(versions)]
+            assert all(torch.equal(u, b) for u, b in zip(results[i + 1:], before[i + 1:])) and not t.any()
+    x = torch.zeros_like(w2).requires_grad_()
+    (x * w2).sum().backward()
+    assert x.grad.shape == w2.shape
