@@ -7,8 +7,8 @@
 // agree stay.  A unit stays if it is above that value, or equal to it and among the first of the equal ones that fill the rest.  A group's weight is the sum of its 32 weights in 64 bits, so that the order of the additions decides
 // no border.  Only counts are added atomically: the result depends on nothing but the weights.
 // Bound: HBM, and before it the selection, which every CTA waits for.  A group's keys are 16 bytes of 128 rows: a quarter of the groups kept
-// reads two thirds of the rows' 64-byte pieces and all of the scales, 261 MB for 8 x 8 heads of 32 768 tokens (40 us at the copy rate, 65
-// measured; four CTAs an SM, each selecting for itself: 82).  16 x 8 heads of 4099 full-precision tokens, a quarter kept: 36 us, 3.9 TB/s.
+// reads two thirds of the rows' 64-byte pieces and all of the scales, 261 MB for 8 x 8 heads of 32 768 tokens (40 us at the copy rate, 62
+// measured; four CTAs an SM, each selecting for itself: 82).  16 x 8 heads of 4099 full-precision tokens, a quarter kept: 35 us, 4 TB/s (31 behind one another).
 // One launch: every CTA of a (batch row, KV head) finds the selection itself and moves its share of the cache.
 #include "cq_common.cuh"
 #include "cq_ptx.cuh"
