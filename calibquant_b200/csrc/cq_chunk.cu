@@ -13,14 +13,15 @@
 //   warp 16          issues the products
 // S = Q K^T with packed keys as two 16-bit terms (their sum is scale * code + minimum exactly), so scores carry no rounding but
 // that of fp32 sums; O += P V with P in tensor memory.  S_A [0,128) S_B [128,256) O_A [256,384) O_B [384,512) TMEM columns.
-// Key tiles that three or more row blocks would unpack are unpacked once, by chunk_unpack_kernel, into images of the shared-memory tiles (96 KB per
+// Key tiles that six or more row blocks would unpack are unpacked once, by chunk_unpack_kernel, into images of the shared-memory tiles (96 KB per
 // 128 visual tokens), which the attention then loads in bulk.
 //
 // What bounds it.  With images: 48 products of 64 cycles a key tile and pair of query tiles; measured 4100 cycles (8 x 1024 queries on
 // 3328 + 1280 keys, bfloat16, at 1.75 GHz under the power cap: 588 us, and 52 for the images at 4.5 TB/s).  What is above is the chain of one query tile
-// (S -> softmax, 1900 cycles -> P V -> next S) that the other one does not cover.  Without images: the issue slots that unpacking
-// (39 instructions per word of eight keys, twice rounded) and softmax share, about 9000 cycles a tile; with images for one row block
-// too, 37 queries of four requests on 6656 tokens took 101 us instead of 67.
+// (S -> softmax, 1900 cycles -> P V -> next S) that the other one does not cover.  Without images: the same chain beside warps that unpack
+// (39 instructions per word of eight keys, twice rounded), and instructions that do not come in time: with the two halves of a row's scores as
+// a loop instead of two copies of the code 73.5 -> 66 us (37 queries of four padded requests on 6656 tokens), 112 -> 98 (40 of 16 on
+// 3328); quarters, or a loop over the warp's two units, gave nothing more.  With images for one row block too: 101.
 // Taken for granted by neither: a slot or tile as an index instead of a constant costs the issuing lane 104 cycles a product (917 -> 1036 us
 // when the slot became a switch, 676 with constants); a ring of five slots held up the keys (980 -> 945).
 // Every wait is bounded; one that runs out sets CQ_ERR_TIMEOUT in the workspace's first word, and the CTA ends.
@@ -528,7 +529,7 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
       };
       if (IMAGE) read(0);
       if (IMAGE) read(1);
-#pragma unroll
+#pragma unroll (IMAGE ? 2 : 1)
       for (int half = 0; half < 2; ++half) {
         if (!IMAGE) read(half);
         if (!IMAGE || half == 0) tmem_ld_wait();
@@ -560,7 +561,7 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
       if (grow) m_ref = m_true;
       const float m_use = m_ref == -INFINITY ? 0.f : m_ref, neg = -m_use * factor;
       float rs[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
+#pragma unroll (IMAGE ? 2 : 1)
       for (int half = 0; half < 2; ++half) {
         uint32_t w[32];
         if (!IMAGE) {
@@ -690,7 +691,9 @@ __global__ void __launch_bounds__(256) chunk_combine_kernel(AttnParams a, int64_
   if (p.lse && lane == 0) p.lse[(b * p.hq + h) * p.q_len + i] = bad ? NAN : l > 0.f ? m + logf(l) : -INFINITY;
 }
 
-constexpr int IMAGE_BLOCKS = 3;
+// 3328 visual tokens, images against unpacking in the kernel: 300 queries of 8 requests (5 row blocks) 290 against 282 us, 400 (7 blocks) 371
+// against 380, 150 (3 blocks) 192 against 167.
+constexpr int IMAGE_BLOCKS = 6;
 
 // ---- host ---------------------------------------------------------------------------------------------------------
 struct Plan {

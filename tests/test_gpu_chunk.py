@@ -86,6 +86,28 @@ def test_masks(dtype, L):
     check(q, kp, vp, k_fp, v_fp, t_sys, mask.view(B, 1, 1, n).float())       # another shape and type of the same numbers
 
 
+@pytest.mark.parametrize("dtype", [HALF, BF16])
+@pytest.mark.parametrize("shape", [(2, 8, 2, 385, 160, 70), (1, 16, 2, 200, 416, 87), (1, 32, 1, 45, 96, 33), (1, 2, 2, 1300, 0, 40), (1, 12, 2, 333, 1312, 0)], ids=str)
+def test_many_row_blocks(shape, dtype):
+    """Six row blocks and more: key tiles unpacked once; a live count that ends inside the first of the tiles; masks."""
+    q, kp, vp, k_fp, v_fp = make(*shape, dtype, seed=sum(shape))
+    check(q, kp, vp, k_fp, v_fp, min(41, shape[5]))
+    t_fp = k_fp.shape[2]
+    for live in (t_fp - 3, shape[3] // 2, 1):
+        k_fp[:, :, live:], v_fp[:, :, live:] = math.nan, math.nan
+        check(q, kp, vp, k_fp, v_fp, min(41, shape[5]), t_fp=t_fp, t_fp_dev=torch.tensor([live], dtype=torch.int32, device="cuda"), live=live)
+
+
+@pytest.mark.parametrize("dtype", [HALF, BF16])
+def test_masks_of_many_row_blocks(dtype):
+    test_masks(dtype, 390)
+
+
+@pytest.mark.parametrize("L,B", [(500, 1), (390, 2)])
+def test_many_row_blocks_captured(L, B):
+    test_captured_and_replayed(L, B)
+
+
 @pytest.mark.parametrize("live", [70, 41, 7, 3, 0])
 def test_live_count(live):
     """Tokens that are not live yet hold anything; fewer live tokens than new ones leave the first queries the visual span alone."""
@@ -208,7 +230,7 @@ def test_captured_and_replayed(L, B):
         torch.cuda.current_stream().wait_stream(side)
         assert torch.equal(out, again[0]) and torch.equal(lse, again[1])
         assert all(torch.equal(2 * t, u) for t, u in zip(ops.key_weights(q, lse, kp, k_fp, 41, t_fp_dev=counter), again_acc))
-        want, want_l, room, room_l = ref.attention64(q, kp, vp, k_fp, v_fp, 41, live=live)
+        want, want_l, room, room_l = ref.attention64(q, kp, vp, k_fp, v_fp, 41, live=min(live, 500))      # a count above the capacity is the capacity
         assert ref.within(out, want, room) and ref.within(lse, want_l, room_l)
 
 
