@@ -123,6 +123,23 @@ def test_live_count(live):
         assert ref.within(out, want, room)
 
 
+@pytest.mark.parametrize("L", [1, 3])
+@pytest.mark.parametrize("cap", [1500, 5000])
+@pytest.mark.parametrize("dtype", [HALF, BF16])
+def test_few_rows_of_a_long_capacity(dtype, cap, L):
+    """Single tokens whose blocks merge as a cluster (1500: seven blocks a head) or by a second launch (5000): a small live count leaves most
+    blocks without a key, and a row without any key has none in all of them."""
+    q, kp, vp, k_fp, v_fp = make(2, 8, 2, L, 96, 700, dtype, seed=cap + L, cap=cap)
+    none = torch.zeros(2, 96 + cap, dtype=dtype, device="cuda")
+    none[1] = -math.inf
+    for live in (cap, 700, 300, 2):
+        k_fp[:, :, live:], v_fp[:, :, live:] = math.nan, math.nan
+        counter = torch.tensor([live], dtype=torch.int32, device="cuda")
+        for mask in (None, none):
+            out, lse, w = check(q, kp, vp, k_fp, v_fp, 41, mask, t_fp=cap, t_fp_dev=counter, live=live)
+        assert not out[1].any() and torch.isneginf(lse[1]).all() and not w[0][1].any()
+
+
 @pytest.mark.parametrize("dtype", [HALF, BF16])
 def test_offsets_and_ends_of_the_range(dtype):
     """Keys far from zero beside their spread (several times the group's range), constant groups, large and tiny ones."""
