@@ -25,6 +25,7 @@
 // Taken for granted by neither: a slot or tile as an index instead of a constant costs the issuing lane 104 cycles a product (917 -> 1036 us
 // when the slot became a switch, 676 with constants); a ring of five slots held up the keys (980 -> 945).
 // Every wait is bounded; one that runs out sets CQ_ERR_TIMEOUT in the workspace's first word, and the CTA ends.
+#include <float.h>
 #include <math.h>
 
 #include <type_traits>
@@ -559,7 +560,9 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
         l_run *= alpha;
       }
       if (grow) m_ref = m_true;
-      const float m_use = m_ref == -INFINITY ? 0.f : m_ref, neg = -m_use * factor;
+      // A row that has seen nothing but keys at the type's lowest value has a reference whose multiple may leave fp32's range, and the hidden
+      // keys of a tile without a mask are at -infinity: what is added to those stays finite
+      const float m_use = m_ref == -INFINITY ? 0.f : m_ref, neg = fminf(-m_use * factor, FLT_MAX);
       float rs[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll (IMAGE ? 2 : 1)
       for (int half = 0; half < 2; ++half) {

@@ -1,0 +1,57 @@
+"""Chunk attention and key weights where a tile, a row or a whole block of rows has next to nothing to look at."""
+
+import math
+
+import pytest
+import torch
+
+import chunk_reference as ref
+from test_gpu_chunk import BF16, HALF, check, make
+
+pytestmark = pytest.mark.gpu
+
+
+def lowest_rows(out, v, first, n):
+    """Query i of the first n sees keys ``first`` .. i, all at bfloat16's lowest value: every key counts alike, exactly (the mask's step in fp32 is 2^104,
+    so that scores drown in it; fp16's lowest value has one of 2^-8, and they do not), and the output is a plain mean of values.  Its sum is cut off at 2^-22 of its largest term per 16 keys, then rounded once."""
+    for i in range(n):
+        rows = v[:, :, first:i + 1].cpu().double()
+        rep = out.shape[2] // rows.shape[1]
+        want = rows.mean(2).repeat_interleave(rep, 1)
+        room = torch.finfo(out.dtype).eps / 2 * want.abs() + 2.0 ** -18 * rows.abs().mean(2).repeat_interleave(rep, 1) + torch.finfo(out.dtype).tiny
+        assert ref.within(out[:, i], want, room), i
+
+
+@pytest.mark.parametrize("dtype", [HALF, BF16])
+@pytest.mark.parametrize("shape,masked", [
+    ((16, 32, 8, 20, 0, 246), (0, 246)),          # the even half of the key tiles: one that is masked as a whole, one that ten queries do not see
+    ((6, 16, 4, 28, 1152, 370), (96, 370)),       # behind a visual span, five parts
+    ((40, 8, 4, 33, 1056, 300), (41, 300)),       # a part per half, six key tiles each
+    ((16, 8, 8, 300, 0, 0), (0, 10)),             # left padding: the first queries see nothing but the padding, then a tile they do not see
+    ((16, 8, 8, 300, 0, 129), (0, 129)),
+    ((4, 24, 8, 430, 0, 0), (0, 120)),            # the same with key tiles unpacked once
+], ids=str)
+def test_lowest_masks_in_front_of_hidden_tiles(shape, masked, dtype):
+    """Padding at the type's lowest value (not -inf) in one tile, and a tile without a mask behind it that causality hides."""
+    B, Hq, Hkv, L, t_vis, before = shape
+    q, kp, vp, k_fp, v_fp = make(*shape, dtype, seed=L)
+    t_sys = min(41, before)
+    mask = torch.zeros(B, t_vis + before + L, dtype=dtype, device="cuda")
+    order = torch.cat([torch.arange(t_sys), torch.arange(t_sys + t_vis, t_vis + before + L)])      # places of the full-precision tokens
+    mask[:, order[masked[0]:masked[1]].cuda()] = torch.finfo(dtype).min
+    out, lse, w = check(q, kp, vp, k_fp, v_fp, t_sys, mask)
+    if dtype == BF16 and t_vis == 0 and before == 0:
+        lowest_rows(out, v_fp, 0, masked[1])
+
+
+@pytest.mark.parametrize("dtype", [HALF, BF16])
+def test_lowest_masks_over_everything_old(dtype):
+    """The visual span and the text before the new tokens at the lowest value, the new tokens' own first ones as well."""
+    q, kp, vp, k_fp, v_fp = make(16, 8, 8, 300, 64, 20, dtype, seed=2)
+    mask = torch.zeros(16, 384, dtype=dtype, device="cuda")
+    mask[::2, :84 + 30] = torch.finfo(dtype).min
+    mask[1::2, :84] = -math.inf
+    mask[1::2, 84:84 + 30] = torch.finfo(dtype).min
+    out, lse, _ = check(q, kp, vp, k_fp, v_fp, 20, mask)
+    if dtype == BF16:
+        lowest_rows(out[1::2], v_fp[1::2, :, 20:], 0, 30)
