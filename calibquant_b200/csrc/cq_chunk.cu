@@ -605,9 +605,10 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
     const float nat = MASK ? 1.f : a.scale;         // reference maximum in natural units
     if (a.parts == 1) {
       // the tile's rows through its query tile in shared memory (no product reads that any more), then 16 lanes a row
-      const float inv = l_run > 0.f ? 1.f / l_run : 0.f;
+      const bool bad = l_run != l_run;              // a key or query that is not a number
+      const float inv = bad ? NAN : l_run > 0.f ? 1.f / l_run : 0.f;
       if (ok && valid_row && p.lse)
-        p.lse[((int64_t)b * p.hq + h) * p.q_len + i] = l_run > 0.f ? m_ref * nat + logf(l_run) : -INFINITY;
+        p.lse[((int64_t)b * p.hq + h) * p.q_len + i] = bad ? NAN : l_run > 0.f ? m_ref * nat + logf(l_run) : -INFINITY;
       const uint32_t stage = q_s + (uint32_t)x * TILE_BYTES;
       if (ok) {
 #pragma unroll 1

@@ -55,3 +55,22 @@ def test_lowest_masks_over_everything_old(dtype):
     out, lse, _ = check(q, kp, vp, k_fp, v_fp, 20, mask)
     if dtype == BF16:
         lowest_rows(out[1::2], v_fp[1::2, :, 20:], 0, 30)
+
+
+@pytest.mark.parametrize("masked", [False, True])
+@pytest.mark.parametrize("shape", [(2, 8, 2, 1, 64, 20), (2, 8, 2, 40, 192, 20), (16, 8, 8, 300, 64, 20), (4, 24, 8, 430, 0, 9)], ids=str)
+def test_a_query_that_is_not_a_number(shape, masked):
+    """Its row is NaN in all three results, whatever way the partial results take (few rows, merged parts, one part, images); the others are what they were."""
+    from calibquant_b200 import ops
+    q, kp, vp, k_fp, v_fp = make(*shape, BF16, seed=9)
+    B, Hq, Hkv, L = shape[:4]
+    mask = torch.randn(B, shape[4] + k_fp.shape[2], device="cuda").bfloat16() if masked else None
+    want = ops.chunk_attention(q, kp, vp, k_fp, v_fp, 9, mask=mask, return_lse=True)
+    q[1, L // 2, 3, 5] = math.nan
+    got = ops.chunk_attention(q, kp, vp, k_fp, v_fp, 9, mask=mask, return_lse=True)
+    assert torch.isnan(got[0][1, L // 2, 3]).all() and torch.isnan(got[1][1, 3, L // 2])
+    w = ops.key_weights(q, got[1], kp, k_fp, 9, mask=mask)
+    seen = k_fp.shape[2] - L + L // 2 + 1
+    assert torch.isnan(w[0][1, 3 // (Hq // Hkv)]).all() and torch.isnan(w[1][1, 3 // (Hq // Hkv), :seen]).all()
+    got[0][1, L // 2, 3], got[1][1, 3, L // 2] = want[0][1, L // 2, 3], want[1][1, 3, L // 2]
+    assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
