@@ -597,7 +597,8 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
       }
       l_run += (rs[0] + rs[1]) + (rs[2] + rs[3]);
     }
-    if (n_x > 0 && ok) ok = mbar_wait_bounded(&bar_pv[x], (n_x - 1) & 1, WAIT_TRIES);
+    // without a key tile no product was waited for, and the queries may still be on their way to where the results are staged
+    if (ok) ok = n_x > 0 ? mbar_wait_bounded(&bar_pv[x], (n_x - 1) & 1, WAIT_TRIES) : mbar_wait_bounded(&bar_q, 0, WAIT_TRIES);
     ok = __all_sync(0xffffffffu, ok);
     if (!ok && lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
     tc_fence_after();

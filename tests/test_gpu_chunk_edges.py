@@ -74,3 +74,21 @@ def test_a_query_that_is_not_a_number(shape, masked):
     assert torch.isnan(w[0][1, 3 // (Hq // Hkv)]).all() and torch.isnan(w[1][1, 3 // (Hq // Hkv), :seen]).all()
     got[0][1, L // 2, 3], got[1][1, 3, L // 2] = want[0][1, L // 2, 3], want[1][1, 3, L // 2]
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
+
+
+@pytest.mark.parametrize("dtype", [HALF, BF16])
+@pytest.mark.parametrize("shape", [(16, 8, 8, 300, 0, 0), (4, 24, 8, 430, 0, 0)], ids=str)
+def test_row_blocks_without_a_key(shape, dtype):
+    """Fewer live tokens than new ones and no visual span: whole row blocks of one part see nothing, and give zeros, whatever the queries are."""
+    from calibquant_b200 import ops
+    q, kp, vp, k_fp, v_fp = make(*shape, dtype, seed=7)
+    t_fp = k_fp.shape[2]
+    for live in (20, 1, 0):
+        k_fp[:, :, live:], v_fp[:, :, live:] = math.nan, math.nan
+        counter = torch.tensor([live], dtype=torch.int32, device="cuda")
+        out, lse, w = check(q, kp, vp, k_fp, v_fp, 0, t_fp=t_fp, t_fp_dev=counter, live=live)
+        none = shape[3] - live
+        assert not out[:, :none].any() and torch.isneginf(lse[..., :none]).all()
+        for _ in range(20):
+            again = ops.chunk_attention(q, kp, vp, k_fp, v_fp, 0, t_fp=t_fp, t_fp_dev=counter, return_lse=True)
+            assert torch.equal(again[0], out) and torch.equal(again[1], lse)
