@@ -24,7 +24,8 @@
 // 3328); quarters, or a loop over the warp's two units, gave nothing more.  With images for one row block too: 101.
 // Taken for granted by neither: a slot or tile as an index instead of a constant costs the issuing lane 104 cycles a product (917 -> 1036 us
 // when the slot became a switch, 676 with constants); a ring of five slots held up the keys (980 -> 945).
-// Every wait is bounded; one that runs out sets CQ_ERR_TIMEOUT in the workspace's first word, and the CTA ends.
+// Every wait is bounded; one that runs out sets CQ_ERR_TIMEOUT in the workspace's first word, and the CTA ends once the copies and products that it
+// started have (another bounded wait), with NaN for the rows whose results did not come.
 #include <float.h>
 #include <math.h>
 
@@ -48,7 +49,7 @@ template <bool IMAGE> struct Roles {
   static constexpr int SOFTMAX_REGS = IMAGE ? 184 : 104, CONTROL_REGS = IMAGE ? 128 : 96, PRODUCER_REGS = 88;
 };
 constexpr int SMEM_BYTES = 7 * TILE_BYTES + 1024;
-constexpr uint32_t WAIT_TRIES = 1u << 22;
+constexpr uint32_t WAIT_TRIES = 1u << 22, DRAIN_TRIES = 1u << 16;      // the latter for what is still under way after a wait that ran out
 constexpr long long WAIT_CYCLES = 1ll << 30;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -194,8 +195,8 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
   constexpr int QT = PAIR ? 2 : 1, MMA_WARP = Roles<IMAGE>::MMA_WARP;      // query tiles
   const uint32_t q_s = smem_u32(smem), k_s = q_s + QT * TILE_BYTES, v_s = k_s + 4 * TILE_BYTES;      // keys: [buffer][large terms, small ones]
   // bar_q (once); bar_k / bar_v[buffer] full, bar_kfree / bar_vfree read; bar_s[X] scores of X ready; bar_p[X][half] probabilities of keys 0-63 / 64-127 stored;
-  // bar_pv[X] the tile's P V done
-  __shared__ __align__(8) uint64_t bar_q, bar_k[2], bar_kfree[2], bar_v[2], bar_vfree[2], bar_s[2], bar_p[2][2], bar_pv[2];
+  // bar_pv[X] the tile's P V done; bar_end all products done
+  __shared__ __align__(8) uint64_t bar_q, bar_k[2], bar_kfree[2], bar_v[2], bar_vfree[2], bar_s[2], bar_p[2][2], bar_pv[2], bar_end;
   __shared__ uint32_t tmem_base_s;
   __shared__ __align__(16) T mask_s[MASK ? 2 : 1][MASK ? 2 : 1][MASK ? 128 : 8];
 
@@ -216,6 +217,7 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
       mbar_init(&bar_p[x][1], 128);
       mbar_init(&bar_pv[x], 1);
     }
+    mbar_init(&bar_end, 1);
     mbar_fence_init();
   }
   pdl_launch_dependents();
@@ -437,7 +439,12 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
         step(C1{}, j + 1);
       }
     }
-    if (!ok && lead) atomicExch(a.status, CQ_ERR_TIMEOUT);
+    commit(&bar_end);
+    ok = all(mbar_wait_bounded(&bar_end, 0, ok ? WAIT_TRIES : DRAIN_TRIES)) && ok;
+    if (!ok) {
+      mbar_wait_bounded(&bar_q, 0, DRAIN_TRIES);
+      if (lead) atomicExch(a.status, CQ_ERR_TIMEOUT);
+    }
     __syncwarp();
     } else if (IMAGE && warp == MMA_WARP + 1) {
       // ================= operands from the images =================
@@ -445,6 +452,7 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
       if (lane == 0) {
         const unsigned char* src = a.image + bh * image_bytes(k.nv, a.image_fp_tiles);
         bool ok = true;
+        int ks = 0, vs = 0;                       // loads requested
         const auto load_k = [&](int j) {
           if (j >= k.n || !ok) return;
           const int tile = k.t0 + j, buf = j & 1;
@@ -453,6 +461,7 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
           const uint32_t bytes = (tile < k.nv ? 2 : 1) * TILE_BYTES;
           mbar_expect_tx(&bar_k[buf], bytes);
           bulk_load_1d(smem + (QT + 2 * buf) * TILE_BYTES, src + (tile < k.nv ? (size_t)tile * 3 * TILE_BYTES : image_bytes(k.nv, tile - k.nv)), bytes, &bar_k[buf]);
+          ks = j + 1;
         };
         load_k(0);
         for (int j = 0; j < k.n && ok; ++j) {
@@ -463,7 +472,12 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
           mbar_expect_tx(&bar_v[0], TILE_BYTES);
           bulk_load_1d(smem + (QT + 4) * TILE_BYTES, src + (tile < k.nv ? (size_t)(3 * tile + 2) * TILE_BYTES : image_bytes(k.nv, tile - k.nv) + TILE_BYTES),
                        TILE_BYTES, &bar_v[0]);
+          vs = j + 1;
         }
+        // whoever reads them may have given up: the last ones have to be there before the CTA ends
+        const auto arrived = [&](uint64_t* bar, int use) { ok = mbar_wait_bounded(bar, use & 1, ok ? WAIT_TRIES : DRAIN_TRIES) && ok; };
+        for (int j = max(0, ks - 2); j < ks; ++j) arrived(&bar_k[j & 1], j >> 1);
+        if (vs > 0) arrived(&bar_v[0], vs - 1);
         if (!ok) atomicExch(a.status, CQ_ERR_TIMEOUT);
       }
       __syncwarp();
@@ -600,39 +614,40 @@ __global__ void __launch_bounds__(Roles<IMAGE>::THREADS, 1) chunk_attn_kernel(co
     // without a key tile no product was waited for, and the queries may still be on their way to where the results are staged
     if (ok) ok = n_x > 0 ? mbar_wait_bounded(&bar_pv[x], (n_x - 1) & 1, WAIT_TRIES) : mbar_wait_bounded(&bar_q, 0, WAIT_TRIES);
     ok = __all_sync(0xffffffffu, ok);
-    if (!ok && lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
+    if (!ok) {
+      mbar_wait_bounded(&bar_q, 0, DRAIN_TRIES);
+      if (lane == 0) atomicExch(a.status, CQ_ERR_TIMEOUT);
+    }
     tc_fence_after();
     const int h = hk * p.n_rep + r_in - i_in * p.n_rep;
     const float nat = MASK ? 1.f : a.scale;         // reference maximum in natural units
     if (a.parts == 1) {
       // the tile's rows through its query tile in shared memory (no product reads that any more), then 16 lanes a row
-      const bool bad = l_run != l_run;              // a key or query that is not a number
+      const bool bad = !ok || l_run != l_run;       // no result, or a key or query that is not a number
       const float inv = bad ? NAN : l_run > 0.f ? 1.f / l_run : 0.f;
-      if (ok && valid_row && p.lse)
-        p.lse[((int64_t)b * p.hq + h) * p.q_len + i] = bad ? NAN : l_run > 0.f ? m_ref * nat + logf(l_run) : -INFINITY;
+      if (valid_row && p.lse) p.lse[((int64_t)b * p.hq + h) * p.q_len + i] = bad ? NAN : l_run > 0.f ? m_ref * nat + logf(l_run) : -INFINITY;
       const uint32_t stage = q_s + (uint32_t)x * TILE_BYTES;
-      if (ok) {
+      const bool sums = n_x > 0 && ok;
 #pragma unroll 1
-        for (int cc = 0; cc < 4; ++cc) {
-          uint32_t r[32];
-          if (n_x > 0) tmem_ld32(tO + cc * 32, r);
+      for (int cc = 0; cc < 4; ++cc) {
+        uint32_t r[32];
+        if (sums) tmem_ld32(tO + cc * 32, r);
 #pragma unroll
-          for (int c = 0; c < 32; ++c) r[c] = n_x > 0 ? __float_as_uint(__uint_as_float(r[c]) * inv) : 0u;
+        for (int c = 0; c < 32; ++c) r[c] = __float_as_uint(sums ? __uint_as_float(r[c]) * inv : inv);
 #pragma unroll
-          for (int c = 0; c < 32; c += 8) {         // columns 0 4 1 5 2 6 3 7 of eight channels
-            const auto f = [&](int e) { return __uint_as_float(r[c + e]); };
-            sts128(chunk_at(stage, r_in, cc * 4 + (c >> 3)), pack16<BF16>(f(0), f(2)), pack16<BF16>(f(4), f(6)), pack16<BF16>(f(1), f(3)),
-                   pack16<BF16>(f(5), f(7)));
-          }
+        for (int c = 0; c < 32; c += 8) {           // columns 0 4 1 5 2 6 3 7 of eight channels
+          const auto f = [&](int e) { return __uint_as_float(r[c + e]); };
+          sts128(chunk_at(stage, r_in, cc * 4 + (c >> 3)), pack16<BF16>(f(0), f(2)), pack16<BF16>(f(4), f(6)), pack16<BF16>(f(1), f(3)),
+                 pack16<BF16>(f(5), f(7)));
         }
-        __syncwarp();
-        for (int it = 0; it < 16; ++it) {
-          const int rr = quarter * 32 + it * 2 + (lane >> 4), ii = rr / p.n_rep;
-          if (rr < a.tile_rows && q_first + ii < p.q_len) {
-            const uint4 v = lds128(chunk_at(stage, rr, lane & 15));
-            T* dst = static_cast<T*>(p.out) + b * p.o_sb + (int64_t)(q_first + ii) * p.o_st + (int64_t)(hk * p.n_rep + rr - ii * p.n_rep) * p.o_sh;
-            *reinterpret_cast<uint4*>(dst + (lane & 15) * 8) = v;
-          }
+      }
+      __syncwarp();
+      for (int it = 0; it < 16; ++it) {
+        const int rr = quarter * 32 + it * 2 + (lane >> 4), ii = rr / p.n_rep;
+        if (rr < a.tile_rows && q_first + ii < p.q_len) {
+          const uint4 v = lds128(chunk_at(stage, rr, lane & 15));
+          T* dst = static_cast<T*>(p.out) + b * p.o_sb + (int64_t)(q_first + ii) * p.o_st + (int64_t)(hk * p.n_rep + rr - ii * p.n_rep) * p.o_sh;
+          *reinterpret_cast<uint4*>(dst + (lane & 15) * 8) = v;
         }
       }
     } else if (__any_sync(0xffffffffu, valid_row)) {

@@ -37,7 +37,7 @@ namespace kw {
 constexpr int WORKERS = 16, MMA_WARP = 16, TMA_WARP = 17, THREADS = 18 * 32;
 constexpr int LSE_BLOCKS = 16;             // blocks whose rows' log-sum-exp are in shared memory at a time
 constexpr int SMEM_BYTES = 6 * TILE_BYTES + 1024;
-constexpr uint32_t WAIT_TRIES = 1u << 22;
+constexpr uint32_t WAIT_TRIES = 1u << 22, DRAIN_TRIES = 1u << 16;      // the latter for what is still under way after a wait that ran out
 constexpr long long WAIT_CYCLES = 1ll << 30;
 constexpr float LOG2E = 1.4426950408889634f;
 
@@ -78,8 +78,8 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
   extern __shared__ unsigned char smem_raw[];
   unsigned char* smem = smem_raw + ((1024u - (smem_u32(smem_raw) & 1023u)) & 1023u);
   const uint32_t k_s = smem_u32(smem), q_s = k_s + 4 * TILE_BYTES;      // key tiles [X][hi, lo], query slots
-  // bar_k the key tiles are there; bar_q/free[slot] query blocks; bar_d/dfree[X][buffer] scores ready / read
-  __shared__ __align__(8) uint64_t bar_k, bar_q[2], bar_free[2], bar_d[2][2], bar_dfree[2][2];
+  // bar_k the key tiles are there; bar_q/free[slot] query blocks; bar_d/dfree[X][buffer] scores ready / read; bar_end all products done
+  __shared__ __align__(8) uint64_t bar_k, bar_q[2], bar_free[2], bar_d[2][2], bar_dfree[2][2], bar_end;
   __shared__ uint32_t tmem_base_s;
   __shared__ __align__(16) float lse_s[2][LSE_BLOCKS * NB];
   __shared__ float half_s[256];
@@ -103,6 +103,7 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
 
   if (tid == 0) {
     mbar_init(&bar_k, WORKERS);
+    mbar_init(&bar_end, 1);
     for (int s = 0; s < 2; ++s) {
       mbar_init(&bar_q[s], 1);
       mbar_init(&bar_free[s], 1);
@@ -123,7 +124,8 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
     // ================= query blocks =================
     if (lane == 0) {
       bool ok = true;
-      for (int n = 0; n < nb && ok; ++n) {
+      int n = 0;
+      for (; n < nb; ++n) {
         const int s = n & 1;
         // rows of a block that no query fills are zeros for good: written before bar_k
         if (n >= 2) ok = mbar_wait_bounded(&bar_free[s], ((n >> 1) - 1) & 1, WAIT_TRIES);
@@ -133,6 +135,8 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
         tma_load_4d(q_s + s * TILE_BYTES, &tm_q, 0, hk * p.n_rep, i0, b, &bar_q[s]);
         tma_load_4d(q_s + s * TILE_BYTES + PANEL_BYTES, &tm_q, 64, hk * p.n_rep, i0, b, &bar_q[s]);
       }
+      // whoever reads them may have given up: the last two blocks have to be there before the CTA ends
+      for (int m = max(0, n - 2); m < n; ++m) ok = mbar_wait_bounded(&bar_q[m & 1], (m >> 1) & 1, ok ? WAIT_TRIES : DRAIN_TRIES) && ok;
       if (!ok) atomicExch(a.status, CQ_ERR_TIMEOUT);
     }
     __syncwarp();
@@ -190,6 +194,8 @@ __global__ void __launch_bounds__(THREADS, 1) key_weights_kernel(const __grid_co
       block(std::integral_constant<int, 0>{}, n);
       if (n + 1 < nb && ok) block(std::integral_constant<int, 1>{}, n + 1);
     }
+    if (lead) umma_commit(&bar_end);
+    ok = all(mbar_wait_bounded(&bar_end, 0, ok ? WAIT_TRIES : DRAIN_TRIES)) && ok;
     if (!ok && lead) atomicExch(a.status, CQ_ERR_TIMEOUT);
     __syncwarp();
   } else {
