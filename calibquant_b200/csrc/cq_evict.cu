@@ -284,7 +284,9 @@ static int slices(int64_t rows, int64_t bytes) {
 
 template <typename... K, typename... A>
 static int run(void (*kern)(K...), dim3 grid, size_t smem, cudaStream_t st, A... args) {
-  if (smem > 48 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM) != cudaSuccess) {
+  // 48 KB need not be asked for, of which the kernels' own variables (Shared, above 1 KB) take their part
+  static_assert(sizeof(Shared) <= 2048, "what is left of 48 KB");
+  if (smem > 46 * 1024 && cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, MAX_SMEM) != cudaSuccess) {
     (void)cudaGetLastError();
     return CQ_ERR_LAUNCH;
   }
