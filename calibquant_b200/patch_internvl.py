@@ -320,35 +320,40 @@ def evict_cache(model, keep_groups=None, keep_tokens=None, recent=32):
     """Drop from the cache of every layer and KV head what ``track_key_weights`` saw the least attention on: all but ``keep_groups`` groups of 32
     visual tokens and / or all but ``keep_tokens`` full-precision tokens, of which the system prompt's and the last
     ``recent`` always stay.  Positions are those of the tokens as they were.  Returns the layers' new ``past_key_values``."""
-    layers, past = _attentions(model), []
-    for attn in layers:      # of the layers none is changed before all may be
-        tc = attn._text_cache
+    layers = _attentions(model)
+    for attn in layers:
         if getattr(attn, "_key_weights", None) is None:
             raise ValueError("no key weights: track_key_weights has to be on while the cache is used")
         if getattr(attn, "_static_decode", False):
             raise ValueError("the cache of a captured decoder stays where it is: close the decoder first")
+        tc = attn._text_cache
         t_sys = min(attn.sprompt_len, tc.length) if LOW_BITS else 0
         if keep_groups is not None and attn.k_pack is not None and not 0 < keep_groups <= attn.k_pack[1].shape[3]:
             raise ValueError(f"keep_groups must be between 1 and the {attn.k_pack[1].shape[3]} groups there are, not {keep_groups}")
         if keep_tokens is not None and not (0 < keep_tokens <= tc.length and 0 <= recent <= keep_tokens - t_sys):
             raise ValueError(f"keep_tokens must hold the {t_sys} system and the last {recent} tokens and be no more than the {tc.length} there are, "
                              f"but is {keep_tokens}")
+    # What may still fail (sizes beyond the kernels', memory) does so before a layer is changed
+    kept = []
     for attn in layers:
         tc, (w_vis, w_fp) = attn._text_cache, attn._key_weights
+        new = {}
         if keep_groups is not None and attn.k_pack is not None:
-            attn.k_pack, attn.v_pack, w_vis, _ = ops.evict_groups(attn.k_pack, attn.v_pack, w_vis, keep_groups, bits=BITS_KV)
-            attn._keys_differ = True
+            new["k_pack"], new["v_pack"], w_vis, _ = ops.evict_groups(attn.k_pack, attn.v_pack, w_vis, keep_groups, bits=BITS_KV)
+            new["_keys_differ"] = True
         if keep_tokens is not None:
             t_sys = min(attn.sprompt_len, tc.length) if LOW_BITS else 0
             k, v, kept_w, _ = ops.evict_tokens(tc.k, tc.v, w_fp, keep_tokens, t_sys=t_sys, recent=recent, t_fp=tc.length)
-            attn._evicted += tc.length - keep_tokens
-            attn._keys_differ = True
-            attn._text_cache = tc = _TextCache(k, v)
+            new["_evicted"] = attn._evicted + tc.length - keep_tokens
+            new["_keys_differ"] = True
+            new["_text_cache"] = tc = _TextCache(k, v)
             w_fp = torch.zeros((*tc.k.shape[:3],), dtype=torch.float32, device=k.device)
             w_fp[:, :, :keep_tokens] = kept_w
-        attn._key_weights = (w_vis, w_fp)
-        past.append(tc.views())
-    return past
+        new["_key_weights"] = (w_vis, w_fp)
+        kept.append((new, tc.views()))
+    for attn, (new, _) in zip(layers, kept):
+        attn.__dict__.update(new)
+    return [views for _, views in kept]
 
 
 def forward_internlm2_calibquant(self, hidden_states: torch.Tensor,

@@ -1,0 +1,36 @@
+"""What the patched model refuses in a conversation, or fails at, leaves its caches and weights as they were."""
+
+import pytest
+import torch
+
+from test_gpu_chat import SYS, VIS, build, embeds, four_bits, positions, prompt      # noqa: F401 (four_bits: a fixture)
+
+pytestmark = pytest.mark.gpu
+
+
+def attentions(shell):
+    return [layer.attention for layer in shell.language_model.model.layers]
+
+
+def state(shell):
+    return [(a.k_pack, a.v_pack, a._text_cache, a._text_cache.length, a._key_weights, a._evicted, a._keys_differ) for a in attentions(shell)]
+
+
+def same(a, b):
+    return all(x is y or isinstance(x, (int, bool)) and x == y for s, t in zip(a, b) for x, y in zip(s, t))
+
+
+def test_an_eviction_beyond_the_kernels_sizes():
+    """More full-precision tokens than can be ranked: the groups of no layer are dropped either, and the conversation goes on."""
+    from calibquant_b200 import patch_internvl as pi
+    shell = build()
+    pi.track_key_weights(shell)
+    lm, n = shell.language_model, 24577 - SYS
+    (_, past), at = prompt(shell, B=1, text=n)
+    before = state(shell)
+    with pytest.raises((ValueError, RuntimeError)):
+        pi.evict_cache(shell, keep_groups=1, keep_tokens=SYS + 100)
+    assert same(state(shell), before)
+    _, past = lm.forward_step(embeds(1, 3, shell, 5), positions(1, at, 3), past)
+    past = pi.evict_cache(shell, keep_groups=1)
+    assert past[1][0].shape[2] == SYS + n + 3 and all(a.k_pack[1].shape[3] == 1 for a in attentions(shell))
