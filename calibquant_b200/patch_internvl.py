@@ -291,11 +291,12 @@ def _forward_chunk(self, hidden_states, attention_mask, position_ids, past_key_v
         position_ids = torch.arange(kv_seq_len - q_len, kv_seq_len, device=hidden_states.device).expand(bsz, q_len)
     tc.reserve(q_len)
     q, _, _ = ops.prefill_rope_split(self.wqkv(hidden_states), cos, sin, position_ids, n_kv, n_rep, tc.k[:, :, tc.length:], tc.v[:, :, tc.length:])
-    tc.length += q_len
+    t_fp = tc.length + q_len
     if getattr(self, "_track_weights", False):
-        attn = _attend_tracked(self, q, tc.length, mask=mask)
+        attn = _attend_tracked(self, q, t_fp, mask=mask)
     else:
-        attn = ops.chunk_attention(q, k_pack, v_pack, tc.k, tc.v, self.sprompt_len if LOW_BITS else 0, mask=mask, t_fp=tc.length)
+        attn = ops.chunk_attention(q, k_pack, v_pack, tc.k, tc.v, self.sprompt_len if LOW_BITS else 0, mask=mask, t_fp=t_fp)
+    tc.length = t_fp      # a call that was refused has appended nothing
     attn = _gather_heads(self, attn.reshape(bsz, q_len, -1))
     return self.wo(attn), None, tc.views() if use_cache else None
 

@@ -34,3 +34,18 @@ def test_an_eviction_beyond_the_kernels_sizes():
     _, past = lm.forward_step(embeds(1, 3, shell, 5), positions(1, at, 3), past)
     past = pi.evict_cache(shell, keep_groups=1)
     assert past[1][0].shape[2] == SYS + n + 3 and all(a.k_pack[1].shape[3] == 1 for a in attentions(shell))
+
+
+@pytest.mark.parametrize("tracked", [False, True])
+def test_a_chunk_that_is_refused_appends_nothing(tracked):
+    from calibquant_b200 import patch_internvl as pi
+    shell = build()
+    pi.track_key_weights(shell, tracked)
+    (_, past), at = prompt(shell)
+    before, attn = state(shell), attentions(shell)[0]
+    x = embeds(2, 5, shell, 1)
+    with pytest.raises((RuntimeError, ValueError)):      # a mask that is not on the GPU
+        attn(x, attention_mask=torch.zeros(2, 1, 5, at + 5), position_ids=positions(2, at, 5), past_key_value=past[0])
+    assert same(state(shell), before)
+    want, _, views = attn(x, position_ids=positions(2, at, 5), past_key_value=past[0], use_cache=True)
+    assert views[0].shape[2] == SYS + 25 and torch.isfinite(want.float()).all()
