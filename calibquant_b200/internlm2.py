@@ -267,6 +267,11 @@ class GraphedDecoder:
         dev = first_token.device
         self.caches = [layer.attention._text_cache for layer in lm.model.layers]
         self.len_dev = torch.tensor([self.caches[0].length], dtype=torch.int32, device=dev)
+        tracked = [layer.attention for layer in lm.model.layers if getattr(layer.attention, "_track_weights", False)]
+        if tracked:
+            from .patch_internvl import _chunk_cache
+            for a in tracked:             # refused before a layer is set up for the graph
+                _chunk_cache(a)
         for layer, tc in zip(lm.model.layers, self.caches):
             assert tc.length == self.caches[0].length
             tc.enable_static(tc.length + max_new_tokens + 2, self.len_dev)
@@ -277,7 +282,6 @@ class GraphedDecoder:
         self.out = torch.zeros((max_new_tokens + 2, B), device=dev, dtype=torch.long)
         self.step_idx = torch.zeros(1, device=dev, dtype=torch.long)
         state0 = (self.tok.clone(), self.caches[0].length)
-        tracked = [layer.attention for layer in lm.model.layers if getattr(layer.attention, "_track_weights", False)]
         weights0 = [None if a._key_weights is None else tuple(t.clone() for t in a._key_weights) for a in tracked]
         side = torch.cuda.Stream()
         side.wait_stream(torch.cuda.current_stream())

@@ -383,6 +383,14 @@ def forward_internlm2_calibquant(self, hidden_states: torch.Tensor,
         attention_mask = _pop_padding_mask(kwargs, attention_mask)
     bsz, q_len, _ = hidden_states.size()
 
+    tracked = getattr(self, "_track_weights", False)
+    if tracked:      # before anything is appended or replaced
+        if q_len > 1 and past_key_value is None:
+            if LOW_BITS and (KV_FORMAT == "uint8" or BITS_KV != 4 and self.image_token_num):
+                raise NotImplementedError(f"tracked weights: the group format with 4 bits only, not {KV_FORMAT} with {BITS_KV}")
+        else:
+            _chunk_cache(self)
+
     if q_len == 1 and getattr(self, "_static_decode", False):
         # graph-replayable step: everything that changes between steps is read from device memory.
         # One launch splits the projection, rotates q and k and appends k, v at the device-side
@@ -394,7 +402,7 @@ def forward_internlm2_calibquant(self, hidden_states: torch.Tensor,
         q = ops.rope_split_append(self.wqkv(hidden_states), cos, sin, position_ids,
                                   self.wqkv.out_features // ((n_rep + 2) * self.head_dim), n_rep,
                                   tc.k, tc.v, t_fp_dev=tc.len_dev)
-        if getattr(self, "_track_weights", False):
+        if tracked:
             attn = _attend_tracked(self, q.transpose(1, 2), tc.k.shape[2], t_fp_dev=tc.len_dev).transpose(1, 2)
         elif getattr(self, "_u8_state", None) is not None:
             from . import calibquant as _cq
@@ -439,7 +447,7 @@ def forward_internlm2_calibquant(self, hidden_states: torch.Tensor,
         state["_key_weights"], state["_evicted"], state["_keys_differ"] = None, 0, False      # _evicted: full-precision tokens
         past_key_value = tc.views() if use_cache else None
         attn = ops.prefill_attention(q, k, v)
-        if getattr(self, "_track_weights", False) and q_len > s0 + n_vis:
+        if tracked and q_len > s0 + n_vis:
             _attend_tracked(self, q[:, s0 + n_vis:], tc.length)      # the question's own look at the cache
         attn = _gather_heads(self, attn.reshape(bsz, q_len, -1))
         attn_output = self.wo(attn.reshape(bsz, q_len, -1))
@@ -476,7 +484,7 @@ def forward_internlm2_calibquant(self, hidden_states: torch.Tensor,
         raise ValueError(f"Attention mask should be of size {(bsz, 1, q_len, kv_seq_len)}, "
                          f"but is {attention_mask.size()}")
     t_sys = self.sprompt_len if LOW_BITS else 0
-    if getattr(self, "_track_weights", False):
+    if tracked:
         attn = _attend_tracked(self, q.transpose(1, 2), tc.length, mask=attention_mask).transpose(1, 2)
     elif getattr(self, "_u8_state", None) is not None:
         from . import calibquant as _cq

@@ -49,3 +49,33 @@ def test_a_chunk_that_is_refused_appends_nothing(tracked):
     assert same(state(shell), before)
     want, _, views = attn(x, position_ids=positions(2, at, 5), past_key_value=past[0], use_cache=True)
     assert views[0].shape[2] == SYS + 25 and torch.isfinite(want.float()).all()
+
+
+@pytest.mark.parametrize("fmt,bits", [("group", 1), ("group", 2), ("uint8", 4), ("uint8", 2)])
+def test_tracking_at_other_widths_changes_nothing(fmt, bits, monkeypatch):
+    """Prompt, single tokens, several at once and the captured decoder are refused before a cache is replaced or appended to; without tracking they go on."""
+    from calibquant_b200 import internlm2, patch_internvl as pi
+    shell = build()
+    lm = shell.language_model
+    (_, past), at = prompt(shell)                     # 4 bits
+    before = state(shell)
+    monkeypatch.setattr(pi, "KV_FORMAT", fmt)
+    monkeypatch.setattr(pi, "BITS_KV", bits)
+    pi.track_key_weights(shell)
+    with pytest.raises(NotImplementedError):
+        prompt(shell)
+    assert same(state(shell), before)
+    pi.track_key_weights(shell, False)
+    (logits, past), at = prompt(shell)
+    one, tok = embeds(2, 1, shell, 1), logits[:, -1].argmax(-1)
+    before, u8 = state(shell), [a._u8_state for a in attentions(shell)]
+    pi.track_key_weights(shell)
+    for call in (lambda: lm.forward_step(one, positions(2, at, 1), past), lambda: internlm2.GraphedDecoder(lm, past, tok, at, 8)):
+        with pytest.raises(NotImplementedError):
+            call()
+        assert same(state(shell), before) and all(a._u8_state is u for a, u in zip(attentions(shell), u8))
+    pi.track_key_weights(shell, False)
+    with pytest.raises(NotImplementedError):
+        lm.forward_step(embeds(2, 3, shell, 1), positions(2, at, 3), past)
+    out, past = lm.forward_step(one, positions(2, at, 1), past)
+    assert past[0][0].shape[2] == SYS + 21 and torch.isfinite(out.float()).all()
