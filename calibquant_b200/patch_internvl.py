@@ -341,12 +341,12 @@ def evict_cache(model, keep_groups=None, keep_tokens=None, recent=32):
         new = {}
         if keep_groups is not None and attn.k_pack is not None:
             new["k_pack"], new["v_pack"], w_vis, _ = ops.evict_groups(attn.k_pack, attn.v_pack, w_vis, keep_groups, bits=BITS_KV)
-            new["_keys_differ"] = True
+            new["_keys_differ"] = attn._keys_differ or keep_groups < attn.k_pack[1].shape[3]
         if keep_tokens is not None:
             t_sys = min(attn.sprompt_len, tc.length) if LOW_BITS else 0
             k, v, kept_w, _ = ops.evict_tokens(tc.k, tc.v, w_fp, keep_tokens, t_sys=t_sys, recent=recent, t_fp=tc.length)
             new["_evicted"] = attn._evicted + tc.length - keep_tokens
-            new["_keys_differ"] = True
+            new["_keys_differ"] = new.get("_keys_differ", attn._keys_differ) or keep_tokens < tc.length
             new["_text_cache"] = tc = _TextCache(k, v)
             w_fp = torch.zeros((*tc.k.shape[:3],), dtype=torch.float32, device=k.device)
             w_fp[:, :, :keep_tokens] = kept_w

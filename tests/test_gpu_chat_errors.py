@@ -79,3 +79,26 @@ def test_tracking_at_other_widths_changes_nothing(fmt, bits, monkeypatch):
         lm.forward_step(embeds(2, 3, shell, 1), positions(2, at, 3), past)
     out, past = lm.forward_step(one, positions(2, at, 1), past)
     assert past[0][0].shape[2] == SYS + 21 and torch.isfinite(out.float()).all()
+
+
+def test_masks_after_an_eviction():
+    """Masks over keys go on as long as all keys are there, in their order; once some are dropped they are refused, whatever is kept later."""
+    from calibquant_b200 import patch_internvl as pi
+    shell = build()
+    pi.track_key_weights(shell)
+    (_, past), at = prompt(shell)
+    attn = attentions(shell)[0]
+    x, mask = embeds(2, 5, shell, 1), torch.zeros(2, 1, 5, at + 5, device="cuda")
+    past = pi.evict_cache(shell, keep_groups=VIS // 32, keep_tokens=SYS + 20, recent=9)      # all of them
+    out, _, views = attn(x, attention_mask=mask, position_ids=positions(2, at, 5), past_key_value=past[0], use_cache=True)
+    assert torch.isfinite(out.float()).all() and views[0].shape[2] == SYS + 25
+    one = torch.zeros(2, 1, 1, at + 6, device="cuda")
+    _, _, views = attn(x[:, :1], attention_mask=one, position_ids=positions(2, at + 5, 1), past_key_value=views, use_cache=True)
+    (_, past), at = prompt(shell)
+    for kw in (dict(keep_tokens=SYS + 19, recent=9), dict(keep_groups=VIS // 32), dict(keep_tokens=SYS + 19, recent=9)):
+        past = pi.evict_cache(shell, **kw)
+        with pytest.raises(ValueError):
+            attn(x, attention_mask=mask, position_ids=positions(2, at, 5), past_key_value=past[0])
+        with pytest.raises(ValueError):
+            attn(x[:, :1], attention_mask=one[..., :at + 1], position_ids=positions(2, at, 1), past_key_value=past[0])
+    assert attn._text_cache.length == SYS + 19
