@@ -3,9 +3,10 @@
 //
 // A CTA goes over tiles of eight groups of 32 keys, a group for each of its eight warps.  Keys are the M side, query rows the N side (NT blocks of eight):
 //   S^T = K Q^T       A = codes (16 keys x 16 channels, pairs along the channels), exact as they are; B = query * scale, which changes with
-//                     the group and is exact as the sum of two 16-bit numbers (the product rounded, and what an fma finds
-//                     missing); the minima come in as a product of their own.  fp16 queries are scaled by a power of two per
-//                     row, so that the products stay in range.
+//                     the group and is the sum of two 16-bit numbers (the product rounded, and what an fma finds missing);
+//                     the minima come in as a product of their own.  In bfloat16 that is exact.  In fp16 the queries are scaled by a power of
+//                     two per row and the scales by one per group: what is lost is below 2^-24, where the largest product of a row and group
+//                     lies between 2^13 and 2^15 (2^8 at least where all of a group's scales are below 2^-9, but not subnormal).
 //   O^T += V^T P^T    A = values (16 channels x 16 keys, pairs along the keys), scale * code + minimum rounded once; B = probabilities,
 //                     transposed from the layout of S^T by movmatrix.
 // Which key (channel) a lane's row of A is, is free to choose: lane (g, c) takes the codes of word g % 4 of its group, the lower or the
@@ -35,6 +36,7 @@ using namespace ptx;
 
 constexpr int WARPS = 8, THREADS = WARPS * 32;
 constexpr float LOG2E = 1.4426950408889634f, SCALE = 0.08838834764831845f;
+constexpr int Q_LOG2 = 7, SCALE_LOG2 = 6;      // fp16: the largest of a row's queries lies in [2^7, 2^8), of a group's scales in [2^6, 2^7)
 
 __device__ __forceinline__ float ex2_approx(float x) {
   float y;
@@ -46,6 +48,17 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   uint32_t r;
   if (BF16) asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
   else asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+  return r;
+}
+// of fp16 pairs
+__device__ __forceinline__ uint32_t hmul2(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("mul.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a), "r"(b));
+  return r;
+}
+__device__ __forceinline__ uint32_t hmax2_abs(uint32_t a, uint32_t b) {
+  uint32_t r;
+  asm("max.f16x2 %0, %1, %2;" : "=r"(r) : "r"(a & 0x7fff7fffu), "r"(b & 0x7fff7fffu));
   return r;
 }
 template <bool BF16>
@@ -104,7 +117,6 @@ struct __align__(1024) Stage {
 struct __align__(1024) KeyStage {
   uint32_t k[128][32];
 };
-template <bool WEIGHTS> using StageOf = typename std::conditional<WEIGHTS, KeyStage, Stage>::type;
 // Scales and minima of a tile's keys: [scale, minimum][group][channel]
 struct __align__(16) Scales {
   uint16_t x[2][8][128];
@@ -160,7 +172,7 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
         }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      const int exponent = top > 0.f && top < INFINITY ? ilogbf(top) : 0;      // -24 .. 15
+      const int exponent = top > 0.f && top < INFINITY ? max(ilogbf(top) - Q_LOG2, -30) : 0;      // -30 .. 8
       const __half down = __float2half_rn(exp2f((float)-(exponent / 2))), down2 = __float2half_rn(exp2f((float)-(exponent - exponent / 2)));
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks)
@@ -298,6 +310,17 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
 #pragma unroll
         for (int e = 0; e < 4; ++e) s[mb][nt][e] = small[mb][nt][e] = 0.f;
     if (vis) {
+      // fp16: the group's scales times a power of two, so that the products are as far from either end of the range as they can be
+      uint32_t up2 = 0;
+      float down = 1.f;
+      if (!BF16) {
+        const uint32_t x = hmax2_abs(sc_s[warp][lane], sc_s[warp][lane + 32]);
+        const int field = (int)(__reduce_max_sync(0xffffffffu, max(x & 0xffffu, x >> 16)) >> 10);      // 2^(field - 15), or below 2^-14
+        const int k = min(SCALE_LOG2 + 15 - field, 15);                                                // -10 .. 15
+        up2 = (uint32_t)(k + 15) << 10;
+        up2 |= up2 << 16;
+        down = __uint_as_float((uint32_t)(127 - k) << 23);
+      }
       float minima[NT][4];                      // the same in every row
 #pragma unroll
       for (int nt = 0; nt < NT; ++nt)
@@ -305,7 +328,11 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
         for (int e = 0; e < 4; ++e) minima[nt][e] = 0.f;
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) {
-        const uint32_t s2[2] = {sc_s[warp][ks * 8 + c], sc_s[warp][ks * 8 + c + 4]};
+        uint32_t s2[2] = {sc_s[warp][ks * 8 + c], sc_s[warp][ks * 8 + c + 4]};
+        if (!BF16) {
+          s2[0] = hmul2(s2[0], up2);
+          s2[1] = hmul2(s2[1], up2);
+        }
         const int row = ks * 16 + 2 * c, quad = (warp ^ (2 * c)) * 4 + (g & 3), quad1 = quad ^ 4;
         const uint32_t za = prmt(st.k[row][quad], st.k[row + 1][quad1], half_sel), zb = prmt(st.k[row + 8][quad], st.k[row + 9][quad1], half_sel);
         uint32_t hi[NT][2], lo[NT][2];
@@ -337,8 +364,13 @@ __global__ void __launch_bounds__(THREADS, NT == 1 || WEIGHTS ? 2 : 1) few_kerne
           const float own = minima[nt][e];
 #pragma unroll
           for (int mb = 0; mb < 2; ++mb) {
-            s[mb][nt][e] += small[mb][nt][e] + own;
-            s[mb][nt][e + 2] += small[mb][nt][e + 2] + own;
+            if (BF16) {
+              s[mb][nt][e] += small[mb][nt][e] + own;
+              s[mb][nt][e + 2] += small[mb][nt][e + 2] + own;
+            } else {
+              s[mb][nt][e] = fmaf(s[mb][nt][e] + small[mb][nt][e], down, own);
+              s[mb][nt][e + 2] = fmaf(s[mb][nt][e + 2] + small[mb][nt][e + 2], down, own);
+            }
           }
         }
     } else if (there > 0) {

@@ -92,3 +92,39 @@ def test_row_blocks_without_a_key(shape, dtype):
         for _ in range(20):
             again = ops.chunk_attention(q, kp, vp, k_fp, v_fp, 0, t_fp=t_fp, t_fp_dev=counter, return_lse=True)
             assert torch.equal(again[0], out) and torch.equal(again[1], lse)
+
+
+def sized(B, Hq, Hkv, L, t_vis, before, dtype, key, query, seed=0):
+    """Inputs whose keys are of size ``key`` (channels lognormal about it) and queries of size ``query``."""
+    from calibquant_b200 import ops
+    g = torch.Generator().manual_seed(seed)
+    rnd = lambda *s: torch.randn(*s, generator=g)
+    f = torch.exp(rnd(128)) * key
+    kp = ops.pack_k_per_channel((rnd(B, Hkv, t_vis, 128) * f).to(dtype).cuda(), 32, 4)
+    vp = ops.pack_v_per_token(rnd(B, Hkv, t_vis, 128).to(dtype).cuda(), 32, 4)
+    fp = lambda s: (rnd(B, Hkv, before + L, 128) * s).to(dtype).cuda()
+    return (rnd(B, L, Hq, 128) * query).to(dtype).cuda(), kp, vp, fp(f), fp(1.0)
+
+
+@pytest.mark.parametrize("key,query", [(1e-2, 30.0), (1e-3, 300.0), (2e-4, 1500.0), (300.0, 1e-3), (2e-4, 1.0), (300.0, 1e-2)])
+@pytest.mark.parametrize("L", [1, 4])
+def test_small_keys_and_large_queries_of_few_rows(L, key, query):
+    """fp16 far from one: the product of a query and a scale in two terms keeps 22 bits wherever in the range they lie."""
+    q, kp, vp, k_fp, v_fp = sized(2, 8, 2, L, 256, 20, HALF, key, query, seed=L)
+    check(q, kp, vp, k_fp, v_fp, 20)
+    q[..., ::3] *= 2.0 ** -9                             # channels far below the row's largest
+    check(q, kp, vp, k_fp, v_fp, 20)
+
+
+def test_ends_of_fp16_of_few_rows():
+    """Scales from subnormal to the largest number beside one another, queries at either end."""
+    q, kp, vp, k_fp, v_fp = sized(1, 8, 2, 2, 128, 20, HALF, 1.0, 1.0)
+    for g, s in enumerate((6e-8, 6.2e-5, 1.0, 65504.0)):
+        kp[1][..., g] = s * torch.randint(1, 2, (1, 2, 128), device="cuda")
+        kp[2][..., g] = 0
+    q[:] = 0
+    q[..., 5], q[..., 9] = 6e-8, -6e-8                   # scores of 65504 * 15 * 2^-24 at most
+    check(q, kp, vp, k_fp, v_fp, 20)
+    kp[1][..., 2:] = 0
+    q[..., 5], q[..., 9] = 60000.0, 2.0                  # of 6e4 * 15 * 2^-14
+    check(q, kp, vp, k_fp * 1e-5, v_fp, 20)
