@@ -128,3 +128,11 @@ def test_ends_of_fp16_of_few_rows():
     kp[1][..., 2:] = 0
     q[..., 5], q[..., 9] = 60000.0, 2.0                  # of 6e4 * 15 * 2^-14
     check(q, kp, vp, k_fp * 1e-5, v_fp, 20)
+
+
+@pytest.mark.parametrize("key,query", [(1e-2, 30.0), (1e-3, 300.0), (2e-4, 1500.0), (300.0, 1e-3), (2e-4, 1.0), (300.0, 1e-2)])
+@pytest.mark.parametrize("L", [24, 390])
+def test_small_keys_and_large_queries(L, key, query):
+    """The same for the tiles of the tensor core, with key tiles unpacked in the kernel and once before it."""
+    q, kp, vp, k_fp, v_fp = sized(1, 8, 2, L, 256, 20, HALF, key, query, seed=L)
+    check(q, kp, vp, k_fp, v_fp, 20)
