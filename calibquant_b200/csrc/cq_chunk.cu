@@ -791,8 +791,9 @@ static int launch_attn(const CUtensorMap& tm, const AttnParams& p, const Plan& p
 
 static bool attn_valid(const cq_chunk_args* a) {
   if (!valid(a) || !a->out || !aligned16(a->out) || !a->v_fp || !aligned16(a->v_fp)) return false;
+  const int extent[3] = {a->batch, a->q_len, a->n_q_heads};
   for (int i = 0; i < 3; ++i)
-    if (a->out_strides[i] % 8) return false;
+    if (a->out_strides[i] % 8 || (extent[i] > 1 && a->out_strides[i] <= 0)) return false;
   return !a->t_vis || (a->v_code && a->v_scale && a->v_mn && aligned16(a->v_code) && aligned16(a->v_scale) && aligned16(a->v_mn));
 }
 static bool attn_supported(const cq_chunk_args* a) {
