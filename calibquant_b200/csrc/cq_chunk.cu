@@ -11,13 +11,13 @@
 //                    buffers of keys (two terms each) and one of values, two where there is one query tile; full-precision
 //                    rows into the same layout
 //   warp 16          issues the products
-// S = Q K^T with packed keys as two 16-bit terms (their sum is scale * code + minimum exactly), so scores carry no rounding but
-// that of fp32 sums; O += P V with P in tensor memory.  S_A [0,128) S_B [128,256) O_A [256,384) O_B [384,512) TMEM columns.
+// S = Q K^T with packed keys as two 16-bit terms, whose sum is scale * code + minimum but for what split_pair says, so scores carry hardly a
+// rounding but that of fp32 sums; O += P V with P in tensor memory.  S_A [0,128) S_B [128,256) O_A [256,384) O_B [384,512) TMEM columns.
 // Key tiles that six or more row blocks would unpack are unpacked once, by chunk_unpack_kernel, into images of the shared-memory tiles (96 KB per
 // 128 visual tokens), which the attention then loads in bulk.
 //
 // What bounds it.  With images: 48 products of 64 cycles a key tile and pair of query tiles; measured 4100 cycles (8 x 1024 queries on
-// 3328 + 1280 keys, bfloat16, at 1.75 GHz under the power cap: 588 us, and 52 for the images at 4.5 TB/s).  What is above is the chain of one query tile
+// 3328 + 1280 keys, bfloat16, at 1.75 GHz under the power cap: 596 us, and 56 for the images at 4.2 TB/s; 684 to 690 in a row).  What is above is the chain of one query tile
 // (S -> softmax, 1900 cycles -> P V -> next S) that the other one does not cover.  Without images: the same chain beside warps that unpack
 // (39 instructions per word of eight keys, twice rounded), and instructions that do not come in time: with the two halves of a row's scores as
 // a loop instead of two copies of the code 73.5 -> 66 us (37 queries of four padded requests on 6656 tokens), 112 -> 98 (40 of 16 on

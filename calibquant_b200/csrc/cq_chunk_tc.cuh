@@ -54,8 +54,9 @@ __device__ __forceinline__ void add_pair(float& s0, float& s1, float a0, float a
       : "+f"(s0), "+f"(s1) : "f"(a0), "f"(a1));
 }
 
-// Two numbers as 16-bit pairs whose sum they are: hi is the number cut off, lo the rest rounded.  A value scale * code + minimum has
-// up to 16 bits in all cases but those where the minimum is hundreds of scales away from zero, and is exact then.
+// Two numbers as 16-bit pairs whose sum they are: hi is the number cut off, lo the rest rounded.  bfloat16: a value scale * code + minimum of
+// up to 16 bits is exact, which it has unless the minimum is hundreds of scales away from zero; others are off by 2^-16 of themselves at most.
+// fp16: 22 bits, but none below 2^-24, so that a value is off by 2^-25 at most: 2^-15 of a key of 2^-10, nothing of one from 2^-3 on.
 template <bool BF16>
 __device__ __forceinline__ void split_pair(float a, float b, uint32_t& hi, uint32_t& lo) {
   if (BF16) {

@@ -4,8 +4,9 @@
 // Selection: the weights become integers whose order is the weights' order (the bits of the number, all of them flipped for a negative one, the
 // sign bit for any other; -0 as +0, NaN above infinity).  Up to a thread's number of units are ranked by counting those above; of more, the
 // value of the keep-th largest is found eight bits at a time from a histogram of the units that agree with it so far, until all that
-// agree stay.  A unit stays if it is above that value, or equal to it and among the first of the equal ones that fill the rest.  A group's weight is the sum of its 32 weights in 64 bits, so that the order of the additions decides
-// no border.  Only counts are added atomically: the result depends on nothing but the weights.
+// agree stay.  A unit stays if it is above that value, or equal to it and among the first of the equal ones that fill the rest.  A group's weight is the sum of its 32 weights in 64
+// bits, in their order: exact, whatever the order, as long as the largest of them is at most 2^24 times the smallest one above zero.  Only counts are
+// added atomically: the result depends on nothing but the weights.
 // Bound: HBM, and before it the selection, which every CTA waits for.  A group's keys are 16 bytes of 128 rows: a quarter of the groups kept
 // reads two thirds of the rows' 64-byte pieces and all of the scales, 261 MB for 8 x 8 heads of 32 768 tokens (40 us at the copy rate, 62
 // measured; four CTAs an SM, each selecting for itself: 82).  16 x 8 heads of 4099 full-precision tokens, a quarter kept: 35 us, 4 TB/s (31 behind one another).

@@ -1,7 +1,7 @@
 // How much attention the queries of a chunk paid to each key: column sums of exp(score - log-sum-exp), on tcgen05.
 //
 // The scores are formed the other way round than for the attention, S^T = K Q^T: a TMEM lane per key, so that a key's sum over the queries
-// stays in one thread and no exchange is needed.  A CTA holds two key tiles of 128 (packed keys as two 16-bit terms, exact as there) and
+// stays in one thread and no exchange is needed.  A CTA holds two key tiles of 128 (packed keys as two 16-bit terms, as there) and
 // goes over the query rows of their KV head in blocks of NB.  Roles:
 //   warps 0-15  the key tiles, once; then the sums: a thread has a key and every other 32 (16) of a block's rows, warps 0-3, 8-11 tile 0,
 //               4-7, 12-15 tile 1
@@ -10,8 +10,8 @@
 // A block is the query heads of the KV head for as many queries as NB rows hold: a row of a block is the same head for every block.
 // Bound: 64 products of 64 cycles per pair of packed key tiles and 256 rows, and the 2 x 128 x 128 exponentials of a block of 128 rows, which
 // take the special-function units as long as its products take the tensor cores (2048 cycles) and run beside them; 2750 cycles a block
-// measured.  8 x 1024 queries on 3328 + 1280 keys, bfloat16: 422 us apart, 460 in a row of launches under the power cap, of which 10 % are
-// the CTAs' starts (key tiles, first block).  Half the products: 407, no exponentials: 385.  Keys in tensor memory as the products' other
+// measured.  8 x 1024 queries on 3328 + 1280 keys, bfloat16: 455 us alone, 460 in a row of launches, of which 10 % are
+// the CTAs' starts (key tiles, first block).  Trials, on a GPU where this form took 422: half the products 407, no exponentials 385.  Keys in tensor memory as the products' other
 // operand (nothing but queries read from shared memory), four query slots, a quarter of the exponentials by a polynomial: 410 to 424, and 4 us
 // more for 20 to 100 queries, whose key tiles go through shared memory first.  Scores in halves of 64 rows: 474.
 // The rows' log-sum-exp come by cp.async one chunk ahead, both key tiles are requested before one is unpacked: 41 -> 39 us (2 x 517

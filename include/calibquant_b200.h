@@ -505,8 +505,9 @@ int cq_qjl_gqa_score(const uint8_t* key_quant, const uint8_t* key_outlier_quant,
  * t <= t_fp - q_len + i, the values of a packed operand being scale * code + mn:
  *   s[i,k] = q_i . K_k / sqrt(128) + mask[k],   lse_i = log sum_k exp(s[i,k]),   out_i = sum_k exp(s[i,k] - lse_i) V_k
  * A key whose mask is -infinity takes no part, whatever its key and value hold; a row without keys gives out 0, lse -infinity.
- * The scores are exact but for their fp32 sums (packed keys are multiplied as two terms), values and probabilities are rounded to
- * `dtype` for the second product.  No calibration of logits (calibrate = 0 of cq_decode_attn).
+ * The scores are those of fp32 sums: packed keys are multiplied as two 16-bit terms, which hold scale * code + mn but for 2^-16 of it in
+ * bfloat16 (nothing where it has 16 bits) and 2^-25 in fp16.  Values and probabilities are rounded to `dtype` for the second product.  No
+ * calibration of logits (calibrate = 0 of cq_decode_attn).
  *   q, out  element (b,i,h,d) at base + b*strides[0] + i*strides[1] + h*strides[2] + d (strides in elements, multiples of 8, above
  *           zero where the extent is above one)
  *   lse     fp32 [B,Hq,q_len], or NULL
@@ -548,14 +549,14 @@ int cq_chunk_attn(const cq_chunk_args* args, void* workspace, size_t workspace_b
  *   args       as for cq_chunk_attn; v_code .. v_mn, v_fp, out are not used, lse is read
  *   w_vis      fp32 [B,Hkv,t_vis]; w_fp fp32 [B,Hkv,w_capacity] with w_capacity >= t_fp: rows of keys that are not live keep w_in
  *   *_in       the same shapes, may be the outputs themselves, or NULL: zeros
- * Sums are fp32, in an order that depends on the sizes alone.
+ * Sums are fp32, in an order that depends on the sizes alone; an exponential below 2^-126 counts as zero.
  */
 size_t cq_key_weights_workspace_bytes(const cq_chunk_args* args, int64_t w_capacity);
 int cq_key_weights(const cq_chunk_args* args, const float* w_vis_in, const float* w_fp_in, float* w_vis, float* w_fp,
                    int64_t w_capacity, void* workspace, size_t workspace_bytes, void* stream);
 
 /*
- * cq_evict_groups: per (batch row, KV head) the `keep` groups of 32 visual tokens with the largest sum of weights (64-bit sums; ties to
+ * cq_evict_groups: per (batch row, KV head) the `keep` groups of 32 visual tokens with the largest sum of weights (64-bit sums in token order; ties to
  * the lowest index; NaN counts as the largest) stay, in their order, as they are packed.
  *   in   K code [B,H,D,t_vis*bits/32], scale, mn [B,H,D,t_vis/32]; V code [B,H,t_vis,D*bits/32], scale, mn [B,H,t_vis,4]; weights
  *        fp32 [B,H,t_vis]
